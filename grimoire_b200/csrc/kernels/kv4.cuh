@@ -1,0 +1,41 @@
+// The 4-bit KV page, shared by the kernels that write, read, weigh and move it (kv4.cu, kv4_attn.cu).
+//
+// A (page, kv head) record of 18 * D bytes holds 16 tokens:
+//   K codes [16][D / 2] | V codes [16][D / 2] | maxima [16][K, V][D / 32] bf16
+// Element d of a token's row is (code - 8) * maximum[(d / 4) % (D / 32)] / 7 with code = round(7 x / maximum) + 8 in 1..15,
+// element d in byte d / 2 (low half for even d).  A quantisation group is 32 elements: the quads (4 consecutive elements)
+// whose index has the same remainder mod D / 32.  Quads are dealt out because a 32-bit word of codes then holds exactly two
+// groups, one per 16-bit half, which is what the tensor-core operands of the attention kernel want: an operand register pairs
+// the same nibble of two words (or two tokens), so both of its elements share one maximum.
+#pragma once
+#include "common.cuh"
+
+namespace kv4 {
+
+constexpr int kPage = 16;
+
+template <int D>
+struct Geo {
+  static constexpr int kGroups = D / 32;             // maxima of a row
+  static constexpr int kRow = D / 2;                 // bytes of a token's codes (K or V)
+  static constexpr int kAmaxTok = 4 * kGroups;       // bytes of a token's maxima (K then V)
+  static constexpr int kV = kPage * kRow;            // offset of the V codes
+  static constexpr int kAmax = 2 * kPage * kRow;     // offset of the maxima
+  static constexpr int kRecord = kAmax + kPage * kAmaxTok;
+  static_assert(kRecord == 18 * D, "page record");
+};
+
+// Pages of one sequence.  A table entry outside [0, pages) maps nothing: its tokens do not exist for any reader or writer.
+struct Table {
+  const int* table;       // [slots][width]
+  int slots, width;       // rows, entries a row
+  long stride;            // entries between rows
+  int pages;              // pages in the pool
+};
+__device__ __forceinline__ int page_of(const Table& t, int slot, int index) {
+  if ((unsigned)slot >= (unsigned)t.slots || (unsigned)index >= (unsigned)t.width) return -1;
+  const int p = __ldg(t.table + (size_t)slot * t.stride + index);
+  return (unsigned)p < (unsigned)t.pages ? p : -1;
+}
+
+}  // namespace kv4

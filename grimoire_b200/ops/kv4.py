@@ -1,0 +1,332 @@
+"""KV cache in 4 bits: the pages of one layer, the calls that write and read them, attention over them, the attention weight
+that every cached token has drawn, and the cut of a cache to the tokens that drew the most (csrc/kernels/kv4.cu, kv4_attn.cu;
+CPU tensors run the fp32 forms of ``ops.ref``).
+
+A page record of 18 * D bytes holds 16 tokens of one kv head: 4-bit codes and one bf16 maximum per 32 elements, 4.5 bits an
+element against 8.25 of the int8 pages at head_dim 128.  Like the int8 pages they are addressed through a block table
+(int32 [slots][pages of a sequence], -1 where nothing is mapped).  A table entry outside the pool maps nothing: rows are not
+written there and keys there do not exist.
+
+Every call checks its arguments' types, shapes and devices on the host, works on the current stream of the tensors' device,
+takes its scratch from the caching allocator (so calls on several streams and captured graphs never share any), and does not
+synchronise.  Lengths, positions and tables are read on the device; values outside the table are ignored, never followed.
+"""
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass
+from typing import Optional
+
+import torch
+
+from .. import _native
+from . import ref
+from .core import PAGE, AttnGeom
+
+HEAD_DIMS = (64, 128, 256)
+MAX_GROUP = 16          # query heads of a kv head
+
+
+@dataclass
+class Kv4Layer:
+    """4-bit K / V pages of one layer: ``data`` uint8 [P][Hkv][18 * D]; ``mass`` (optional) fp32 [P][Hkv][16], the attention
+    weight drawn by every cached token."""
+
+    data: torch.Tensor
+    mass: Optional[torch.Tensor] = None
+
+    @staticmethod
+    def alloc(pages: int, Hkv: int, D: int, device, mass: bool = False) -> "Kv4Layer":
+        if D not in HEAD_DIMS:
+            raise ValueError(f"4-bit KV pages need head_dim in {HEAD_DIMS}, got {D}")
+        return Kv4Layer(torch.zeros(pages, Hkv, 18 * D, dtype=torch.uint8, device=device),
+                        torch.zeros(pages, Hkv, PAGE, dtype=torch.float32, device=device) if mass else None)
+
+    @property
+    def D(self) -> int:
+        return self.data.shape[2] // 18
+
+    def bytes_per_token(self) -> int:
+        Hkv, rec = self.data.shape[1], self.data.shape[2]
+        return Hkv * rec // PAGE + (4 * Hkv if self.mass is not None else 0)
+
+
+_lib = None
+
+
+def _cuda():
+    """The kernel library with the argument types of this module's entry points declared (numbers need no wrapping then)."""
+    global _lib
+    if _lib is None:
+        lib = _native.cuda()
+        p, i, l, f = ctypes.c_void_p, ctypes.c_int, ctypes.c_long, ctypes.c_float
+        lib.grm_kv4_append.argtypes = [p, p, p, p, l, l, p, p, p, i, i, l, i, i, i, i, i, p]
+        lib.grm_kv4_gather.argtypes = [p, p, i, i, l, i, p, p, p, p, l, l, l, l, i, i, i, i, i, p]
+        lib.grm_kv4_select.argtypes = [p, p, i, i, l, i, p, p, p, i, i, i, i, i, p]
+        lib.grm_kv4_compact.argtypes = [p, p, p, i, i, l, i, p, p, p, l, i, i, i, i, i, p]
+        lib.grm_kv4_attn_scratch.argtypes = [i, i, i, i, i]
+        lib.grm_kv4_attn_scratch.restype = l
+        lib.grm_kv4_attn.argtypes = [p, p, p, i, i, l, i, p, l, p, p, p, l, p, l, p, i, i, i, i, i, i, f, i, i, i, p]
+        _lib = lib
+    return _lib
+
+
+def _check(kv: Kv4Layer, block_table: torch.Tensor, *ints: Optional[torch.Tensor], what: str) -> None:
+    data, mass = kv.data, kv.mass
+    if data.dim() != 3 or data.dtype != torch.uint8 or not data.is_contiguous() or data.shape[2] not in (1152, 2304, 4608):
+        raise ValueError(f"{what}: data must be a contiguous uint8 [pages][kv heads][18 * head_dim] with head_dim in {HEAD_DIMS}")
+    if data.numel() == 0 or data.data_ptr() % 16:
+        raise ValueError(f"{what}: data must hold a page and start on a 16-byte boundary")
+    if mass is not None and (mass.dtype != torch.float32 or not mass.is_contiguous() or tuple(mass.shape) != (data.shape[0], data.shape[1], PAGE)
+                             or mass.device != data.device):
+        raise ValueError(f"{what}: mass must be a contiguous fp32 [pages][kv heads][16] on the cache's device")
+    if block_table.dim() != 2 or block_table.dtype != torch.int32 or (block_table.stride(1) != 1 and block_table.shape[1] > 1) or block_table.numel() == 0 or block_table.device != data.device:
+        raise ValueError(f"{what}: block_table must be a non-empty int32 [slots][pages] with contiguous rows on the cache's device")
+    for t in ints:
+        if t is not None and (t.dim() != 1 or t.dtype != torch.int32 or not t.is_contiguous() or t.device != data.device):
+            raise ValueError(f"{what}: rows, positions, slots and lengths must be contiguous int32 vectors on the cache's device")
+
+
+def _check_rows(t: torch.Tensor, kv: Kv4Layer, M: int, width: int, name: str, what: str) -> None:
+    if t.dim() != 2 or t.shape[0] != M or t.shape[1] != width or t.dtype != torch.bfloat16 or (t.stride(1) != 1 and width > 1) or t.device != kv.data.device:
+        raise ValueError(f"{what}: {name} must be bf16 [{M}][{width}] with contiguous rows on the cache's device")
+
+
+def _here(kv: Kv4Layer):
+    """Makes the cache's device the current one for the launch."""
+    return torch.cuda.device(kv.data.device)
+
+
+def _slots(block_table: torch.Tensor):
+    return block_table.data_ptr(), block_table.shape[0], block_table.shape[1], block_table.stride(0)
+
+
+def _ptr(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+# ---------------------------------------------------------------------------------------------
+# write and read back
+# ---------------------------------------------------------------------------------------------
+def kv4_append(kv: Kv4Layer, k: torch.Tensor, v: torch.Tensor, row_pos: torch.Tensor, row_seq: torch.Tensor, block_table: torch.Tensor) -> None:
+    """Quantise row m of ``k`` / ``v`` (bf16 [M][Hkv * D], after norm and RoPE) into position ``row_pos[m]`` of sequence
+    slot ``row_seq[m]``; its mass starts at zero.  Rows with a negative position or slot, or whose page is not mapped, are
+    skipped.  A position may come once per call.
+
+    Per group of 32 elements ``code = round(7 x / max|x|)``, ties to even, exactly as in 64-bit arithmetic.  A group with an
+    infinity or a NaN reads back as NaN."""
+    M, Hkv, D = k.shape[0], kv.data.shape[1], kv.D
+    _check(kv, block_table, row_pos, row_seq, what="kv4_append")
+    _check_rows(k, kv, M, Hkv * D, "k", "kv4_append")
+    _check_rows(v, kv, M, Hkv * D, "v", "kv4_append")
+    if row_pos.numel() != M or row_seq.numel() != M:
+        raise ValueError("kv4_append: row_pos and row_seq need an entry per row")
+    if M == 0:
+        return
+    if not kv.data.is_cuda:
+        codes, amax = ref.kv4_views(kv.data)
+        for m in range(M):
+            page, slot, ok = ref.kv4_place(block_table, int(row_seq[m]), row_pos[m: m + 1], kv.data.shape[0])
+            if bool(ok):
+                for which, x in ((0, k), (1, v)):
+                    c, a = ref.quant_kv4(x[m].reshape(Hkv, D))
+                    codes[page[0], :, which, slot[0]] = c[:, 0::2] | (c[:, 1::2] << 4)
+                    amax[page[0], :, slot[0], which] = a
+                if kv.mass is not None:
+                    kv.mass[page[0], :, slot[0]] = 0
+        return
+    vec = int((k.data_ptr() | v.data_ptr() | 2 * k.stride(0) | 2 * v.stride(0)) % 8 == 0)
+    with _here(kv):
+        code = _cuda().grm_kv4_append(kv.data.data_ptr(), _ptr(kv.mass), k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0), row_pos.data_ptr(),
+                                      row_seq.data_ptr(), *_slots(block_table), kv.data.shape[0], M, Hkv, D, vec, _native.stream_ptr())
+    _native.check(code, "kv4_append")
+
+
+def kv4_gather(kv: Kv4Layer, block_table: torch.Tensor, slots: Optional[torch.Tensor], lengths: Optional[torch.Tensor], out_k: torch.Tensor,
+               out_v: torch.Tensor) -> None:
+    """Dequantise the first ``min(lengths[i], T)`` cached tokens of sequence slot ``slots[i]`` into ``out_k[i]`` / ``out_v[i]``
+    (bf16 [S][T][Hkv * D], rounded once).  ``slots`` None: sequence i is row i of the table; ``lengths`` None: all T tokens.
+    Rows past a sequence's length, and those of pages that are not mapped, stay as they are."""
+    _check(kv, block_table, slots, lengths, what="kv4_gather")
+    P, Hkv, D = kv.data.shape[0], kv.data.shape[1], kv.D
+    for t in (out_k, out_v):
+        if t.dim() != 3 or t.dtype != torch.bfloat16 or t.shape[2] != Hkv * D or t.shape[:2] != out_k.shape[:2] or t.stride(2) != 1 or t.device != kv.data.device:
+            raise ValueError("kv4_gather: out_k / out_v must be bf16 [sequences][tokens][kv heads * head_dim] with contiguous rows on the cache's device")
+    S, T = out_k.shape[:2]
+    if (slots is None and S > block_table.shape[0]) or any(t is not None and t.numel() != S for t in (slots, lengths)):
+        raise ValueError("kv4_gather: slots and lengths need an entry per sequence")
+    if S > 65535:
+        raise ValueError("kv4_gather: at most 65535 sequences")
+    if S == 0 or T == 0:
+        return
+    if not kv.data.is_cuda:
+        for i in range(S):
+            n = max(0, T if lengths is None else min(T, int(lengths[i])))
+            t = torch.arange(n)
+            page, slot, ok = ref.kv4_place(block_table, i if slots is None else int(slots[i]), t, P)
+            for out, x in zip((out_k, out_v), ref.kv4_rows(kv.data, page, slot)):
+                out[i, :n][ok] = x[ok].reshape(-1, Hkv * D).to(torch.bfloat16)
+        return
+    align = out_k.data_ptr() | out_v.data_ptr()
+    for t in (out_k, out_v):
+        align |= 2 * t.stride(0) | 2 * t.stride(1)
+    with _here(kv):
+        code = _cuda().grm_kv4_gather(kv.data.data_ptr(), *_slots(block_table), P, _ptr(slots), _ptr(lengths), out_k.data_ptr(), out_v.data_ptr(),
+                                      out_k.stride(1), out_v.stride(1), out_k.stride(0), out_v.stride(0), S, T, Hkv, D, int(align % 16 == 0),
+                                      _native.stream_ptr())
+    _native.check(code, "kv4_gather")
+
+
+# ---------------------------------------------------------------------------------------------
+# attention
+# ---------------------------------------------------------------------------------------------
+def kv4_splits(max_len: int, rows: int, Hkv: int) -> int:
+    """How many CTAs share the keys of one (row, kv head)."""
+    pages = max(1, (max_len + PAGE - 1) // PAGE)
+    return max(1, min(64, pages // 8, 592 // max(1, rows * Hkv)))
+
+
+def kv4_attn(q: torch.Tensor, row_seq: torch.Tensor, row_pos: torch.Tensor, block_table: torch.Tensor, kv: Kv4Layer, geom: AttnGeom,
+             out: torch.Tensor, max_len: int, gate: Optional[torch.Tensor] = None, block: int = 1, observe: Optional[str] = None) -> torch.Tensor:
+    """Attention of M rows over the 4-bit pages: row m (bf16 [Hq * D], after norm and RoPE) of sequence slot ``row_seq[m]`` sees
+    the cached positions 0 .. ``row_pos[m]``, the last ``geom.window`` of them with a window, and leaves its output (bf16,
+    times sigmoid(``gate[m]``) with a gate) in ``out[m]``.  A row that sees no key (a negative position, no mapped page)
+    gives zeros.  ``max_len`` is the longest row's ``row_pos + 1`` as the host knows it: it sets how the keys are split, and
+    bounds the tokens that ``observe`` covers.
+
+    ``block`` > 1: every ``block`` consecutive rows belong to one sequence (the last rows of a prompt, a verify block).
+    ``observe``: "set" or "add" the softmax weight that every token drew from the rows of its sequence in this call, summed
+    over the rows and the query heads of a kv head, to ``kv.mass``; "set" covers all tokens up to the block's last position.
+    """
+    M, Hq, D, Hkv = q.shape[0], geom.Hq, geom.D, geom.Hkv
+    _check(kv, block_table, row_seq, row_pos, what="kv4_attn")
+    if kv.D != D or kv.data.shape[1] != Hkv:
+        raise ValueError(f"kv4_attn: the cache holds {kv.data.shape[1]} kv heads of {kv.D}, the geometry says {Hkv} of {D}")
+    if Hkv < 1 or Hq % Hkv or not 1 <= Hq // Hkv <= MAX_GROUP:
+        raise ValueError(f"kv4_attn: {Hq} query heads over {Hkv} kv heads: 1 to {MAX_GROUP} query heads a kv head are served")
+    _check_rows(q, kv, M, Hq * D, "q", "kv4_attn")
+    _check_rows(out, kv, M, Hq * D, "out", "kv4_attn")
+    if gate is not None:
+        _check_rows(gate, kv, M, Hq * D, "gate", "kv4_attn")
+    if row_seq.numel() != M or row_pos.numel() != M:
+        raise ValueError("kv4_attn: row_seq and row_pos need an entry per row")
+    if block < 1 or M % block or M > 65535:
+        raise ValueError(f"kv4_attn: {M} rows in blocks of {block}: a whole number of blocks and at most 65535 rows are served")
+    if observe not in (None, "set", "add"):
+        raise ValueError(f"kv4_attn: observe must be None, 'set' or 'add', got {observe!r}")
+    if observe is not None and kv.mass is None:
+        raise ValueError("kv4_attn: observe needs a cache with mass")
+    if max_len < 1:
+        raise ValueError("kv4_attn: max_len must be at least 1")
+    if M == 0:
+        return out
+    if not kv.data.is_cuda:
+        o, weights = ref.kv4_attention(q, row_seq, row_pos, block_table, kv.data, Hq, geom.scale, geom.window)
+        if gate is not None:
+            o = o * torch.sigmoid(gate.float())
+        out.copy_(o.to(out.dtype))
+        if observe is not None:
+            for slot in dict.fromkeys(row_seq[::block].tolist()):
+                rows = [m for m in range(M) if int(row_seq[m // block * block]) == slot]
+                n = max(weights[m].shape[1] for m in rows)
+                n = min(n, (max_len + PAGE - 1) // PAGE * PAGE)
+                w = torch.zeros(Hkv, n)
+                for m in rows:
+                    x = weights[m].reshape(Hkv, Hq // Hkv, -1).sum(1)[:, :n]
+                    w[:, : x.shape[1]] += x
+                page, place, ok = ref.kv4_place(block_table, int(slot), torch.arange(n), kv.data.shape[0])
+                old = kv.mass[page[ok], :, place[ok]] if observe == "add" else 0
+                kv.mass[page[ok], :, place[ok]] = old + w[:, ok].t()
+        return out
+    splits = kv4_splits(max_len, M, Hkv)
+    lib = _cuda()
+    mode = 0 if observe is None else (1 if observe == "set" else 2)
+    with _here(kv):
+        scratch = torch.empty(lib.grm_kv4_attn_scratch(M, Hq, D, splits, mode), dtype=torch.float32, device=kv.data.device)
+        code = lib.grm_kv4_attn(kv.data.data_ptr(), _ptr(kv.mass), *_slots(block_table), kv.data.shape[0], q.data_ptr(), q.stride(0), row_seq.data_ptr(),
+                                row_pos.data_ptr(), _ptr(gate), 0 if gate is None else gate.stride(0), out.data_ptr(), out.stride(0), scratch.data_ptr(),
+                                M, Hq, Hkv, D, splits, geom.window, geom.scale, block, mode, max_len, _native.stream_ptr())
+    _native.check(code, "kv4_attn")
+    return out
+
+
+# ---------------------------------------------------------------------------------------------
+# eviction
+# ---------------------------------------------------------------------------------------------
+def kv4_select(kv: Kv4Layer, slots: Optional[torch.Tensor], lengths: torch.Tensor, block_table: torch.Tensor, keep: int, recent: int,
+               sink: int = 0) -> torch.Tensor:
+    """Which tokens stay when sequence ``slots[i]`` of ``lengths[i]`` cached tokens is cut to ``keep``: the first ``sink``, the
+    last ``recent`` and, per kv head, those of the rest with the most mass (ties to the earlier token; NaN and tokens without
+    a page come last).  Returns int32 [S][Hkv][keep], positions in ascending order, -1 behind the last one of a sequence
+    that is not longer than ``keep``."""
+    _check(kv, block_table, slots, lengths, what="kv4_select")
+    S, Hkv = lengths.numel(), kv.data.shape[1]
+    if kv.mass is None:
+        raise ValueError("kv4_select needs a cache with mass")
+    if keep < 1 or recent < 0 or sink < 0 or recent + sink > keep:
+        raise ValueError(f"kv4_select: keep {keep} >= 1, recent {recent} and sink {sink} >= 0 and recent + sink <= keep are wanted")
+    if (slots is None and S > block_table.shape[0]) or (slots is not None and slots.numel() != S):
+        raise ValueError("kv4_select: slots and lengths need an entry per sequence")
+    if S > 65535:
+        raise ValueError("kv4_select: at most 65535 sequences")
+    idx = torch.empty(S, Hkv, keep, dtype=torch.int32, device=kv.data.device)
+    if S == 0:
+        return idx
+    if not kv.data.is_cuda:
+        idx.fill_(-1)
+        for i in range(S):
+            n = max(0, min(int(lengths[i]), block_table.shape[1] * PAGE))
+            t = torch.arange(n)
+            page, place, ok = ref.kv4_place(block_table, i if slots is None else int(slots[i]), t, kv.data.shape[0])
+            must = (t < sink) | (t >= n - recent)
+            for h in range(Hkv):
+                m = kv.mass[page, h, place]
+                last = ~ok | torch.isnan(m)                                   # three keys, the least significant first: a stable sort each
+                order = torch.sort(m.masked_fill(last, 0), descending=True, stable=True).indices
+                order = order[torch.sort(last[order].int(), stable=True).indices]
+                order = order[torch.sort((~must[order]).int(), stable=True).indices]
+                got = order[:keep].sort().values
+                idx[i, h, : got.numel()] = got.to(torch.int32)
+        return idx
+    with _here(kv):
+        code = _cuda().grm_kv4_select(kv.mass.data_ptr(), *_slots(block_table), kv.data.shape[0], _ptr(slots), lengths.data_ptr(), idx.data_ptr(), S, Hkv,
+                                      keep, recent, sink, _native.stream_ptr())
+    _native.check(code, "kv4_select")
+    return idx
+
+
+def kv4_compact(kv: Kv4Layer, slots: Optional[torch.Tensor], idx: torch.Tensor, block_table: torch.Tensor, dst_table: torch.Tensor) -> None:
+    """Copy token ``idx[i][h][j]`` of sequence ``slots[i]`` (kv head h, codes, maxima and mass as they are) to place j of the
+    pages ``dst_table[i]`` (int32 [S][>= ceil(keep / 16)]).  The destination pages must not be among the sources: pages that
+    other sequences share stay intact, and the caller swaps the tables afterwards.  Places whose ``idx`` is -1 stay as they
+    are."""
+    _check(kv, block_table, slots, what="kv4_compact")
+    if idx.dim() != 3 or idx.dtype != torch.int32 or not idx.is_contiguous() or idx.shape[1] != kv.data.shape[1] or idx.device != kv.data.device:
+        raise ValueError("kv4_compact: idx must be a contiguous int32 [sequences][kv heads][keep] on the cache's device")
+    S, Hkv, keep = idx.shape
+    if dst_table.dim() != 2 or dst_table.dtype != torch.int32 or dst_table.shape[0] != S or dst_table.shape[1] * PAGE < keep or \
+            (dst_table.stride(1) != 1 and dst_table.shape[1] > 1) or dst_table.device != kv.data.device:
+        raise ValueError("kv4_compact: dst_table must be int32 [sequences][>= keep / 16 pages] with contiguous rows on the cache's device")
+    if (slots is None and S > block_table.shape[0]) or (slots is not None and slots.numel() != S):
+        raise ValueError("kv4_compact: slots needs an entry per sequence")
+    if S > 65535:
+        raise ValueError("kv4_compact: at most 65535 sequences")
+    if S == 0 or keep == 0:
+        return
+    if not kv.data.is_cuda:
+        codes, amax = ref.kv4_views(kv.data)
+        P = kv.data.shape[0]
+        for i in range(S):
+            to, place, into = ref.kv4_place(dst_table, i, torch.arange(keep), P)
+            for h in range(Hkv):
+                page, at, ok = ref.kv4_place(block_table, i if slots is None else int(slots[i]), idx[i, h], P)
+                ok = ok & into
+                a, b, c, d = page[ok], at[ok], to[ok], place[ok]
+                codes[c, h, :, d], amax[c, h, d] = codes[a, h, :, b], amax[a, h, b]
+                if kv.mass is not None:
+                    kv.mass[c, h, d] = kv.mass[a, h, b]
+        return
+    with _here(kv):
+        code = _cuda().grm_kv4_compact(kv.data.data_ptr(), _ptr(kv.mass), *_slots(block_table), kv.data.shape[0], _ptr(slots), idx.data_ptr(),
+                                       dst_table.data_ptr(), dst_table.stride(0), dst_table.shape[1], S, Hkv, kv.D, keep, _native.stream_ptr())
+    _native.check(code, "kv4_compact")

@@ -89,3 +89,69 @@ def argmax_lowest(logits: torch.Tensor) -> torch.Tensor:
 
 def softmax_scale(head_dim: int) -> float:
     return 1.0 / math.sqrt(head_dim)
+
+
+# ---------------------------------------------------------------------------------------------
+# 4-bit KV pages (layout: csrc/kernels/kv4.cuh)
+# ---------------------------------------------------------------------------------------------
+def quant_kv4(x: torch.Tensor):
+    """bf16 [..., D] -> (codes uint8 [..., D] in 1..15, maxima bf16 [..., D / 32]).  The group of element d is
+    (d / 4) % (D / 32); a group whose maximum is zero or not finite has codes of zero (8).  The factor 7 is split so that it
+    cannot overflow; numerator and denominator are exact."""
+    ng = x.shape[-1] // 32
+    quads = x.float().unflatten(-1, (8, ng, 4))
+    amax = quads.abs().amax(dim=(-3, -1))
+    ok = (amax > 0) & torch.isfinite(amax)
+    div = torch.where(ok, amax, torch.ones_like(amax))[..., None, :, None]
+    q = torch.where(ok[..., None, :, None], torch.round(0.875 * quads / (0.125 * div)), torch.zeros_like(quads))
+    return (q + 8).to(torch.uint8).flatten(-3), amax.to(torch.bfloat16)
+
+
+def kv4_views(data: torch.Tensor):
+    """(codes uint8 [P][Hkv][K, V][16][D / 2], maxima bf16 [P][Hkv][16][K, V][D / 32]): views of the page records."""
+    D = data.shape[-1] // 18
+    return (data[..., : 16 * D].unflatten(-1, (2, PAGE, D // 2)),
+            data[..., 16 * D:].view(torch.bfloat16).unflatten(-1, (PAGE, 2, D // 32)))
+
+
+def kv4_rows(data: torch.Tensor, page: torch.Tensor, slot: torch.Tensor):
+    """K, V of the cached tokens (page[i], slot[i]) as fp32 [n][Hkv][D]."""
+    codes, amax = kv4_views(data)
+    c, a = codes[page, :, :, slot], amax[page, :, slot].float()              # [n][Hkv][2][D/2], [n][Hkv][2][D/32]
+    q = torch.stack((c & 15, c >> 4), dim=-1).flatten(-2).float() - 8
+    x = (0.125 * q.unflatten(-1, (8, a.shape[-1], 4)) * a[..., None, :, None] / 7 * 8).flatten(-3)
+    return x[:, :, 0], x[:, :, 1]
+
+
+def kv4_place(block_table: torch.Tensor, slot: int, positions: torch.Tensor, pages: int):
+    """(page, place in the page, mapped) of positions of one sequence; a table entry outside [0, pages) maps nothing."""
+    inside = (positions >= 0) & (positions < block_table.shape[1] * PAGE)
+    if not 0 <= slot < block_table.shape[0]:
+        inside = torch.zeros_like(inside)
+        slot = 0
+    p = positions.clamp(0, block_table.shape[1] * PAGE - 1).long()
+    page = block_table[slot, p // PAGE].long()
+    ok = inside & (page >= 0) & (page < pages)
+    return page.clamp(0, pages - 1), p % PAGE, ok
+
+
+def kv4_attention(q, row_seq, row_pos, block_table, data, Hq: int, scale: float, window: int = 0):
+    """Attention of independent rows over the pages: (out fp32 [M][Hq * D], weights: list of fp32 [Hq][tokens])."""
+    P, Hkv, D = data.shape[0], data.shape[1], data.shape[2] // 18
+    M, G = q.shape[0], Hq // Hkv
+    out, weights = torch.zeros(M, Hq, D), []
+    for m in range(M):
+        n = max(0, min(int(row_pos[m]) + 1, block_table.shape[1] * PAGE))
+        t = torch.arange(n)
+        page, slot, ok = kv4_place(block_table, int(row_seq[m]), t, P)
+        if window > 0:
+            ok = ok & (t >= n - window)
+        w = torch.zeros(Hq, n)
+        if bool(ok.any()):
+            k, v = kv4_rows(data, page[ok], slot[ok])
+            s = torch.einsum("hgd,thd->hgt", q[m].float().reshape(Hkv, G, D), k) * scale
+            p = torch.softmax(s, dim=-1)
+            out[m] = torch.einsum("hgt,thd->hgd", p, v).reshape(Hq, D)
+            w[:, ok] = p.reshape(Hq, -1)
+        weights.append(w)
+    return out.reshape(M, Hq * D), weights
