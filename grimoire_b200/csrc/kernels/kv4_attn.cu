@@ -37,9 +37,43 @@ __device__ __forceinline__ int row_first(const AttnParams& p, int len) { return 
 
 template <int D>
 struct Ring {
-  static constexpr int kStages = D == 256 ? 3 : 4;
-  static constexpr int kBytes = kWarps * kStages * Geo<D>::kRecord;
+  static constexpr int kStages = D == 64 ? 3 : 2;        // of two page records each
+  static constexpr int kWarpBytes = kStages * 2 * Geo<D>::kRecord + 2 * 32 * 4 * Geo<D>::kGroups;
+  static constexpr int kBytes = kWarps * kWarpBytes;
 };
+
+template <int N>
+__device__ __forceinline__ void load_words(const uint8_t* src, uint32_t (&w)[N]) {
+  static_assert(N == 1 || N == 2 || N % 4 == 0, "");
+  if constexpr (N == 1) {
+    w[0] = *reinterpret_cast<const uint32_t*>(src);
+  } else if constexpr (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2*>(src);
+    w[0] = v.x; w[1] = v.y;
+  } else {
+#pragma unroll
+    for (int j = 0; j < N / 4; ++j) {
+      const uint4 v = *reinterpret_cast<const uint4*>(src + 16 * j);
+      w[4 * j] = v.x; w[4 * j + 1] = v.y; w[4 * j + 2] = v.z; w[4 * j + 3] = v.w;
+    }
+  }
+}
+template <int N>
+__device__ __forceinline__ void load_floats(const float* src, float (&f)[N]) {
+  uint32_t w[N];
+  load_words<N>(reinterpret_cast<const uint8_t*>(src), w);
+#pragma unroll
+  for (int i = 0; i < N; ++i) f[i] = __uint_as_float(w[i]);
+}
+template <int N>
+__device__ __forceinline__ void store_floats(float* dst, const float (&f)[N]) {
+  if constexpr (N == 2) {
+    *reinterpret_cast<float2*>(dst) = make_float2(f[0], f[1]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N / 4; ++j) *reinterpret_cast<float4*>(dst + 4 * j) = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
+  }
+}
 
 __device__ __forceinline__ float deq(const uint8_t* row, const unsigned short* am, int d, int groups) {
   const int c = (row[d >> 1] >> (4 * (d & 1))) & 15;
@@ -56,6 +90,11 @@ __device__ __forceinline__ uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
   asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
   return d;
 }
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
 __device__ __forceinline__ float exp2_fast(float x) {         // 2 ulp; results below 2^-126 are zero
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -67,9 +106,9 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
   attn_mma::mma_f16_16816(d, a0, a1, a2, a3, b0, b1);
 }
 
-// Place of token column n (of 8-token tile b) in its page: the columns that lane t of a quad owns in the accumulator fragment
-// (2t, 2t + 1) are the tokens t and 4 + (t ^ 1) of the tile, so that neighbouring lanes read rows of different parity and the
-// 64-byte rows of a 128-element head meet no bank conflict as the K operand.
+// Place of token n (of 8-token tile b) of an operand in its page: n = 2t and 2t + 1, the pair of a lane in the V operand, are the
+// tokens t and 4 + (t ^ 1), so that neighbouring lanes read rows of different parity and the 64-byte rows of a 128-element head
+// meet no bank conflict as the K operand and two-way ones as the V operand.
 __device__ __forceinline__ int tok_of(int b, int n) { return 8 * b + ((n & 1) ? 4 + ((n >> 1) ^ 1) : (n >> 1)); }
 
 // The codes of a 16-bit half word, two words at once (two tokens, or two places of a row): element i of the result holds
@@ -90,19 +129,21 @@ __device__ __forceinline__ float exp2_pos(int e) { return __uint_as_float((uint3
 
 // Attention of up to 8 * HH (row, head) pairs of one kv head over one split of the sequence's pages.
 //
-// Bound by the cache's bytes (18 D per 16 tokens and kv head) and, close behind, by issue slots: one warp and page has to take
-// less than four times the ~100 cycles in which an SM receives the record.  Hence
-//   * a warp owns whole pages; each is ONE bulk copy (the record is contiguous) into a per-warp ring of kStages;
-//   * S[pair][token] = Q K^T with the pairs as MMA rows and the codes, as the fp16 integers that they are, as the column
-//     operand.  q is scaled by a power of two to fill fp16's range (bf16 has fewer bits: exact); a quantisation group is two
-//     k-steps whose sum is scaled by the group's maximum in fp32;
-//   * the accumulator fragment of S IS the column operand of O^T[dim][pair] += V^T[dim][token] P^T[token][pair]: no shuffle, and
-//     8 pairs fill the MMA's 8 columns.  P is scaled by the token's V maximum before it is rounded to fp16 (11 bits, on top of
-//     the output's 8); a running power of two keeps the largest maximum seen at the top of fp16's range, whatever the values'
-//     magnitude.
+// Bound by the cache's bytes (18 D per 16 tokens and kv head) and, close behind, by issue slots (a record has to cost a warp less
+// than four times the ~100 cycles in which an SM receives it), of them most by the integer pipe that unpacks the codes.  Hence
+//   * a warp owns steps of two pages (32 tokens); a page is ONE bulk copy (the record is contiguous) into a per-warp ring;
+//   * S^T[token][pair] = K Q^T with the codes, as the fp16 integers that they are, as the MMA's row operand: 16 tokens fill its
+//     rows and 8 pairs its columns.  q is scaled by a power of two to fill fp16's range (bf16 has fewer bits: exact); a
+//     quantisation group is two k-steps whose sum is scaled by the group's maximum in fp32;
+//   * O^T[dim][pair] += V^T[dim][token] P^T[token][pair].  P is multiplied by the token's V maximum in fp32, rounded to fp16
+//     (11 bits, against the output's 8) and transposed from the accumulator's layout to the column operand's by one movmatrix
+//     per 8 tokens; a running power of two keeps the largest product at the top of fp16's range, whatever the values'
+//     magnitude.  (Rounding P first and multiplying in fp16 saves 14 instructions a page and loses tokens whose values are
+//     2^-24 of the largest ones.)
+//   * the maxima are unpacked once a step, a token per lane, and handed round through shared memory.
 // Softmax statistics, scores and outputs are fp32.
 template <int D, int HH>
-__global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) attn_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(kThreads, HH == 2 ? 3 : (D == 256 ? 3 : 4)) attn_kernel(const AttnParams p) {
   using Gm = Geo<D>;
   constexpr int NG = Gm::kGroups, WT = D / 64, PP = 8 * HH;
   constexpr int kStages = Ring<D>::kStages;
@@ -133,46 +174,48 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) attn_kernel(const 
   const int page_lo = len_hi > 0 ? first_lo / kPage : 0, page_hi = (len_hi + kPage - 1) / kPage;
   const int pps = (page_hi - page_lo + nsplit - 1) / nsplit;
   const int pbeg = page_lo + split * pps, pend = min(pbeg + pps, page_hi);
-  const int n_it = pbeg + warp < pend ? (pend - pbeg - warp + kWarps - 1) / kWarps : 0;      // pages of this warp
+  const int n_it = pbeg + 2 * warp < pend ? (pend - pbeg - 2 * warp + 2 * kWarps - 1) / (2 * kWarps) : 0;      // steps of two pages of this warp
 
   // ---- ring ----
-  uint8_t* ring = smem + (size_t)warp * kStages * Gm::kRecord;
+  uint8_t* ring = smem + (size_t)warp * Ring<D>::kWarpBytes;
+  float* am_k = reinterpret_cast<float*>(ring + kStages * 2 * Gm::kRecord);                  // [32 tokens][NG]
+  float* am_v = am_k + 32 * NG;                                                              // [32 tokens][NG]
   if (lane == 0) {
 #pragma unroll
     for (int s = 0; s < kStages; ++s) mbar_init(&bars[warp][s], 1);
     mbar_fence_init();
   }
   __syncwarp();
-  auto load_ids = [&](int base) { return base + lane < n_it ? page_of(p.t, slot, pbeg + warp + kWarps * (base + lane)) : -1; };
-  int ids = load_ids(0), ids_next = load_ids(32);        // pages of iterations 32 i + lane and 32 (i + 1) + lane
-  auto issue = [&](int it, int id) {
+  // page ids of 16 steps, a lane each; -1: not there
+  auto load_ids = [&](int base) {
+    const int pg = pbeg + 2 * (warp + kWarps * (base + (lane >> 1))) + (lane & 1);
+    return pg < pend ? page_of(p.t, slot, pg) : -1;
+  };
+  int ids = load_ids(0), ids_next = load_ids(16);
+  auto issue = [&](int it, int id0, int id1) {
     if (lane == 0) {
       uint64_t* bar = &bars[warp][it % kStages];
-      if (id >= 0) {
-        mbar_expect_tx(bar, Gm::kRecord);
-        bulk_load(ring + (it % kStages) * Gm::kRecord, p.data + ((size_t)id * p.Hkv + kvh) * Gm::kRecord, Gm::kRecord, bar);
-      } else {
-        mbar_arrive(bar);
-      }
+      uint8_t* dst = ring + (it % kStages) * 2 * Gm::kRecord;
+      mbar_expect_tx(bar, (id0 >= 0 ? Gm::kRecord : 0) + (id1 >= 0 ? Gm::kRecord : 0));
+      if (id0 >= 0) bulk_load(dst, p.data + ((size_t)id0 * p.Hkv + kvh) * Gm::kRecord, Gm::kRecord, bar);
+      if (id1 >= 0) bulk_load(dst + Gm::kRecord, p.data + ((size_t)id1 * p.Hkv + kvh) * Gm::kRecord, Gm::kRecord, bar);
     }
   };
 #pragma unroll
   for (int s = 0; s < kStages; ++s)
-    if (s < n_it) issue(s, __shfl_sync(0xffffffffu, ids, s));
+    if (s < n_it) issue(s, __shfl_sync(0xffffffffu, ids, 2 * s), __shfl_sync(0xffffffffu, ids, 2 * s + 1));
 
-  // ---- q: row operands of S for the pairs g and g + 8 ----
+  // ---- q: column operands of S^T for the pairs g and g + 8 ----
   // k-step (group gi = 2 w + half, odd): the words w and w + NG / 2 of lane t's NG words, nibbles odd and odd + 2
-  uint32_t qa[HH][NG][2][2];
-  float fh[HH], m[HH], l[HH];
-  int lim[HH], low[HH];
+  uint32_t qb[HH][NG][2][2];
+  float fh[HH][2], m[HH][2], l[HH][2];                   // of the pairs 2 t, 2 t + 1 (+ 8 x)
+  int lim[HH][2], low[HH][2];
 #pragma unroll
   for (int x = 0; x < HH; ++x) {
     const int pr = g + 8 * x;
     const bool live = pr < np;
     const int row = row0 + (live ? pr / nh : 0), head = kvh * p.G + head0 + (live ? pr % nh : 0);
-    lim[x] = live ? row_len(p, row) : 0;
-    low[x] = row_first(p, lim[x]);
-    m[x] = -INFINITY; l[x] = 0.f;
+    const int seen = live ? row_len(p, row) : 0;
     const unsigned short* src = reinterpret_cast<const unsigned short*>(p.q) + (size_t)row * p.ld_q + (size_t)head * D;
     uint2 raw[NG][2];
     uint32_t mx = 0;
@@ -190,8 +233,16 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) attn_kernel(const 
     mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
     mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
     const int e = max((int)(mx >> 7), 14);               // biased exponent of the largest magnitude
-    const float up = e == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)(268 - e) << 23);   // 2^14 / 2^(e - 127)
-    fh[x] = p.scale_log2 * (1.f / 7.f / 16384.f) * exp2_pos(min(e - 127, 127));                              // 1 / up
+    float up = e == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)(268 - e) << 23);   // 2^14 / 2^(e - 127)
+    up = p.scale_log2 < 0.f ? -up : up;                  // the factor of s is positive, so that its maximum is s's maximum
+    const float f = fmaxf(fabsf(p.scale_log2) * (1.f / 7.f / 16384.f) * exp2_pos(min(e - 127, 127)), 1e-37f);       // scale / 7 / up
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      fh[x][j] = __shfl_sync(0xffffffffu, f, 8 * t + 4 * j);
+      lim[x][j] = __shfl_sync(0xffffffffu, seen, 8 * t + 4 * j);
+      low[x][j] = row_first(p, lim[x][j]);
+      m[x][j] = -INFINITY; l[x][j] = 0.f;
+    }
 #pragma unroll
     for (int gi = 0; gi < NG; ++gi) {
       float a[4], b[4];
@@ -202,7 +253,7 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) attn_kernel(const 
 #pragma unroll
       for (int odd = 0; odd < 2; ++odd)
 #pragma unroll
-        for (int j = 0; j < 2; ++j) qa[x][gi][odd][j] = attn_mma::pack_f16x2(a[odd + 2 * j], b[odd + 2 * j]);
+        for (int j = 0; j < 2; ++j) qb[x][gi][odd][j] = attn_mma::pack_f16x2(a[odd + 2 * j], b[odd + 2 * j]);
     }
   }
 
@@ -214,206 +265,195 @@ __global__ void __launch_bounds__(kThreads, D == 256 ? 2 : 3) attn_kernel(const 
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[x][gi][0][i] = acc[x][gi][1][i] = 0.f;
   int e_run = 14;                                        // biased exponent of the largest V maximum so far
+  float corr_e = 1.f;
   uint32_t limit = 4000000u;
 
-  auto page_work = [&](auto edge_tag, const uint8_t* rec, int tok0) {
-    constexpr bool kEdge = decltype(edge_tag)::value;    // some token of the page is hidden from some row
-    int tk[4];
+  auto step_work = [&](auto edge_tag, const uint8_t* rec, int tok0, int have) {
+    constexpr bool kEdge = decltype(edge_tag)::value;    // some token of the step is hidden from some row
+    // ---- maxima as fp32, a token per lane; those of V normalised ----
+    {
+      const int pg = lane >> 4, tok = tok_of((lane >> 3) & 1, lane & 7);
+      uint32_t w[NG];                                    // K: words 0 .. NG / 2 - 1, V: the others
+      const uint8_t* src = rec + pg * Gm::kRecord + Gm::kAmax + tok * Gm::kAmaxTok;
+      load_words<NG>(src, w);
+      if constexpr (kEdge) {                             // a token that no row sees must not set the scale of the values
+        const int at = tok0 + pg * kPage + tok;
+        if (at >= len_hi || at < first_lo || !(have >> pg & 1))
 #pragma unroll
-    for (int i = 0; i < 4; ++i) tk[i] = tok_of(i >> 1, 2 * t + (i & 1));
-    uint32_t am[4][NG];                                  // the lane's tokens: words 0 .. NG / 2 - 1 of K, then of V
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint8_t* src = rec + Gm::kAmax + tk[i] * Gm::kAmaxTok;
-      if constexpr (NG == 2) {
-        const uint2 v = *reinterpret_cast<const uint2*>(src);
-        am[i][0] = v.x; am[i][1] = v.y;
-      } else {
-#pragma unroll
-        for (int j = 0; j < NG / 4; ++j) {
-          const uint4 v = *reinterpret_cast<const uint4*>(src + 16 * j);
-          am[i][4 * j] = v.x; am[i][4 * j + 1] = v.y; am[i][4 * j + 2] = v.z; am[i][4 * j + 3] = v.w;
-        }
+          for (int j = 0; j < NG / 2; ++j) w[NG / 2 + j] = 0u;
       }
-    }
-    auto k_max = [&](int i, int gi) { return (gi & 1) ? bf16hi_to_f(am[i][gi / 2]) : bf16lo_to_f(am[i][gi / 2]); };
-    auto v_max = [&](int i, int gi) { return (gi & 1) ? bf16hi_to_f(am[i][NG / 2 + gi / 2]) : bf16lo_to_f(am[i][NG / 2 + gi / 2]); };
-    // ---- S ----
-    float s[HH][4];
+      float kf[NG];
 #pragma unroll
-    for (int x = 0; x < HH; ++x)
+      for (int j = 0; j < NG / 2; ++j) { kf[2 * j] = bf16lo_to_f(w[j]); kf[2 * j + 1] = bf16hi_to_f(w[j]); }
+      store_floats<NG>(am_k + lane * NG, kf);
+      uint32_t vm = w[NG / 2];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[x][i] = 0.f;
+      for (int j = 1; j < NG / 2; ++j) vm = __vmaxu2(vm, w[NG / 2 + j]);
+      int e = (int)(__reduce_max_sync(0xffffffffu, max(vm & 0xffffu, vm >> 16)) >> 7);
+      if (e >= 255) {                                    // a group that is not a number: it must not hide the others
+        e = 0;
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const uint8_t* src = rec + tok_of(b, g) * Gm::kRow + t * (D / 8);
-      uint32_t kw[NG];
-      if constexpr (NG == 2) {
-        const uint2 v = *reinterpret_cast<const uint2*>(src);
-        kw[0] = v.x; kw[1] = v.y;
-      } else {
-#pragma unroll
-        for (int j = 0; j < NG / 4; ++j) {
-          const uint4 v = *reinterpret_cast<const uint4*>(src + 16 * j);
-          kw[4 * j] = v.x; kw[4 * j + 1] = v.y; kw[4 * j + 2] = v.z; kw[4 * j + 3] = v.w;
+        for (int j = 0; j < NG / 2; ++j) {
+          const int lo = (int)(w[NG / 2 + j] >> 7) & 255, hi = (int)(w[NG / 2 + j] >> 23) & 255;
+          e = max(e, max(lo < 255 ? lo : 0, hi < 255 ? hi : 0));
         }
+        e = (int)__reduce_max_sync(0xffffffffu, (uint32_t)e);
+      }
+      corr_e = 1.f;
+      if (e > e_run) {
+        corr_e = e - e_run < 127 ? exp2_pos(e_run - e) : 0.f;
+        e_run = e;
+      }
+      const float vs = exp2_pos(127 - e_run);            // the largest maximum becomes 1 .. 2
+      float vf[NG];
+#pragma unroll
+      for (int j = 0; j < NG / 2; ++j) { vf[2 * j] = bf16lo_to_f(w[NG / 2 + j]) * vs; vf[2 * j + 1] = bf16hi_to_f(w[NG / 2 + j]) * vs; }
+      store_floats<NG>(am_v + lane * NG, vf);
+    }
+    __syncwarp();
+    // ---- S^T: rows are tokens, columns pairs; value i of a lane: page i >> 2, tile i >> 1 & 1 (token column g), pair 2 t + (i & 1) ----
+    float s[HH][8];
+#pragma unroll
+    for (int pg = 0; pg < 2; ++pg) {
+      uint32_t kw[2][NG];
+      float km[2][NG];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        load_words<NG>(rec + pg * Gm::kRecord + tok_of(b, g) * Gm::kRow + t * (D / 8), kw[b]);
+        load_floats<NG>(am_k + (16 * pg + 8 * b + g) * NG, km[b]);
       }
 #pragma unroll
       for (int gi = 0; gi < NG; ++gi) {
-        uint32_t nb[4];
-        nibbles(kw[gi / 2], kw[gi / 2 + NG / 2], gi & 1, nb);
-        float c[4] = {0.f, 0.f, 0.f, 0.f};
-        mma(c, qa[0][gi][0][0], HH == 2 ? qa[HH - 1][gi][0][0] : 0u, qa[0][gi][0][1], HH == 2 ? qa[HH - 1][gi][0][1] : 0u, nb[0], nb[2]);
-        mma(c, qa[0][gi][1][0], HH == 2 ? qa[HH - 1][gi][1][0] : 0u, qa[0][gi][1][1], HH == 2 ? qa[HH - 1][gi][1][1] : 0u, nb[1], nb[3]);
+        uint32_t n0[4], n1[4];
+        nibbles(kw[0][gi / 2], kw[0][gi / 2 + NG / 2], gi & 1, n0);
+        nibbles(kw[1][gi / 2], kw[1][gi / 2 + NG / 2], gi & 1, n1);
 #pragma unroll
-        for (int x = 0; x < HH; ++x)
+        for (int x = 0; x < HH; ++x) {
+          float c[4] = {0.f, 0.f, 0.f, 0.f};
+          mma(c, n0[0], n1[0], n0[2], n1[2], qb[x][gi][0][0], qb[x][gi][0][1]);
+          mma(c, n0[1], n1[1], n0[3], n1[3], qb[x][gi][1][0], qb[x][gi][1][1]);
 #pragma unroll
-          for (int j = 0; j < 2; ++j) s[x][2 * b + j] = fmaf(c[2 * x + j], k_max(2 * b + j, gi), s[x][2 * b + j]);
+          for (int i = 0; i < 4; ++i) s[x][4 * pg + i] = gi == 0 ? c[i] * km[i >> 1][gi] : fmaf(c[i], km[i >> 1][gi], s[x][4 * pg + i]);
+        }
       }
     }
-    if constexpr (kEdge) {                               // a token that no row sees must not set the scale of the values
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (tok0 + tk[i] >= len_hi || tok0 + tk[i] < first_lo)
-#pragma unroll
-          for (int j = 0; j < NG / 2; ++j) am[i][NG / 2 + j] = 0u;
-    }
-    // ---- running scale of the values: the exponent of the largest finite maximum ----
-    uint32_t vm = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-      for (int j = 0; j < NG / 2; ++j) vm = __vmaxu2(vm, am[i][NG / 2 + j]);
-    int e = (int)(max(vm & 0xffffu, vm >> 16) >> 7);
-    e = max(e, __shfl_xor_sync(0xffffffffu, e, 1));
-    e = max(e, __shfl_xor_sync(0xffffffffu, e, 2));
-    if (e >= 255) {                                      // a group that is not a number: it must not hide the others
-      e = 0;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int gi = 0; gi < NG; ++gi) {
-          const int one = (int)(__float_as_uint(v_max(i, gi)) >> 23);
-          e = one < 255 ? max(e, one) : e;
-        }
-      e = max(e, __shfl_xor_sync(0xffffffffu, e, 1));
-      e = max(e, __shfl_xor_sync(0xffffffffu, e, 2));
-    }
-    float corr_e = 1.f;
-    if (e > e_run) {
-      corr_e = e - e_run < 127 ? exp2_pos(e_run - e) : 0.f;
-      e_run = e;
-    }
-    const float vs = __uint_as_float((uint32_t)(268 - e_run) << 23);           // 2^14 / 2^(e_run - 127): the largest P is below 2^15
-    // ---- online softmax ----
-    float corr[HH];
+    // ---- online softmax; the maximum is kept in units of s, P comes with a factor of 2^14 ----
+    float corr[HH][2];
+    uint32_t hidden[HH];
     bool change = corr_e != 1.f;
 #pragma unroll
     for (int x = 0; x < HH; ++x) {
-      float mx = -INFINITY;
+      hidden[x] = 0u;
+      if constexpr (kEdge) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s[x][i] *= fh[x];
-        if (kEdge && (tok0 + tk[i] >= lim[x] || tok0 + tk[i] < low[x])) s[x][i] = -INFINITY;
-        mx = fmaxf(mx, s[x][i]);
+        for (int i = 0; i < 8; ++i) {
+          const int at = tok0 + (i >> 2) * kPage + tok_of((i >> 1) & 1, g);
+          if (at >= lim[x][i & 1] || at < low[x][i & 1] || !(have >> (i >> 2) & 1)) {
+            hidden[x] |= 1u << i;
+            s[x][i] = -INFINITY;
+          }
+        }
       }
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const float mn = fmaxf(m[x], mx), ref = mn == -INFINITY ? 0.f : mn;
-      corr[x] = exp2_fast(m[x] - ref);
-      change = change || corr[x] != 1.f;
-      m[x] = mn;
-      float sum = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s[x][i] = exp2_fast(s[x][i] - ref);
-        sum += s[x][i];
+      for (int j = 0; j < 2; ++j) {
+        float mx = fmaxf(fmaxf(s[x][j], s[x][2 + j]), fmaxf(s[x][4 + j], s[x][6 + j]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        const float mn = fmaxf(m[x][j], mx), ref = mn == -INFINITY ? 0.f : mn;
+        corr[x][j] = exp2_fast((m[x][j] - ref) * fh[x][j]);
+        change = change || corr[x][j] != 1.f;
+        m[x][j] = mn;
+        const float off = fmaf(-ref, fh[x][j], 14.f);
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[x][2 * i + j] = exp2_fast(fmaf(s[x][2 * i + j], fh[x][j], off));
+          sum += s[x][2 * i + j];
+        }
+        l[x][j] = fmaf(l[x][j], corr[x][j], sum);
+        corr[x][j] *= corr_e;
       }
-      l[x] = fmaf(l[x], corr[x], sum);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s[x][i] *= vs;
-      corr[x] *= corr_e;
     }
     if (__any_sync(0xffffffffu, change)) {
 #pragma unroll
-      for (int x = 0; x < HH; ++x) {
-        const float ca = __shfl_sync(0xffffffffu, corr[x], 8 * t), cb = __shfl_sync(0xffffffffu, corr[x], 8 * t + 4);
+      for (int x = 0; x < HH; ++x)
 #pragma unroll
         for (int gi = 0; gi < NG; ++gi)
 #pragma unroll
-          for (int ii = 0; ii < 2; ++ii) {
-            acc[x][gi][ii][0] *= ca; acc[x][gi][ii][1] *= cb; acc[x][gi][ii][2] *= ca; acc[x][gi][ii][3] *= cb;
-          }
-      }
+          for (int ii = 0; ii < 2; ++ii)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[x][gi][ii][i] *= corr[x][i & 1];
     }
     // ---- O^T += V^T P^T ----
-    uint32_t vw[4][WT];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint8_t* src = rec + Gm::kV + tk[i] * Gm::kRow + g * (4 * WT);
-      if constexpr (WT == 1) {
-        vw[i][0] = *reinterpret_cast<const uint32_t*>(src);
-      } else if constexpr (WT == 2) {
-        const uint2 v = *reinterpret_cast<const uint2*>(src);
-        vw[i][0] = v.x; vw[i][1] = v.y;
-      } else {
-        const uint4 v = *reinterpret_cast<const uint4*>(src);
-        vw[i][0] = v.x; vw[i][1] = v.y; vw[i][2] = v.z; vw[i][3] = v.w;
+    for (int pg = 0; pg < 2; ++pg) {
+      uint32_t vw[4][WT];
+      float vm[2][NG];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        load_words<WT>(rec + pg * Gm::kRecord + Gm::kV + tok_of(i >> 1, 2 * t + (i & 1)) * Gm::kRow + g * (4 * WT), vw[i]);
+#pragma unroll
+      for (int b = 0; b < 2; ++b) load_floats<NG>(am_v + (16 * pg + 8 * b + g) * NG, vm[b]);
+#pragma unroll
+      for (int gi = 0; gi < NG; ++gi) {
+        uint32_t pb[HH][2];
+#pragma unroll
+        for (int x = 0; x < HH; ++x)
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            pb[x][b] = attn_mma::pack_f16x2(s[x][4 * pg + 2 * b] * vm[b][gi], s[x][4 * pg + 2 * b + 1] * vm[b][gi]);
+            if constexpr (kEdge) {                       // 0 * NaN
+              const uint32_t hd = hidden[x] >> (4 * pg + 2 * b);
+              pb[x][b] &= ((hd & 1u) ? 0u : 0xffffu) | ((hd & 2u) ? 0u : 0xffff0000u);
+            }
+            pb[x][b] = transpose8x8(pb[x][b]);           // [token][pair] accumulator rows -> column operand
+          }
+        uint32_t v01[4], v23[4];
+        nibbles(vw[0][gi / 2], vw[1][gi / 2], gi & 1, v01);
+        nibbles(vw[2][gi / 2], vw[3][gi / 2], gi & 1, v23);
+#pragma unroll
+        for (int ii = 0; ii < 2; ++ii)
+#pragma unroll
+          for (int x = 0; x < HH; ++x) mma(acc[x][gi][ii], v01[2 * ii], v01[2 * ii + 1], v23[2 * ii], v23[2 * ii + 1], pb[x][0], pb[x][1]);
       }
-    }
-#pragma unroll
-    for (int gi = 0; gi < NG; ++gi) {
-      uint32_t pb[HH][2];
-#pragma unroll
-      for (int x = 0; x < HH; ++x) {
-        float v[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          v[i] = s[x][i] * v_max(i, gi);
-          if (kEdge && (tok0 + tk[i] >= lim[x] || tok0 + tk[i] < low[x])) v[i] = 0.f;      // 0 * NaN
-        }
-        pb[x][0] = attn_mma::pack_f16x2(v[0], v[1]);
-        pb[x][1] = attn_mma::pack_f16x2(v[2], v[3]);
-      }
-      uint32_t v01[4], v23[4];
-      nibbles(vw[0][gi / 2], vw[1][gi / 2], gi & 1, v01);
-      nibbles(vw[2][gi / 2], vw[3][gi / 2], gi & 1, v23);
-#pragma unroll
-      for (int ii = 0; ii < 2; ++ii)
-#pragma unroll
-        for (int x = 0; x < HH; ++x) mma(acc[x][gi][ii], v01[2 * ii], v01[2 * ii + 1], v23[2 * ii], v23[2 * ii + 1], pb[x][0], pb[x][1]);
     }
   };
 
   for (int it = 0; it < n_it; ++it) {
-    const int id = __shfl_sync(0xffffffffu, ids, it & 31);
-    const int stage = it % kStages, pg = pbeg + warp + kWarps * it;
+    const int id0 = __shfl_sync(0xffffffffu, ids, (2 * it) & 31), id1 = __shfl_sync(0xffffffffu, ids, (2 * it + 1) & 31);
+    const int stage = it % kStages, tok0 = (pbeg + 2 * (warp + kWarps * it)) * kPage;
     const bool here = __all_sync(0xffffffffu, mbar_wait(&bars[warp][stage], (uint32_t)(it / kStages) & 1u, p.status, 0x4b563400u | warp, limit));
     if (!here) limit = 16;                               // the call has failed: do not wait at length again
-    const int tok0 = pg * kPage;
-    if (id >= 0 && here) {
-      const uint8_t* rec = ring + stage * Gm::kRecord;
-      if (tok0 + kPage > len_lo || tok0 < first_hi) page_work(std::true_type{}, rec, tok0);
-      else page_work(std::false_type{}, rec, tok0);
+    const int have = here ? (id0 >= 0 ? 1 : 0) | (id1 >= 0 ? 2 : 0) : 0;
+    if (have) {
+      const uint8_t* rec = ring + stage * 2 * Gm::kRecord;
+      if (have != 3 || tok0 + 2 * kPage > len_lo || tok0 < first_hi) step_work(std::true_type{}, rec, tok0, have);
+      else step_work(std::false_type{}, rec, tok0, 3);
     }
     __syncwarp();
     const int nx = it + kStages;
-    if (nx < n_it) issue(nx, __shfl_sync(0xffffffffu, (nx >> 5) == (it >> 5) ? ids : ids_next, nx & 31));
-    if ((it & 31) == 31) {
+    if (nx < n_it) {
+      const int from = (nx >> 4) == (it >> 4) ? ids : ids_next;
+      issue(nx, __shfl_sync(0xffffffffu, from, (2 * nx) & 31), __shfl_sync(0xffffffffu, from, (2 * nx + 1) & 31));
+    }
+    if ((it & 15) == 15) {
       ids = ids_next;
-      ids_next = load_ids(((it >> 5) + 2) * 32);
+      ids_next = load_ids(((it >> 4) + 2) * 16);
     }
   }
 #pragma unroll
-  for (int x = 0; x < HH; ++x) {
-    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 1);
-    l[x] += __shfl_xor_sync(0xffffffffu, l[x], 2);
-    if (t == 0) { sm_ml[warp][g + 8 * x][0] = m[x]; sm_ml[warp][g + 8 * x][1] = l[x]; }
-  }
+  for (int x = 0; x < HH; ++x)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) l[x][j] += __shfl_xor_sync(0xffffffffu, l[x][j], o);
+      if (g == 0) { sm_ml[warp][2 * t + j + 8 * x][0] = m[x][j] * fh[x][j]; sm_ml[warp][2 * t + j + 8 * x][1] = l[x][j] * (1.f / 16384.f); }
+    }
   __syncthreads();                                       // the rings become the merge buffer [warp][pair][nibble of a lane][lane row g]
   float* so = reinterpret_cast<float*>(smem);
   {
-    const float fo = exp2_pos(e_run - 127) * (1.f / 7.f / 16384.f);
+    const float fo = exp2_pos(e_run - 127) * (1.f / 7.f / 16384.f);            // maxima's and P's powers of two
 #pragma unroll
     for (int x = 0; x < HH; ++x)
 #pragma unroll
