@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(128) compact_kernel(const CompactParams p) {
   }
 }
 
-bool table_ok(const void* table, int slots, int width, int pages) { return table && slots >= 1 && width >= 1 && width <= (1 << 27) && pages >= 1; }
+bool table_ok(const void* table, int slots, int width, int pages) { return table && slots >= 1 && width >= 1 && width <= kMaxWidth && pages >= 1; }
 
 }  // namespace
 

@@ -13,6 +13,7 @@
 namespace kv4 {
 
 constexpr int kPage = 16;
+constexpr int kMaxWidth = 1 << 20;                   // pages of a sequence: sums over 1024 sequences fit 32 bits
 
 template <int D>
 struct Geo {

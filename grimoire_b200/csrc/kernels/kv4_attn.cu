@@ -12,7 +12,7 @@ using namespace kv4;
 
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
-constexpr int kMaxSplits = 64;
+constexpr int kMaxUnits = 1024;      // groups of rows whose page counts a CTA keeps (streamed schedule)
 
 struct AttnParams {
   const uint8_t* data; float* mass;
@@ -21,14 +21,18 @@ struct AttnParams {
   const int* row_seq; const int* row_pos;
   const bf16* gate; long ld_gate;
   bf16* out; long ld_o;
-  float* part_o;            // [M][Hkv][splits][G][D]
-  float* part_ml;           // [M][Hkv][splits][G][2]
+  float* part_o;            // [slots][pairs of a CTA][D]: sums over a part of a unit's pages, not divided
+  float* part_ml;           // [slots][pairs of a CTA][2]: their softmax maximum (log2 domain) and sum
+  long long* sched;         // streamed schedule: pages per CTA, then the pages before each group of rows
   float* fin;               // [M][Hq][2]: softmax maximum (log2 domain) and reciprocal sum of every row, or null
   unsigned int* status;     // device status block (bounded waits report here)
   int M, Hkv, G, window, block, add;
   int rows, groups;         // rows of a block that share a CTA, groups of them in a block
   int heads, subs;          // query heads of a kv head that share a CTA, CTAs a kv head
-  int vec;                  // q rows are 8-byte aligned
+  int vec, vec_out;         // q rows are 8-byte aligned, output rows 4-byte
+  int units, uheads;        // groups of rows in all; CTA head groups (kv heads * subs).  A unit is one of each
+  int splits;               // CTAs a unit; 0: streamed
+  int ctas, pairs;          // CTAs of the streamed schedule, pairs of a CTA
   float scale_log2;         // softmax scale * log2(e)
 };
 
@@ -80,11 +84,6 @@ __device__ __forceinline__ float deq(const uint8_t* row, const unsigned short* a
   return (float)(c - 8) * __uint_as_float((uint32_t)am[(d >> 2) % groups] << 16) * (1.f / 7.f);
 }
 
-__device__ __forceinline__ uint32_t h2_add(uint32_t a, uint32_t b) {
-  uint32_t d;
-  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
-  return d;
-}
 __device__ __forceinline__ uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t d;
   asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
@@ -101,6 +100,29 @@ __device__ __forceinline__ float exp2_fast(float x) {         // 2 ulp; results 
   return y;
 }
 
+// Two elements of an output row: divided by the sum, gated, rounded; the row's statistics for the observed weight.
+__device__ __forceinline__ void finish(const AttnParams& p, int row, int head, int d, int D, float o0, float o1, float mx, float l) {
+  const float inv = l != 0.f ? 1.f / l : 0.f;
+  o0 = l != 0.f ? o0 * inv : 0.f;
+  o1 = l != 0.f ? o1 * inv : 0.f;
+  const size_t col = (size_t)head * D + d;
+  if (p.gate) {
+    o0 *= sigmoid_f(__bfloat162float(p.gate[(size_t)row * p.ld_gate + col]));
+    o1 *= sigmoid_f(__bfloat162float(p.gate[(size_t)row * p.ld_gate + col + 1]));
+  }
+  bf16* dst = p.out + (size_t)row * p.ld_o + col;
+  if (p.vec_out) {
+    *reinterpret_cast<uint32_t*>(dst) = pack_bf16x2(o0, o1);
+  } else {
+    dst[0] = __float2bfloat16(o0);
+    dst[1] = __float2bfloat16(o1);
+  }
+  if (p.fin && d == 0) {
+    p.fin[2 * ((size_t)row * p.Hkv * p.G + head)] = mx;
+    p.fin[2 * ((size_t)row * p.Hkv * p.G + head) + 1] = inv;
+  }
+}
+
 // f16 x f16 -> f32, D += A B
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   attn_mma::mma_f16_16816(d, a0, a1, a2, a3, b0, b1);
@@ -112,17 +134,18 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
 __device__ __forceinline__ int tok_of(int b, int n) { return 8 * b + ((n & 1) ? 4 + ((n >> 1) ^ 1) : (n >> 1)); }
 
 // The codes of a 16-bit half word, two words at once (two tokens, or two places of a row): element i of the result holds
-// nibble i of x's low half in its low half and of y's in its high half, as the fp16 number code - 8: the nibble becomes the
-// last mantissa bits of 1024 (or, four bits higher, of 1024 + 16 code), and one exact fp16 operation takes the offset away.
+// nibble i of x's low half in its low half and of y's in its high half, as the fp16 number (code - 8) / 2: the nibble becomes
+// the last mantissa bits of 1024 (or, four bits higher, of 1024 + 16 code), and one exact fp16 operation takes the offset away
+// (halved, because a fused multiply-add with a factor of one is compiled to an addition, which takes the integer pipe's time).
 // (Leaving the offset to the end, with the bare nibbles as fp16 subnormals, saves that operation and was measured to lose five
 // bits of the fp32 sums: the MMA aligns a subnormal's product by its unnormalised exponent.)
 __device__ __forceinline__ void nibbles(uint32_t x, uint32_t y, bool high, uint32_t (&o)[4]) {
   const uint32_t p = attn_mma::prmt(x, y, high ? 0x7632u : 0x5410u);
   const uint32_t q = p >> 8;
-  o[0] = h2_add((p & 0x000f000fu) | 0x64006400u, 0xe408e408u);                       // - 1032
-  o[1] = h2_fma((p & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, 0xd480d480u);          // / 16 - 72
-  o[2] = h2_add((q & 0x000f000fu) | 0x64006400u, 0xe408e408u);
-  o[3] = h2_fma((q & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, 0xd480d480u);
+  o[0] = h2_fma((p & 0x000f000fu) | 0x64006400u, 0x38003800u, 0xe008e008u);          // / 2 - 516
+  o[1] = h2_fma((p & 0x00f000f0u) | 0x64006400u, 0x28002800u, 0xd080d080u);          // / 32 - 36
+  o[2] = h2_fma((q & 0x000f000fu) | 0x64006400u, 0x38003800u, 0xe008e008u);
+  o[3] = h2_fma((q & 0x00f000f0u) | 0x64006400u, 0x28002800u, 0xd080d080u);
 }
 
 __device__ __forceinline__ float exp2_pos(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }   // 2^e, -127 < e < 128
@@ -142,41 +165,72 @@ __device__ __forceinline__ float exp2_pos(int e) { return __uint_as_float((uint3
 //     2^-24 of the largest ones.)
 //   * the maxima are unpacked once a step, a token per lane, and handed round through shared memory.
 // Softmax statistics, scores and outputs are fp32.
+// Rows of unit group u and the tokens they see.
+struct Rows {
+  int row0, nr, slot;
+  int len_hi, len_lo, first_lo, first_hi;                // longest and shortest row, earliest and latest first token
+  int page_lo, pages;
+};
+__device__ __forceinline__ Rows rows_of(const AttnParams& p, int u) {
+  Rows r;
+  const int blk = u / p.groups, grp = u % p.groups;
+  r.row0 = blk * p.block + grp * p.rows;
+  r.nr = min(p.rows, p.block - grp * p.rows);
+  r.slot = p.row_seq[blk * p.block];
+  r.len_hi = 0; r.len_lo = 0x7fffffff; r.first_lo = 0x7fffffff; r.first_hi = 0;
+  for (int i = 0; i < r.nr; ++i) {
+    const int len = row_len(p, r.row0 + i), first = row_first(p, len);
+    r.len_lo = min(r.len_lo, len);
+    if (len > 0) {                                       // a row without keys widens nothing
+      r.len_hi = max(r.len_hi, len);
+      r.first_lo = min(r.first_lo, first); r.first_hi = max(r.first_hi, first);
+    }
+  }
+  r.page_lo = r.len_hi > 0 ? r.first_lo / kPage : 0;
+  r.pages = r.len_hi > 0 ? (r.len_hi + kPage - 1) / kPage - r.page_lo : 0;
+  return r;
+}
+
+// Pages before each group of rows, in shared memory, by one CTA; returns the pages per CTA of the streamed schedule.
+__device__ __forceinline__ int stream_schedule(const AttnParams& p, int (&before)[kMaxUnits + 1]) {
+  __shared__ int warp_sum_[kWarps];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  int run = 0;
+  for (int base = 0; base < p.units; base += kThreads) {
+    int n = base + tid < p.units ? rows_of(p, base + tid).pages : 0, x = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) warp_sum_[warp] = x;
+    __syncthreads();
+    int ahead = run;
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) ahead += warp_sum_[w];
+      run += warp_sum_[w];
+    }
+    if (base + tid < p.units) before[base + tid] = ahead + x - n;
+    __syncthreads();
+  }
+  if (tid == 0) before[p.units] = run;
+  __syncthreads();
+  const long long total = (long long)run * p.uheads;
+  return max(8, (int)((total + p.ctas - 1) / p.ctas + 7) / 8 * 8);       // whole steps of the four warps
+}
+
 template <int D, int HH>
 __global__ void __launch_bounds__(kThreads, HH == 2 ? 3 : (D == 256 ? 3 : 4)) attn_kernel(const AttnParams p) {
   using Gm = Geo<D>;
   constexpr int NG = Gm::kGroups, WT = D / 64, PP = 8 * HH;
   constexpr int kStages = Ring<D>::kStages;
-  constexpr int kOld = D + 4;                           // floats between the pairs of the merge buffer
+  constexpr int kOld = D + 4;                            // floats between the pairs of the merge buffer
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) uint64_t bars[kWarps][kStages];
   __shared__ float sm_ml[kWarps][PP][2];
-  const int split = blockIdx.x, nsplit = gridDim.x;
-  const int kvh = blockIdx.y / p.subs, sub = blockIdx.y % p.subs;
-  const int blk = blockIdx.z / p.groups, grp = blockIdx.z % p.groups;
+  __shared__ int before[kMaxUnits + 1];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  // pairs of this CTA: rows row0 .. row0 + nr - 1 of the block x heads head0 .. head0 + nh - 1 of the kv head
-  const int row0 = blk * p.block + grp * p.rows, nr = min(p.rows, p.block - grp * p.rows);
-  const int head0 = sub * p.heads, nh = min(p.heads, p.G - head0), np = nr * nh;
-  const int slot = p.row_seq[blk * p.block];
-
-  int len_hi = 0, len_lo = 0x7fffffff, first_lo = 0x7fffffff, first_hi = 0;      // over the rows that see a key at all
-  for (int r = 0; r < nr; ++r) {
-    const int len = row_len(p, row0 + r);
-    if (len > 0) {
-      const int first = row_first(p, len);
-      len_hi = max(len_hi, len); len_lo = min(len_lo, len);
-      first_lo = min(first_lo, first); first_hi = max(first_hi, first);
-    } else {
-      len_lo = 0;
-    }
-  }
-  const int page_lo = len_hi > 0 ? first_lo / kPage : 0, page_hi = (len_hi + kPage - 1) / kPage;
-  const int pps = (page_hi - page_lo + nsplit - 1) / nsplit;
-  const int pbeg = page_lo + split * pps, pend = min(pbeg + pps, page_hi);
-  const int n_it = pbeg + 2 * warp < pend ? (pend - pbeg - 2 * warp + 2 * kWarps - 1) / (2 * kWarps) : 0;      // steps of two pages of this warp
-
-  // ---- ring ----
+  grm_pdl_trigger();
   uint8_t* ring = smem + (size_t)warp * Ring<D>::kWarpBytes;
   float* am_k = reinterpret_cast<float*>(ring + kStages * 2 * Gm::kRecord);                  // [32 tokens][NG]
   float* am_v = am_k + 32 * NG;                                                              // [32 tokens][NG]
@@ -186,24 +240,74 @@ __global__ void __launch_bounds__(kThreads, HH == 2 ? 3 : (D == 256 ? 3 : 4)) at
     mbar_fence_init();
   }
   __syncwarp();
-  // page ids of 16 steps, a lane each; -1: not there
+  uint32_t step = 0;                                     // steps of this warp so far: ring stage and barrier phase
+  uint32_t limit = 4000000u;
+
+  // the pages [at, end) of the flat list (group of rows, head group, page) that this CTA works on
+  long long at = 0, end = 1;
+  if (p.splits == 0) {
+    const int q = stream_schedule(p, before);
+    at = (long long)blockIdx.x * q;
+    end = min(at + q, (long long)before[p.units] * p.uheads);
+    if (blockIdx.x == 0) {
+      if (tid == 0) p.sched[0] = q;
+      for (int i = tid; i <= p.units; i += kThreads) p.sched[1 + i] = before[i];
+    }
+  }
+  while (at < end) {
+  int u, uh, n0, n1, part;
+  Rows rw;
+  if (p.splits == 0) {
+    int lo = 0, hi = p.units;                            // the last group with at most `at` pages before it
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if ((long long)before[mid] * p.uheads <= at) lo = mid;
+      else hi = mid;
+    }
+    u = lo;
+    rw = rows_of(p, u);
+    const long long rest = at - (long long)before[u] * p.uheads;
+    uh = (int)(rest / rw.pages);
+    n0 = (int)(rest % rw.pages);
+    n1 = (int)min((long long)rw.pages, n0 + (end - at));
+    at += n1 - n0;
+    part = (int)blockIdx.x + u * p.uheads + uh;          // parts of a unit are consecutive, units too
+  } else {
+    u = blockIdx.z; uh = blockIdx.y;
+    rw = rows_of(p, u);
+    const int per = (rw.pages + p.splits - 1) / p.splits;
+    n0 = min((int)blockIdx.x * per, rw.pages);
+    n1 = min(n0 + per, rw.pages);
+    at = end;
+    part = (u * p.uheads + uh) * p.splits + blockIdx.x;
+  }
+  const int kvh = uh / p.subs, sub = uh % p.subs;
+  // pairs of this CTA: the group's rows x heads head0 .. head0 + nh - 1 of the kv head
+  const int row0 = rw.row0, nr = rw.nr, slot = rw.slot;
+  const int head0 = sub * p.heads, nh = min(p.heads, p.G - head0), np = nr * nh;
+  const int len_hi = rw.len_hi, len_lo = rw.len_lo, first_lo = rw.first_lo, first_hi = rw.first_hi;
+  const int pbeg = rw.page_lo + n0, pend = rw.page_lo + n1;
+  const int n_it = pbeg + 2 * warp < pend ? (pend - pbeg - 2 * warp + 2 * kWarps - 1) / (2 * kWarps) : 0;      // steps of two pages of this warp
+
+  // ---- ring ----
+  // page ids of 16 steps, a lane each; -1: not there.  The lane that holds an id issues its copy.
   auto load_ids = [&](int base) {
     const int pg = pbeg + 2 * (warp + kWarps * (base + (lane >> 1))) + (lane & 1);
     return pg < pend ? page_of(p.t, slot, pg) : -1;
   };
   int ids = load_ids(0), ids_next = load_ids(16);
-  auto issue = [&](int it, int id0, int id1) {
-    if (lane == 0) {
-      uint64_t* bar = &bars[warp][it % kStages];
-      uint8_t* dst = ring + (it % kStages) * 2 * Gm::kRecord;
-      mbar_expect_tx(bar, (id0 >= 0 ? Gm::kRecord : 0) + (id1 >= 0 ? Gm::kRecord : 0));
-      if (id0 >= 0) bulk_load(dst, p.data + ((size_t)id0 * p.Hkv + kvh) * Gm::kRecord, Gm::kRecord, bar);
-      if (id1 >= 0) bulk_load(dst + Gm::kRecord, p.data + ((size_t)id1 * p.Hkv + kvh) * Gm::kRecord, Gm::kRecord, bar);
+  uint32_t mapped = __ballot_sync(0xffffffffu, ids >= 0), mapped_next = __ballot_sync(0xffffffffu, ids_next >= 0);
+  auto issue = [&](int it, uint32_t st, int id, uint32_t map) {
+    if ((lane >> 1) == (it & 15)) {
+      uint64_t* bar = &bars[warp][st % kStages];
+      if (!(lane & 1)) mbar_expect_tx(bar, Gm::kRecord * __popc(map >> lane & 3u));
+      if (id >= 0)
+        bulk_load(ring + (2 * (st % kStages) + (lane & 1)) * Gm::kRecord, p.data + ((size_t)id * p.Hkv + kvh) * Gm::kRecord, Gm::kRecord, bar);
     }
   };
 #pragma unroll
   for (int s = 0; s < kStages; ++s)
-    if (s < n_it) issue(s, __shfl_sync(0xffffffffu, ids, 2 * s), __shfl_sync(0xffffffffu, ids, 2 * s + 1));
+    if (s < n_it) issue(s, step + s, ids, mapped);
 
   // ---- q: column operands of S^T for the pairs g and g + 8 ----
   // k-step (group gi = 2 w + half, odd): the words w and w + NG / 2 of lane t's NG words, nibbles odd and odd + 2
@@ -235,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, HH == 2 ? 3 : (D == 256 ? 3 : 4)) at
     const int e = max((int)(mx >> 7), 14);               // biased exponent of the largest magnitude
     float up = e == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)(268 - e) << 23);   // 2^14 / 2^(e - 127)
     up = p.scale_log2 < 0.f ? -up : up;                  // the factor of s is positive, so that its maximum is s's maximum
-    const float f = fmaxf(fabsf(p.scale_log2) * (1.f / 7.f / 16384.f) * exp2_pos(min(e - 127, 127)), 1e-37f);       // scale / 7 / up
+    const float f = fmaxf(fabsf(p.scale_log2) * (2.f / 7.f / 16384.f) * exp2_pos(min(e - 127, 127)), 1e-37f);       // 2 scale / 7 / up
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       fh[x][j] = __shfl_sync(0xffffffffu, f, 8 * t + 4 * j);
@@ -266,7 +370,6 @@ __global__ void __launch_bounds__(kThreads, HH == 2 ? 3 : (D == 256 ? 3 : 4)) at
       for (int i = 0; i < 4; ++i) acc[x][gi][0][i] = acc[x][gi][1][i] = 0.f;
   int e_run = 14;                                        // biased exponent of the largest V maximum so far
   float corr_e = 1.f;
-  uint32_t limit = 4000000u;
 
   auto step_work = [&](auto edge_tag, const uint8_t* rec, int tok0, int have) {
     constexpr bool kEdge = decltype(edge_tag)::value;    // some token of the step is hidden from some row
@@ -420,26 +523,28 @@ __global__ void __launch_bounds__(kThreads, HH == 2 ? 3 : (D == 256 ? 3 : 4)) at
     }
   };
 
-  for (int it = 0; it < n_it; ++it) {
-    const int id0 = __shfl_sync(0xffffffffu, ids, (2 * it) & 31), id1 = __shfl_sync(0xffffffffu, ids, (2 * it + 1) & 31);
-    const int stage = it % kStages, tok0 = (pbeg + 2 * (warp + kWarps * it)) * kPage;
-    const bool here = __all_sync(0xffffffffu, mbar_wait(&bars[warp][stage], (uint32_t)(it / kStages) & 1u, p.status, 0x4b563400u | warp, limit));
-    if (!here) limit = 16;                               // the call has failed: do not wait at length again
-    const int have = here ? (id0 >= 0 ? 1 : 0) | (id1 >= 0 ? 2 : 0) : 0;
+  for (int it = 0; it < n_it; ++it, ++step) {
+    const int tok0 = (pbeg + 2 * (warp + kWarps * it)) * kPage;
+    const int have = (int)(mapped >> (2 * (it & 15))) & 3;
+    // a wait that runs out is on record in the status block; the call's result is void then, so do not wait at length again
+    if (!mbar_wait(&bars[warp][step % kStages], (step / kStages) & 1u, p.status, 0x4b563400u | warp, limit)) limit = 16;
+    __syncwarp();
     if (have) {
-      const uint8_t* rec = ring + stage * 2 * Gm::kRecord;
+      const uint8_t* rec = ring + (step % kStages) * 2 * Gm::kRecord;
       if (have != 3 || tok0 + 2 * kPage > len_lo || tok0 < first_hi) step_work(std::true_type{}, rec, tok0, have);
       else step_work(std::false_type{}, rec, tok0, 3);
     }
     __syncwarp();
     const int nx = it + kStages;
     if (nx < n_it) {
-      const int from = (nx >> 4) == (it >> 4) ? ids : ids_next;
-      issue(nx, __shfl_sync(0xffffffffu, from, (2 * nx) & 31), __shfl_sync(0xffffffffu, from, (2 * nx + 1) & 31));
+      const bool later = (nx ^ it) & 16;
+      issue(nx, step + kStages, later ? ids_next : ids, later ? mapped_next : mapped);
     }
     if ((it & 15) == 15) {
       ids = ids_next;
-      ids_next = load_ids(((it >> 4) + 2) * 16);
+      mapped = mapped_next;
+      ids_next = load_ids(it + 17);
+      mapped_next = __ballot_sync(0xffffffffu, ids_next >= 0);
     }
   }
 #pragma unroll
@@ -453,7 +558,7 @@ __global__ void __launch_bounds__(kThreads, HH == 2 ? 3 : (D == 256 ? 3 : 4)) at
   __syncthreads();                                       // the rings become the merge buffer [warp][pair][nibble of a lane][lane row g]
   float* so = reinterpret_cast<float*>(smem);
   {
-    const float fo = exp2_pos(e_run - 127) * (1.f / 7.f / 16384.f);            // maxima's and P's powers of two
+    const float fo = exp2_pos(e_run - 127) * (2.f / 7.f / 16384.f);            // codes' half, maxima's and P's powers of two
 #pragma unroll
     for (int x = 0; x < HH; ++x)
 #pragma unroll
@@ -486,40 +591,80 @@ __global__ void __launch_bounds__(kThreads, HH == 2 ? 3 : (D == 256 ? 3 : 4)) at
         o[0] += f[w] * so[(w * PP + pr) * kOld + at];
         o[1] += f[w] * so[(w * PP + pr) * kOld + at + 8];
       }
-    const int row = row0 + pr / nh, hd = head0 + pr % nh;
-    const size_t pi = (((size_t)row * p.Hkv + kvh) * nsplit + split) * p.G + hd;
-    *reinterpret_cast<float2*>(p.part_o + pi * D + d) = make_float2(o[0], o[1]);
-    if (d == 0) { p.part_ml[2 * pi] = mx; p.part_ml[2 * pi + 1] = ls; }
+    if (p.splits == 1) {
+      const int row = row0 + pr / nh, head = kvh * p.G + head0 + pr % nh;
+      finish(p, row, head, d, D, o[0], o[1], mx, ls);
+    } else {
+      const size_t pi = (size_t)part * PP + pr;
+      *reinterpret_cast<float2*>(p.part_o + pi * D + d) = make_float2(o[0], o[1]);
+      if (d == 0) { p.part_ml[2 * pi] = mx; p.part_ml[2 * pi + 1] = ls; }
+    }
+  }
+  if (p.splits == 0) {                                   // the merge buffer becomes the rings again
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncthreads();
+  }
   }
 }
 
-// Joins the splits of a row in split order, applies the gate, leaves (maximum, 1 / sum) for the weights.
-__global__ void __launch_bounds__(128) merge_kernel(const AttnParams p, int nsplit, int D) {
-  const int kvh = blockIdx.y, row = blockIdx.z, g = blockIdx.x;
-  const size_t pi = ((size_t)row * p.Hkv + kvh) * nsplit * p.G + g;
+// Joins the parts of a unit: one CTA per (query head, row).  Groups of D / 2 threads (two dims each) take every n-th part and are
+// joined in order: the result does not depend on timing.
+constexpr int kMergeThreads = 256, kMergeParts = 512;
+template <int D>
+__global__ void __launch_bounds__(kMergeThreads) merge_kernel(const AttnParams p) {
+  constexpr int kGroups = kMergeThreads / (D / 2);
+  __shared__ float wt[kMergeParts], red[kMergeThreads / 32];
+  __shared__ float2 so[kGroups][D / 2];
+  __shared__ float sl[kGroups];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, grp = tid / (D / 2), d = 2 * (tid % (D / 2));
+  const int row = blockIdx.y, head = blockIdx.x;
+  const int kvh = head / p.G, hg = head % p.G, blk = row / p.block, in = row % p.block;
+  const int u = blk * p.groups + in / p.rows, uh = kvh * p.subs + hg / p.heads;
+  const int nh = min(p.heads, p.G - hg / p.heads * p.heads), pr = (in % p.rows) * nh + hg % p.heads;
+  grm_pdl_wait();
+  long first = ((long)u * p.uheads + uh) * p.splits;
+  int n = p.splits;
+  if (p.splits == 0) {
+    const long long q = p.sched[0], lo = p.sched[1 + u], pages = p.sched[2 + u] - lo;
+    const long long beg = lo * p.uheads + uh * pages;
+    first = beg / q + (long)u * p.uheads + uh;
+    n = pages > 0 ? (int)((beg + pages - 1) / q - beg / q) + 1 : 0;
+  }
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + first * p.pairs + pr;
+  const float* po = p.part_o + (first * p.pairs + pr) * D + d;
   float mx = -INFINITY;
-  for (int s = 0; s < nsplit; ++s) mx = fmaxf(mx, p.part_ml[2 * (pi + (size_t)s * p.G)]);
-  float l = 0.f;
-  for (int s = 0; s < nsplit; ++s) {
-    const float* ml = p.part_ml + 2 * (pi + (size_t)s * p.G);
-    if (ml[1] != 0.f) l += (ml[0] == -INFINITY ? 1.f : exp2f(ml[0] - mx)) * ml[1];
-  }
-  const float inv = l != 0.f ? 1.f / l : 0.f;
-  const int head = kvh * p.G + g;
-  for (int d = threadIdx.x; d < D; d += blockDim.x) {
-    float o = 0.f;
-    for (int s = 0; s < nsplit; ++s) {
-      const size_t at = pi + (size_t)s * p.G;
-      const float* ml = p.part_ml + 2 * at;
-      if (ml[1] != 0.f) o += (ml[0] == -INFINITY ? 1.f : exp2f(ml[0] - mx)) * p.part_o[at * D + d];
+  for (int s = tid; s < n; s += kMergeThreads) mx = fmaxf(mx, ml[(size_t)s * p.pairs].x);
+  mx = warp_max(mx);
+  if (lane == 0) red[warp] = mx;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kMergeThreads / 32; ++w) mx = fmaxf(mx, red[w]);
+  float l = 0.f, o0 = 0.f, o1 = 0.f;
+  for (int base = 0; base < n; base += kMergeParts) {    // weights of the parts; a part without keys has a sum of zero
+    const int here = min(kMergeParts, n - base);
+    __syncthreads();
+    for (int s = tid; s < here; s += kMergeThreads) {
+      const float2 v = ml[(size_t)(base + s) * p.pairs];
+      wt[s] = v.y == 0.f ? 0.f : (v.x == -INFINITY ? 1.f : exp2f(v.x - mx));
     }
-    o = l != 0.f ? o * inv : 0.f;
-    if (p.gate) o *= 1.f / (1.f + __expf(-__bfloat162float(p.gate[(size_t)row * p.ld_gate + (size_t)head * D + d])));
-    p.out[(size_t)row * p.ld_o + (size_t)head * D + d] = __float2bfloat16(o);
+    __syncthreads();
+#pragma unroll 4
+    for (int s = grp; s < here; s += kGroups) {
+      const float2 v = *reinterpret_cast<const float2*>(po + (size_t)(base + s) * p.pairs * D);
+      const float f = wt[s], ls = ml[(size_t)(base + s) * p.pairs].y;
+      if (ls != 0.f) { l = fmaf(f, ls, l); o0 = fmaf(f, v.x, o0); o1 = fmaf(f, v.y, o1); }      // a NaN sum counts
+    }
   }
-  if (p.fin && threadIdx.x == 0) {
-    p.fin[2 * ((size_t)row * p.Hkv * p.G + head)] = mx;
-    p.fin[2 * ((size_t)row * p.Hkv * p.G + head) + 1] = inv;
+  so[grp][d / 2] = make_float2(o0, o1);
+  if (d == 0) sl[grp] = l;
+  __syncthreads();
+  if (grp == 0) {
+#pragma unroll
+    for (int i = 1; i < kGroups; ++i) {
+      const float2 v = so[i][d / 2];
+      o0 += v.x; o1 += v.y; l = l + sl[i];
+    }
+    finish(p, row, head, d, D, o0, o1, mx, l);
   }
 }
 
@@ -576,68 +721,114 @@ __global__ void __launch_bounds__(128) mass_kernel(const AttnParams p, int nbloc
   }
 }
 
+// How a call is cut into CTAs, and what it needs as scratch.
+struct Plan {
+  int heads, subs, rows, groups, units, uheads, pairs, splits, ctas;
+  long slots;               // parts that are stored
+  long floats(int M, int Hq, int D, int observe) const {
+    return (splits == 1 ? 0 : slots * pairs * (D + 2)) + (splits == 0 ? 2L * (units + 2) : 0) + (observe ? 2L * M * Hq : 0);
+  }
+};
+
+int plan(Plan& pl, int M, int Hq, int Hkv, int D, int block, int max_len) {
+  if (M < 1 || M > 65535 || Hkv < 1 || Hq < 1 || Hq % Hkv || Hq / Hkv > 16 || block < 1 || M % block || max_len < 1) return -2;
+  if (D != 64 && D != 128 && D != 256) return -2;
+  const int G = Hq / Hkv;
+  // (row, head) pairs of a CTA: one MMA column tile holds 8.  Two tiles where more pairs than that share the keys, except at
+  // head_dim 256, whose accumulators fill the registers with one.
+  const int most = D == 256 ? 8 : 16;
+  pl.heads = G < most ? G : most;
+  pl.subs = (G + pl.heads - 1) / pl.heads;
+  pl.rows = pl.subs > 1 ? 1 : most / G;
+  if (pl.rows > block) pl.rows = block;
+  pl.groups = (block + pl.rows - 1) / pl.rows;
+  pl.pairs = pl.rows * pl.heads <= 8 ? 8 : 16;
+  pl.uheads = Hkv * pl.subs;
+  const long units = (long)(M / block) * pl.groups;
+  if (units > 65535 || pl.uheads > 65535) return -2;
+  pl.units = (int)units;
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return -2;
+  pl.ctas = sms * (pl.pairs == 16 || D == 256 ? 3 : 4);
+  const long cells = units * pl.uheads, pages = (max_len + kPage - 1) / kPage;
+  // Streamed: every CTA gets the same number of pages of the flat list, whatever the rows' lengths, at the price of a scan over
+  // the rows and of parts that begin anywhere.  Split: a fixed number of CTAs a unit, at least eight pages (a step of the four
+  // warps) each.
+  pl.splits = 0;
+  if (units > kMaxUnits || cells * pages < 32L * pl.ctas) {
+    long s = pages / 8 < pl.ctas / cells ? pages / 8 : pl.ctas / cells;
+    pl.splits = (int)(s < 1 ? 1 : s);
+  }
+  pl.slots = pl.splits == 0 ? pl.ctas + cells : cells * pl.splits;
+  return 0;
+}
+
 template <int D, int HH>
-int launch_attn(const AttnParams& p, int splits, int nblocks, cudaStream_t st) {
+int launch_attn(const AttnParams& p, cudaStream_t st) {
   constexpr int kMerge = kWarps * 8 * HH * (D + 4) * 4;
   constexpr int kSmem = Ring<D>::kBytes > kMerge ? Ring<D>::kBytes : kMerge;
   cudaError_t e = cudaFuncSetAttribute(attn_kernel<D, HH>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
   if (e != cudaSuccess) return (int)e;
-  attn_kernel<D, HH><<<dim3(splits, p.Hkv * p.subs, nblocks * p.groups), kThreads, kSmem, st>>>(p);
+  attn_kernel<D, HH><<<p.splits ? dim3(p.splits, p.uheads, p.units) : dim3(p.ctas), kThreads, kSmem, st>>>(p);
   GRM_LAUNCH_RET();
 }
 
 template <int D>
-int launch(AttnParams p, int splits, int nblocks, int mass_pages, cudaStream_t st) {
-  // (row, head) pairs of a CTA: one MMA column tile holds 8.  Two tiles where more pairs than that share the keys, except at
-  // head_dim 256, whose accumulators fill the registers with one.
-  constexpr int kMost = D == 256 ? 8 : 16;
-  p.heads = p.G < kMost ? p.G : kMost;
-  p.subs = (p.G + p.heads - 1) / p.heads;
-  p.rows = p.subs > 1 ? 1 : kMost / p.G;
-  if (p.rows > p.block) p.rows = p.block;
-  p.groups = (p.block + p.rows - 1) / p.rows;
-  if ((long)p.Hkv * p.subs > 65535 || (long)nblocks * p.groups > 65535) return -2;
+int launch(const AttnParams& p, int nblocks, int mass_pages, cudaStream_t st) {
   int rc;
-  if constexpr (D == 256) rc = launch_attn<D, 1>(p, splits, nblocks, st);
-  else rc = p.rows * p.heads <= 8 ? launch_attn<D, 1>(p, splits, nblocks, st) : launch_attn<D, 2>(p, splits, nblocks, st);
+  if constexpr (D == 256) rc = launch_attn<D, 1>(p, st);
+  else rc = p.pairs == 8 ? launch_attn<D, 1>(p, st) : launch_attn<D, 2>(p, st);
   if (rc) return rc;
-  merge_kernel<<<dim3(p.G, p.Hkv, p.M), 128, 0, st>>>(p, splits, D);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return (int)e;
+  if (p.splits != 1) {
+    const cudaError_t e = grm_launch_pdl(GRM_PDL_ATTN, merge_kernel<D>, dim3(p.Hkv * p.G, p.M), dim3(kMergeThreads), 0, st, p);
+    if (e != cudaSuccess) return (int)e;
+  }
   if (p.mass) mass_kernel<D><<<dim3(mass_pages, p.Hkv, nblocks), 128, 0, st>>>(p, nblocks);
   GRM_LAUNCH_RET();
 }
 
 }  // namespace
 
-// Scratch of a call in fp32 words: the split partials and, with ``observe``, the softmax statistics of every row.
-GRM_API long grm_kv4_attn_scratch(int M, int Hq, int D, int splits, int observe) {
-  return (long)M * Hq * splits * (D + 2) + (observe ? 2L * M * Hq : 0);
+// Scratch of a call in fp32 words, or -2 for arguments that are not served.
+GRM_API long grm_kv4_attn_scratch(int M, int Hq, int Hkv, int D, int block, int max_len, int observe) {
+  Plan pl;
+  const int rc = plan(pl, M, Hq, Hkv, D, block, max_len);
+  return rc ? rc : pl.floats(M, Hq, D, observe);
 }
 
-// observe: 0 nothing, 1 set, 2 add.  max_len bounds the positions of the call's rows for the observed weight.
+// observe: 0 nothing, 1 set, 2 add.  max_len bounds the positions of the call's rows for the observed weight and sets how the
+// keys are cut.  scratch: 8-byte aligned.
 GRM_API int grm_kv4_attn(const void* data, void* mass, const void* table, int slots_n, int width, long stride, int pages, const void* q, long ld_q,
                          const void* row_seq, const void* row_pos, const void* gate, long ld_gate, void* out, long ld_o, void* scratch, int M, int Hq,
-                         int Hkv, int D, int splits, int window, float scale, int block, int observe, int max_len, void* stream) {
-  if (M < 1 || M > 65535 || Hkv < 1 || Hkv > 65535 || Hq % Hkv || Hq / Hkv > 16 || splits < 1 || splits > kMaxSplits || block < 1 || M % block) return -2;
-  if (!table || slots_n < 1 || width < 1 || width > (1 << 27) || pages < 1 || !scratch || (observe && !mass) || max_len < 1) return -2;
+                         int Hkv, int D, int window, float scale, int block, int observe, int max_len, void* stream) {
+  Plan pl;
+  const int rc = plan(pl, M, Hq, Hkv, D, block, max_len);
+  if (rc) return rc;
+  if (!table || slots_n < 1 || width < 1 || width > kMaxWidth || pages < 1 || !scratch || (observe && !mass)) return -2;
   AttnParams p;
   p.data = (const uint8_t*)data; p.mass = observe ? (float*)mass : nullptr;
   p.t = Table{(const int*)table, slots_n, width, stride, pages};
   p.q = (const bf16*)q; p.ld_q = ld_q; p.row_seq = (const int*)row_seq; p.row_pos = (const int*)row_pos;
   p.gate = (const bf16*)gate; p.ld_gate = ld_gate; p.out = (bf16*)out; p.ld_o = ld_o;
   p.M = M; p.Hkv = Hkv; p.G = Hq / Hkv; p.window = window; p.block = block; p.add = observe == 2;
+  p.heads = pl.heads; p.subs = pl.subs; p.rows = pl.rows; p.groups = pl.groups;
+  p.units = pl.units; p.uheads = pl.uheads; p.splits = pl.splits; p.ctas = pl.ctas; p.pairs = pl.pairs;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.status = grm_status_ptr();
   p.vec = ((uintptr_t)q | (uintptr_t)(2 * ld_q)) % 8 == 0;
-  p.part_o = (float*)scratch;
-  p.part_ml = p.part_o + (size_t)M * Hq * splits * D;
-  p.fin = observe ? p.part_ml + (size_t)M * Hq * splits * 2 : nullptr;
+  p.vec_out = ((uintptr_t)out | (uintptr_t)(2 * ld_o)) % 4 == 0;
+  float* s = (float*)scratch;
+  p.sched = (long long*)s;
+  if (pl.splits == 0) s += 2L * (pl.units + 2);
+  p.part_o = s;
+  if (pl.splits != 1) s += pl.slots * pl.pairs * D;
+  p.part_ml = s;
+  if (pl.splits != 1) s += pl.slots * pl.pairs * 2;
+  p.fin = observe ? s : nullptr;
   const int mass_pages = (max_len + kPage - 1) / kPage < width ? (max_len + kPage - 1) / kPage : width;
   switch (D) {
-    case 64: return launch<64>(p, splits, M / block, mass_pages, (cudaStream_t)stream);
-    case 128: return launch<128>(p, splits, M / block, mass_pages, (cudaStream_t)stream);
-    case 256: return launch<256>(p, splits, M / block, mass_pages, (cudaStream_t)stream);
-    default: return -2;
+    case 64: return launch<64>(p, M / block, mass_pages, (cudaStream_t)stream);
+    case 128: return launch<128>(p, M / block, mass_pages, (cudaStream_t)stream);
+    default: return launch<256>(p, M / block, mass_pages, (cudaStream_t)stream);
   }
 }

@@ -25,6 +25,7 @@ from .core import PAGE, AttnGeom
 
 HEAD_DIMS = (64, 128, 256)
 MAX_GROUP = 16          # query heads of a kv head
+MAX_PAGES = 1 << 20     # pages of a sequence
 
 
 @dataclass
@@ -64,9 +65,9 @@ def _cuda():
         lib.grm_kv4_gather.argtypes = [p, p, i, i, l, i, p, p, p, p, l, l, l, l, i, i, i, i, i, p]
         lib.grm_kv4_select.argtypes = [p, p, i, i, l, i, p, p, p, i, i, i, i, i, p]
         lib.grm_kv4_compact.argtypes = [p, p, p, i, i, l, i, p, p, p, l, i, i, i, i, i, p]
-        lib.grm_kv4_attn_scratch.argtypes = [i, i, i, i, i]
+        lib.grm_kv4_attn_scratch.argtypes = [i, i, i, i, i, i, i]
         lib.grm_kv4_attn_scratch.restype = l
-        lib.grm_kv4_attn.argtypes = [p, p, p, i, i, l, i, p, l, p, p, p, l, p, l, p, i, i, i, i, i, i, f, i, i, i, p]
+        lib.grm_kv4_attn.argtypes = [p, p, p, i, i, l, i, p, l, p, p, p, l, p, l, p, i, i, i, i, i, f, i, i, i, p]
         _lib = lib
     return _lib
 
@@ -82,6 +83,8 @@ def _check(kv: Kv4Layer, block_table: torch.Tensor, *ints: Optional[torch.Tensor
         raise ValueError(f"{what}: mass must be a contiguous fp32 [pages][kv heads][16] on the cache's device")
     if block_table.dim() != 2 or block_table.dtype != torch.int32 or (block_table.stride(1) != 1 and block_table.shape[1] > 1) or block_table.numel() == 0 or block_table.device != data.device:
         raise ValueError(f"{what}: block_table must be a non-empty int32 [slots][pages] with contiguous rows on the cache's device")
+    if block_table.shape[1] > MAX_PAGES:
+        raise ValueError(f"{what}: at most {MAX_PAGES} pages a sequence are served")
     for t in ints:
         if t is not None and (t.dim() != 1 or t.dtype != torch.int32 or not t.is_contiguous() or t.device != data.device):
             raise ValueError(f"{what}: rows, positions, slots and lengths must be contiguous int32 vectors on the cache's device")
@@ -180,12 +183,6 @@ def kv4_gather(kv: Kv4Layer, block_table: torch.Tensor, slots: Optional[torch.Te
 # ---------------------------------------------------------------------------------------------
 # attention
 # ---------------------------------------------------------------------------------------------
-def kv4_splits(max_len: int, rows: int, Hkv: int) -> int:
-    """How many CTAs share the keys of one (row, kv head)."""
-    pages = max(1, (max_len + PAGE - 1) // PAGE)
-    return max(1, min(64, pages // 8, 592 // max(1, rows * Hkv)))
-
-
 def kv4_attn(q: torch.Tensor, row_seq: torch.Tensor, row_pos: torch.Tensor, block_table: torch.Tensor, kv: Kv4Layer, geom: AttnGeom,
              out: torch.Tensor, max_len: int, gate: Optional[torch.Tensor] = None, block: int = 1, observe: Optional[str] = None) -> torch.Tensor:
     """Attention of M rows over the 4-bit pages: row m (bf16 [Hq * D], after norm and RoPE) of sequence slot ``row_seq[m]`` sees
@@ -238,14 +235,16 @@ def kv4_attn(q: torch.Tensor, row_seq: torch.Tensor, row_pos: torch.Tensor, bloc
                 old = kv.mass[page[ok], :, place[ok]] if observe == "add" else 0
                 kv.mass[page[ok], :, place[ok]] = old + w[:, ok].t()
         return out
-    splits = kv4_splits(max_len, M, Hkv)
     lib = _cuda()
     mode = 0 if observe is None else (1 if observe == "set" else 2)
     with _here(kv):
-        scratch = torch.empty(lib.grm_kv4_attn_scratch(M, Hq, D, splits, mode), dtype=torch.float32, device=kv.data.device)
+        floats = lib.grm_kv4_attn_scratch(M, Hq, Hkv, D, block, max_len, mode)
+        if floats < 0:
+            _native.check(int(floats), "kv4_attn")
+        scratch = torch.empty(max(1, floats), dtype=torch.float32, device=kv.data.device)
         code = lib.grm_kv4_attn(kv.data.data_ptr(), _ptr(kv.mass), *_slots(block_table), kv.data.shape[0], q.data_ptr(), q.stride(0), row_seq.data_ptr(),
                                 row_pos.data_ptr(), _ptr(gate), 0 if gate is None else gate.stride(0), out.data_ptr(), out.stride(0), scratch.data_ptr(),
-                                M, Hq, Hkv, D, splits, geom.window, geom.scale, block, mode, max_len, _native.stream_ptr())
+                                M, Hq, Hkv, D, geom.window, geom.scale, block, mode, max_len, _native.stream_ptr())
     _native.check(code, "kv4_attn")
     return out
 

@@ -348,6 +348,30 @@ def test_attention_with_one_token_of_far_larger_values(device):
         close(c.attend([0], [pos], q, 2, 0.1), ref, size)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,Hkv,G,block,window", [(128, 8, 5, 1, 0), (64, 8, 12, 1, 0), (256, 4, 6, 1, 0), (128, 8, 4, 3, 0), (64, 16, 1, 1, 3000)])
+def test_attention_of_a_large_ragged_batch(D, Hkv, G, block, window):
+    """Enough pages for every SM: the keys are dealt out over the whole batch, whatever the rows' lengths; some rows see nothing."""
+    lens = [5000, 33, 4811, 2600, 16, 4999, 3333, 1, 4096, 4990]
+    c = Cache(lens, Hkv, D, "cuda", seed=D)
+    seqs = [s for s in range(10) for _ in range(block)]
+    pos = [max(0, lens[s] - block + r) for s in range(10) for r in range(block)]
+    for m in (3 * block, 10 * block - 1):
+        pos[m] = -1
+    q = torch.randn(len(seqs), Hkv * G * D, generator=torch.Generator().manual_seed(G)).bfloat16()
+    scale = 1 / math.sqrt(D)
+    out = c.attend(seqs, pos, q, G, scale, window, block=block, observe="set")
+    ref, size, w, top = c.expect(seqs, pos, q, G, scale, window)
+    scores_in_range(D, top)
+    close(out, ref, size)
+    eps = 2 * (D + 16) * 2 ** -24 * top + 2 ** -19
+    for s in range(10):
+        rows = range(s * block, (s + 1) * block)
+        want, seen = sum(w[r] for r in rows), max(pos[r] for r in rows) + 1
+        got = c.mass_of(s).double()
+        assert bool(((got - want)[:, :seen].abs() <= eps * want[:, :seen] + 1e-35).all())
+
+
 # ---------------------------------------------------------------------------------------------
 # observed weight
 # ---------------------------------------------------------------------------------------------
