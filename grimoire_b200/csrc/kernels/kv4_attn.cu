@@ -139,13 +139,33 @@ __device__ __forceinline__ int tok_of(int b, int n) { return 8 * b + ((n & 1) ? 
 // (halved, because a fused multiply-add with a factor of one is compiled to an addition, which takes the integer pipe's time).
 // (Leaving the offset to the end, with the bare nibbles as fp16 subnormals, saves that operation and was measured to lose five
 // bits of the fp32 sums: the MMA aligns a subnormal's product by its unnormalised exponent.)
-__device__ __forceinline__ void nibbles(uint32_t x, uint32_t y, bool high, uint32_t (&o)[4]) {
+// The constants come in registers whose value the compiler does not see: it would otherwise spend a second instruction on
+// (p & mask) | magic for want of room for two constants in one.
+struct Magic {
+  uint32_t one, even, odd;
+  __device__ __forceinline__ Magic() {
+    asm volatile("mov.b32 %0, 0x64006400;" : "=r"(one));       // 1024
+    asm volatile("mov.b32 %0, 0x38003800;" : "=r"(even));      // 1 / 2
+    asm volatile("mov.b32 %0, 0x28002800;" : "=r"(odd));       // 1 / 32
+  }
+};
+__device__ __forceinline__ uint32_t low_nibble(uint32_t p, uint32_t one) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, 0x000f000f, %2, 0xEA;" : "=r"(d) : "r"(p), "r"(one));      // (p & mask) | one
+  return d;
+}
+__device__ __forceinline__ uint32_t high_nibble(uint32_t p, uint32_t one) {
+  uint32_t d;
+  asm("lop3.b32 %0, %1, 0x00f000f0, %2, 0xEA;" : "=r"(d) : "r"(p), "r"(one));
+  return d;
+}
+__device__ __forceinline__ void nibbles(const Magic& mg, uint32_t x, uint32_t y, bool high, uint32_t (&o)[4]) {
   const uint32_t p = attn_mma::prmt(x, y, high ? 0x7632u : 0x5410u);
   const uint32_t q = p >> 8;
-  o[0] = h2_fma((p & 0x000f000fu) | 0x64006400u, 0x38003800u, 0xe008e008u);          // / 2 - 516
-  o[1] = h2_fma((p & 0x00f000f0u) | 0x64006400u, 0x28002800u, 0xd080d080u);          // / 32 - 36
-  o[2] = h2_fma((q & 0x000f000fu) | 0x64006400u, 0x38003800u, 0xe008e008u);
-  o[3] = h2_fma((q & 0x00f000f0u) | 0x64006400u, 0x28002800u, 0xd080d080u);
+  o[0] = h2_fma(low_nibble(p, mg.one), mg.even, 0xe008e008u);          // / 2 - 516
+  o[1] = h2_fma(high_nibble(p, mg.one), mg.odd, 0xd080d080u);          // / 32 - 36
+  o[2] = h2_fma(low_nibble(q, mg.one), mg.even, 0xe008e008u);
+  o[3] = h2_fma(high_nibble(q, mg.one), mg.odd, 0xd080d080u);
 }
 
 __device__ __forceinline__ float exp2_pos(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }   // 2^e, -127 < e < 128
@@ -231,6 +251,7 @@ __global__ void __launch_bounds__(kThreads, HH == 2 ? 3 : (D == 256 ? 3 : 4)) at
   __shared__ int before[kMaxUnits + 1];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   grm_pdl_trigger();
+  const Magic mg;
   uint8_t* ring = smem + (size_t)warp * Ring<D>::kWarpBytes;
   float* am_k = reinterpret_cast<float*>(ring + kStages * 2 * Gm::kRecord);                  // [32 tokens][NG]
   float* am_v = am_k + 32 * NG;                                                              // [32 tokens][NG]
@@ -428,8 +449,8 @@ __global__ void __launch_bounds__(kThreads, HH == 2 ? 3 : (D == 256 ? 3 : 4)) at
 #pragma unroll
       for (int gi = 0; gi < NG; ++gi) {
         uint32_t n0[4], n1[4];
-        nibbles(kw[0][gi / 2], kw[0][gi / 2 + NG / 2], gi & 1, n0);
-        nibbles(kw[1][gi / 2], kw[1][gi / 2 + NG / 2], gi & 1, n1);
+        nibbles(mg, kw[0][gi / 2], kw[0][gi / 2 + NG / 2], gi & 1, n0);
+        nibbles(mg, kw[1][gi / 2], kw[1][gi / 2 + NG / 2], gi & 1, n1);
 #pragma unroll
         for (int x = 0; x < HH; ++x) {
           float c[4] = {0.f, 0.f, 0.f, 0.f};
@@ -513,8 +534,8 @@ __global__ void __launch_bounds__(kThreads, HH == 2 ? 3 : (D == 256 ? 3 : 4)) at
             pb[x][b] = transpose8x8(pb[x][b]);           // [token][pair] accumulator rows -> column operand
           }
         uint32_t v01[4], v23[4];
-        nibbles(vw[0][gi / 2], vw[1][gi / 2], gi & 1, v01);
-        nibbles(vw[2][gi / 2], vw[3][gi / 2], gi & 1, v23);
+        nibbles(mg, vw[0][gi / 2], vw[1][gi / 2], gi & 1, v01);
+        nibbles(mg, vw[2][gi / 2], vw[3][gi / 2], gi & 1, v23);
 #pragma unroll
         for (int ii = 0; ii < 2; ++ii)
 #pragma unroll
