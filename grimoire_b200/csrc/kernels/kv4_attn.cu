@@ -33,6 +33,7 @@ struct AttnParams {
   int units, uheads;        // groups of rows in all; CTA head groups (kv heads * subs).  A unit is one of each
   int splits;               // CTAs a unit; 0: streamed
   int ctas, pairs;          // CTAs of the streamed schedule, pairs of a CTA
+  int sms;
   float scale_log2;         // softmax scale * log2(e)
 };
 
@@ -79,14 +80,14 @@ __device__ __forceinline__ void store_floats(float* dst, const float (&f)[N]) {
   }
 }
 
-__device__ __forceinline__ float deq(const uint8_t* row, const unsigned short* am, int d, int groups) {
-  const int c = (row[d >> 1] >> (4 * (d & 1))) & 15;
-  return (float)(c - 8) * __uint_as_float((uint32_t)am[(d >> 2) % groups] << 16) * (1.f / 7.f);
-}
-
 __device__ __forceinline__ uint32_t h2_fma(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t d;
   asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(c));
+  return d;
+}
+__device__ __forceinline__ uint32_t h2_mul(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t a) {
@@ -169,6 +170,48 @@ __device__ __forceinline__ void nibbles(const Magic& mg, uint32_t x, uint32_t y,
 }
 
 __device__ __forceinline__ float exp2_pos(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }   // 2^e, -127 < e < 128
+
+// Lane (g, t)'s part of one query row as the column operand of K Q^T (the row is pair g's): q times a power of two that fills
+// fp16's range (exact: bf16 has fewer bits), k-step (group gi = 2 w + half, odd) made of the words w and w + NG / 2 of the
+// lane's NG words of codes, nibbles odd and odd + 2.  Returns what a product with the codes' halves has to be multiplied by
+// (and by the group's maximum) to give the score in the log2 domain; positive, so that maxima stay maxima: a negative softmax
+// scale goes into the operand.
+template <int D>
+__device__ __forceinline__ float load_q(const AttnParams& p, int row, int head, bool live, int t, uint32_t (&qb)[D / 32][2][2]) {
+  constexpr int NG = D / 32;
+  const unsigned short* src = reinterpret_cast<const unsigned short*>(p.q) + (size_t)row * p.ld_q + (size_t)head * D;
+  uint2 raw[NG][2];
+  uint32_t mx = 0;
+#pragma unroll
+  for (int gi = 0; gi < NG; ++gi)
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+      const unsigned short* at = src + (t * NG + gi / 2 + y * (NG / 2)) * 8 + (gi & 1) * 4;
+      if (!live) raw[gi][y] = make_uint2(0u, 0u);
+      else if (p.vec) raw[gi][y] = *reinterpret_cast<const uint2*>(at);
+      else raw[gi][y] = make_uint2(at[0] | ((uint32_t)at[1] << 16), at[2] | ((uint32_t)at[3] << 16));
+      const uint32_t mm = __vmaxu2(raw[gi][y].x & 0x7fff7fffu, raw[gi][y].y & 0x7fff7fffu);
+      mx = max(mx, max(mm & 0xffffu, mm >> 16));
+    }
+  mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+  mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+  const int e = max((int)(mx >> 7), 14);                 // biased exponent of the largest magnitude
+  float up = e == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)(268 - e) << 23);   // 2^14 / 2^(e - 127)
+  up = p.scale_log2 < 0.f ? -up : up;
+#pragma unroll
+  for (int gi = 0; gi < NG; ++gi) {
+    float a[4], b[4];
+    a[0] = bf16lo_to_f(raw[gi][0].x) * up; a[1] = bf16hi_to_f(raw[gi][0].x) * up;
+    a[2] = bf16lo_to_f(raw[gi][0].y) * up; a[3] = bf16hi_to_f(raw[gi][0].y) * up;
+    b[0] = bf16lo_to_f(raw[gi][1].x) * up; b[1] = bf16hi_to_f(raw[gi][1].x) * up;
+    b[2] = bf16lo_to_f(raw[gi][1].y) * up; b[3] = bf16hi_to_f(raw[gi][1].y) * up;
+#pragma unroll
+    for (int odd = 0; odd < 2; ++odd)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) qb[gi][odd][j] = attn_mma::pack_f16x2(a[odd + 2 * j], b[odd + 2 * j]);
+  }
+  return fmaxf(fabsf(p.scale_log2) * (2.f / 7.f / 16384.f) * exp2_pos(min(e - 127, 127)), 1e-37f);
+}
 
 // Attention of up to 8 * HH (row, head) pairs of one kv head over one split of the sequence's pages.
 //
@@ -331,7 +374,6 @@ __global__ void __launch_bounds__(kThreads, HH == 2 ? 3 : (D == 256 ? 3 : 4)) at
     if (s < n_it) issue(s, step + s, ids, mapped);
 
   // ---- q: column operands of S^T for the pairs g and g + 8 ----
-  // k-step (group gi = 2 w + half, odd): the words w and w + NG / 2 of lane t's NG words, nibbles odd and odd + 2
   uint32_t qb[HH][NG][2][2];
   float fh[HH][2], m[HH][2], l[HH][2];                   // of the pairs 2 t, 2 t + 1 (+ 8 x)
   int lim[HH][2], low[HH][2];
@@ -341,44 +383,13 @@ __global__ void __launch_bounds__(kThreads, HH == 2 ? 3 : (D == 256 ? 3 : 4)) at
     const bool live = pr < np;
     const int row = row0 + (live ? pr / nh : 0), head = kvh * p.G + head0 + (live ? pr % nh : 0);
     const int seen = live ? row_len(p, row) : 0;
-    const unsigned short* src = reinterpret_cast<const unsigned short*>(p.q) + (size_t)row * p.ld_q + (size_t)head * D;
-    uint2 raw[NG][2];
-    uint32_t mx = 0;
-#pragma unroll
-    for (int gi = 0; gi < NG; ++gi)
-#pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        const unsigned short* at = src + (t * NG + gi / 2 + y * (NG / 2)) * 8 + (gi & 1) * 4;
-        if (!live) raw[gi][y] = make_uint2(0u, 0u);
-        else if (p.vec) raw[gi][y] = *reinterpret_cast<const uint2*>(at);
-        else raw[gi][y] = make_uint2(at[0] | ((uint32_t)at[1] << 16), at[2] | ((uint32_t)at[3] << 16));
-        const uint32_t mm = __vmaxu2(raw[gi][y].x & 0x7fff7fffu, raw[gi][y].y & 0x7fff7fffu);
-        mx = max(mx, max(mm & 0xffffu, mm >> 16));
-      }
-    mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-    mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-    const int e = max((int)(mx >> 7), 14);               // biased exponent of the largest magnitude
-    float up = e == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)(268 - e) << 23);   // 2^14 / 2^(e - 127)
-    up = p.scale_log2 < 0.f ? -up : up;                  // the factor of s is positive, so that its maximum is s's maximum
-    const float f = fmaxf(fabsf(p.scale_log2) * (2.f / 7.f / 16384.f) * exp2_pos(min(e - 127, 127)), 1e-37f);       // 2 scale / 7 / up
+    const float f = load_q<D>(p, row, head, live, t, qb[x]);
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       fh[x][j] = __shfl_sync(0xffffffffu, f, 8 * t + 4 * j);
       lim[x][j] = __shfl_sync(0xffffffffu, seen, 8 * t + 4 * j);
       low[x][j] = row_first(p, lim[x][j]);
       m[x][j] = -INFINITY; l[x][j] = 0.f;
-    }
-#pragma unroll
-    for (int gi = 0; gi < NG; ++gi) {
-      float a[4], b[4];
-      a[0] = bf16lo_to_f(raw[gi][0].x) * up; a[1] = bf16hi_to_f(raw[gi][0].x) * up;
-      a[2] = bf16lo_to_f(raw[gi][0].y) * up; a[3] = bf16hi_to_f(raw[gi][0].y) * up;
-      b[0] = bf16lo_to_f(raw[gi][1].x) * up; b[1] = bf16hi_to_f(raw[gi][1].x) * up;
-      b[2] = bf16lo_to_f(raw[gi][1].y) * up; b[3] = bf16hi_to_f(raw[gi][1].y) * up;
-#pragma unroll
-      for (int odd = 0; odd < 2; ++odd)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) qb[x][gi][odd][j] = attn_mma::pack_f16x2(a[odd + 2 * j], b[odd + 2 * j]);
     }
   }
 
@@ -689,62 +700,166 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const AttnParams p
   }
 }
 
-// One CTA per (page, kv head, block of rows).  All rows of one sequence are summed by the CTA of its first block, in the
-// order of the rows, so that two blocks of one sequence neither race nor depend on the order of CTAs.
+// The observed weight: mass[token] (=, +=) sum over the rows and heads of a block of exp2(score - maximum) / sum.
+//
+// Scores are computed once more rather than stored: K is half of the cache, a stored score would be 4 bytes per query head.  A
+// warp takes whole pages; the page's K becomes the MMA's row operand once, (code - 8) / 2 times its group's maximum, which fp16
+// holds exactly (3 + 8 bits), and every tile of 8 (row, head) pairs is one column operand from shared memory: D / 16 MMAs and
+// four exponentials a lane.  Bound by the MMAs (16 cycles of an SM a tile and page at D = 128) where a block has many pairs, by
+// the K bytes where it has few.  All rows of one sequence are summed by the CTAs of its first block, in the order of the rows:
+// two blocks of one sequence neither race nor depend on timing.
 template <int D>
-__global__ void __launch_bounds__(128) mass_kernel(const AttnParams p, int nblocks) {
-  using Gm = Geo<D>;
-  __shared__ float sk[kPage][D + 1];
-  __shared__ float part[8][kPage];
-  __shared__ int s_len;
-  const int pg = blockIdx.x, kvh = blockIdx.y, blk = blockIdx.z;
-  const int tid = threadIdx.x;
-  const int slot = p.row_seq[blk * p.block];
-  for (int b = 0; b < blk; ++b)
-    if (p.row_seq[b * p.block] == slot) return;
-  const int page = page_of(p.t, slot, pg);
-  if (page < 0) return;
-  if (tid == 0) {
-    int len = 0;
-    for (int b = blk; b < nblocks; ++b)
-      if (p.row_seq[b * p.block] == slot)
-        for (int r = 0; r < p.block; ++r) len = max(len, p.row_pos[b * p.block + r] + 1);
-    s_len = len;
-  }
-  const uint8_t* rec = p.data + ((size_t)page * p.Hkv + kvh) * Gm::kRecord;
-  for (int i = tid; i < kPage * D; i += 128) {
-    const int tok = i / D, d = i % D;
-    sk[tok][d] = deq(rec + tok * Gm::kRow, reinterpret_cast<const unsigned short*>(rec + Gm::kAmax + tok * Gm::kAmaxTok), d, Gm::kGroups);
-  }
-  __syncthreads();
-  const int tok = tid & 15, part_id = tid >> 4, t = pg * kPage + tok;
-  float sum = 0.f;
-  for (int b = blk; b < nblocks; ++b) {
-    if (p.row_seq[b * p.block] != slot) continue;
-    for (int i = part_id; i < p.block * p.G; i += 8) {
-      const int row = b * p.block + i / p.G, head = kvh * p.G + i % p.G;
-      const int len = p.row_pos[row] + 1, first = (p.window > 0 && len > p.window) ? len - p.window : 0;
-      if (t >= len || t < first) continue;
-      const bf16* q = p.q + (size_t)row * p.ld_q + (size_t)head * D;
-      float s = 0.f;
-      for (int d = 0; d < D; ++d) s = fmaf(__bfloat162float(q[d]), sk[tok][d], s);
-      const float* f = p.fin + 2 * ((size_t)row * p.Hkv * p.G + head);
-      sum += exp2f(s * p.scale_log2 - f[0]) * f[1];
+struct MassTile {
+  static constexpr int kTiles = 2560 / D;                // tiles in shared memory at a time
+  static constexpr int kBytes = kTiles * (32 * D / 2 + 8 * 24);       // operands, (factor, maximum, 1 / sum), (seen, first)
+};
+// The weights that a page's tokens g and g + 8 draw from the lane's pairs of every tile.
+template <int D, bool kEdge>
+__device__ __forceinline__ void page_sums(const uint32_t (&ka)[D / 32][2][4], const uint4* sq, const float4* sf, const int2* sl, int tiles, float pf,
+                                          int tok0, int lane, float (&sum)[2]) {
+  constexpr int NG = D / 32;
+  const int g = lane >> 2, t = lane & 3;
+#pragma unroll 2
+  for (int i = 0; i < tiles; ++i) {
+    float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int gi = 0; gi < NG; ++gi) {
+      const uint4 q = sq[(i * NG + gi) * 32 + lane];
+      mma(c, ka[gi][0][0], ka[gi][0][1], ka[gi][0][2], ka[gi][0][3], q.x, q.y);
+      mma(c, ka[gi][1][0], ka[gi][1][1], ka[gi][1][2], ka[gi][1][3], q.z, q.w);
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float4 f = sf[8 * i + 2 * t + j];
+      const int2 lim = kEdge ? sl[8 * i + 2 * t + j] : make_int2(0, 0);
+      const float k = f.x * pf;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float e = exp2_fast(fmaf(c[2 * r + j], k, -f.y));
+        const int at = tok0 + g + 8 * r;
+        if (!kEdge || (at < lim.x && at >= lim.y)) sum[r] = fmaf(e, f.z, sum[r]);
+      }
     }
   }
-  part[part_id][tok] = sum;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads) mass_kernel(const AttnParams p, int nblocks, int pages, int per_cta) {
+  using Gm = Geo<D>;
+  constexpr int NG = Gm::kGroups, kTiles = MassTile<D>::kTiles;
+  extern __shared__ __align__(128) uint8_t smem[];
+  uint4* sq = reinterpret_cast<uint4*>(smem);                                        // [tile][NG][lane]
+  float4* sf = reinterpret_cast<float4*>(smem + kTiles * 32 * D / 2);                // [tile][pair]
+  int2* sl = reinterpret_cast<int2*>(smem + kTiles * (32 * D / 2 + 8 * 16));         // [tile][pair]
+  __shared__ int s_len, s_dup;
+  const int kvh = blockIdx.y, blk = blockIdx.z;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const int slot = p.row_seq[blk * p.block];
+  const Magic mg;
+  if (tid == 0) { s_len = 0; s_dup = 0; }
   __syncthreads();
-  if (part_id == 0 && t < min(s_len, p.t.width * kPage)) {
-    float w = 0.f;
-    for (int i = 0; i < 8; ++i) w += part[i][tok];
-    float* dst = p.mass + ((size_t)page * p.Hkv + kvh) * kPage + tok;
-    *dst = p.add ? *dst + w : w;
+  for (int b = tid; b < blk; b += kThreads)
+    if (p.row_seq[b * p.block] == slot) s_dup = 1;
+  int len = 0;
+  for (int r = blk * p.block + tid; r < nblocks * p.block; r += kThreads)
+    if (p.row_seq[r / p.block * p.block] == slot) len = max(len, row_len(p, r));
+  atomicMax(&s_len, len);
+  __syncthreads();
+  if (s_dup) return;
+  len = s_len;
+  const int beg = blockIdx.x * per_cta, end = min(min(beg + per_cta, pages), (len + kPage - 1) / kPage);
+  if (beg >= end) return;
+
+  bool first = true;                                     // nothing of this call is in the mass yet
+  for (int b = blk; b < nblocks; ++b) {
+    if (p.row_seq[b * p.block] != slot) continue;
+    const int np = p.block * p.G;
+    for (int pair0 = 0; pair0 < np; pair0 += 8 * kTiles) {
+      const int tiles = min(kTiles, (np - pair0 + 7) / 8);
+      __syncthreads();
+      for (int i = warp; i < tiles; i += kWarps) {
+        const int pr = pair0 + 8 * i + g;
+        const bool live = pr < np;
+        const int row = b * p.block + (live ? pr / p.G : 0), head = kvh * p.G + (live ? pr % p.G : 0);
+        uint32_t qb[NG][2][2];
+        const float f = load_q<D>(p, row, head, live, t, qb);
+#pragma unroll
+        for (int gi = 0; gi < NG; ++gi) sq[(i * NG + gi) * 32 + lane] = make_uint4(qb[gi][0][0], qb[gi][0][1], qb[gi][1][0], qb[gi][1][1]);
+        if (t == 0) {
+          const float* fin = p.fin + 2 * ((size_t)row * p.Hkv * p.G + head);
+          const bool any = live && fin[1] != 0.f;        // a row without keys has no reciprocal sum
+          const int seen = any ? row_len(p, row) : 0;
+          sf[8 * i + g] = any ? make_float4(f, fin[0], fin[1], 0.f) : make_float4(0.f, 0.f, 0.f, 0.f);
+          sl[8 * i + g] = make_int2(seen, row_first(p, seen));
+        }
+      }
+      __syncthreads();
+      int len_lo = 0x7fffffff, first_hi = 0;
+      for (int i = lane; i < min(8 * tiles, np - pair0); i += 32) { len_lo = min(len_lo, sl[i].x); first_hi = max(first_hi, sl[i].y); }
+      len_lo = __reduce_min_sync(0xffffffffu, len_lo);
+      first_hi = __reduce_max_sync(0xffffffffu, first_hi);
+
+      for (int pg = beg + warp; pg < end; pg += kWarps) {
+        const int page = page_of(p.t, slot, pg), tok0 = pg * kPage;
+        if (page < 0) continue;
+        const uint8_t* rec = p.data + ((size_t)page * p.Hkv + kvh) * Gm::kRecord;
+        uint32_t kw[2][NG], am[2][NG / 2];
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          load_words<NG>(rec + (g + 8 * r) * Gm::kRow + t * (D / 8), kw[r]);
+          load_words<NG / 2>(rec + Gm::kAmax + (g + 8 * r) * Gm::kAmaxTok, am[r]);
+          if (tok0 + g + 8 * r >= len)                   // what lies behind the sequence must not set the scale
+#pragma unroll
+            for (int j = 0; j < NG / 2; ++j) am[r][j] = 0u;
+        }
+        int e = 14;                                      // biased exponent of the page's largest finite maximum
+#pragma unroll
+        for (int r = 0; r < 2; ++r)
+#pragma unroll
+          for (int j = 0; j < NG / 2; ++j) {
+            const int lo = (int)(am[r][j] >> 7) & 255, hi = (int)(am[r][j] >> 23) & 255;
+            e = max(e, max(lo < 255 ? lo : 0, hi < 255 ? hi : 0));
+          }
+        e = __reduce_max_sync(0xffffffffu, e);
+        const float down = exp2_pos(138 - e), pf = exp2_pos(e - 138);    // 2^11 / 2^(e - 127): a product with a code stays below 2^14
+        uint32_t ka[NG][2][4];
+#pragma unroll
+        for (int gi = 0; gi < NG; ++gi)
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            const float a = ((gi & 1) ? bf16hi_to_f(am[r][gi / 2]) : bf16lo_to_f(am[r][gi / 2])) * down;
+            const uint32_t aa = attn_mma::pack_f16x2(a, a);
+            uint32_t n[4];
+            nibbles(mg, kw[r][gi / 2], kw[r][gi / 2 + NG / 2], gi & 1, n);
+#pragma unroll
+            for (int odd = 0; odd < 2; ++odd) {
+              ka[gi][odd][r] = h2_mul(n[odd], aa);
+              ka[gi][odd][2 + r] = h2_mul(n[odd + 2], aa);
+            }
+          }
+        float sum[2] = {0.f, 0.f};
+        if (tok0 + kPage > len_lo || tok0 < first_hi) page_sums<D, true>(ka, sq, sf, sl, tiles, pf, tok0, lane, sum);
+        else page_sums<D, false>(ka, sq, sf, sl, tiles, pf, tok0, lane, sum);
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
+          sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
+        }
+        if (t < 2) {
+          const int at = g + 8 * t;
+          const float w = t == 0 ? sum[0] : sum[1];
+          float* dst = p.mass + ((size_t)page * p.Hkv + kvh) * kPage + at;
+          if (tok0 + at < len) *dst = (first && !p.add) ? w : *dst + w;
+        }
+      }
+      first = false;
+    }
   }
 }
 
 // How a call is cut into CTAs, and what it needs as scratch.
 struct Plan {
-  int heads, subs, rows, groups, units, uheads, pairs, splits, ctas;
+  int heads, subs, rows, groups, units, uheads, pairs, splits, ctas, sms;
   long slots;               // parts that are stored
   long floats(int M, int Hq, int D, int observe) const {
     return (splits == 1 ? 0 : slots * pairs * (D + 2)) + (splits == 0 ? 2L * (units + 2) : 0) + (observe ? 2L * M * Hq : 0);
@@ -770,6 +885,7 @@ int plan(Plan& pl, int M, int Hq, int Hkv, int D, int block, int max_len) {
   pl.units = (int)units;
   int dev = 0, sms = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return -2;
+  pl.sms = sms;
   pl.ctas = sms * (pl.pairs == 16 || D == 256 ? 3 : 4);
   const long cells = units * pl.uheads, pages = (max_len + kPage - 1) / kPage;
   // Streamed: every CTA gets the same number of pages of the flat list, whatever the rows' lengths, at the price of a scan over
@@ -804,7 +920,15 @@ int launch(const AttnParams& p, int nblocks, int mass_pages, cudaStream_t st) {
     const cudaError_t e = grm_launch_pdl(GRM_PDL_ATTN, merge_kernel<D>, dim3(p.Hkv * p.G, p.M), dim3(kMergeThreads), 0, st, p);
     if (e != cudaSuccess) return (int)e;
   }
-  if (p.mass) mass_kernel<D><<<dim3(mass_pages, p.Hkv, nblocks), 128, 0, st>>>(p, nblocks);
+  if (p.mass) {
+    // pages of a CTA: enough CTAs for the GPU, at least a page a warp
+    const long cells = (long)mass_pages * p.Hkv * nblocks;
+    long per = (cells + 4L * p.sms - 1) / (4L * p.sms);
+    per = (per + kWarps - 1) / kWarps * kWarps;
+    const cudaError_t e = cudaFuncSetAttribute(mass_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, MassTile<D>::kBytes);
+    if (e != cudaSuccess) return (int)e;
+    mass_kernel<D><<<dim3((unsigned)((mass_pages + per - 1) / per), p.Hkv, nblocks), kThreads, MassTile<D>::kBytes, st>>>(p, nblocks, mass_pages, (int)per);
+  }
   GRM_LAUNCH_RET();
 }
 
@@ -833,7 +957,7 @@ GRM_API int grm_kv4_attn(const void* data, void* mass, const void* table, int sl
   p.gate = (const bf16*)gate; p.ld_gate = ld_gate; p.out = (bf16*)out; p.ld_o = ld_o;
   p.M = M; p.Hkv = Hkv; p.G = Hq / Hkv; p.window = window; p.block = block; p.add = observe == 2;
   p.heads = pl.heads; p.subs = pl.subs; p.rows = pl.rows; p.groups = pl.groups;
-  p.units = pl.units; p.uheads = pl.uheads; p.splits = pl.splits; p.ctas = pl.ctas; p.pairs = pl.pairs;
+  p.units = pl.units; p.uheads = pl.uheads; p.splits = pl.splits; p.ctas = pl.ctas; p.pairs = pl.pairs; p.sms = pl.sms;
   p.scale_log2 = scale * 1.4426950408889634f;
   p.status = grm_status_ptr();
   p.vec = ((uintptr_t)q | (uintptr_t)(2 * ld_q)) % 8 == 0;
