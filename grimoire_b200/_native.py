@@ -91,3 +91,12 @@ def stream_ptr() -> ctypes.c_void_p:
     import torch
 
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def raw_stream(index: int) -> int:
+    """The current stream of device ``index`` as a plain number (the C binding behind ``torch.cuda.current_stream``, which takes
+    3 us to build its object; that object is the fallback)."""
+    import torch
+
+    fn = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return fn(index) if fn is not None else torch.cuda.current_stream(index).cuda_stream

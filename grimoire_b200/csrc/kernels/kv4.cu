@@ -249,7 +249,7 @@ struct CompactParams {
   Table src;
   const int* slots;
   const int* idx;          // [S][Hkv][keep]
-  const int* dst; long dst_stride; int dst_width;      // fresh pages [S][>= ceil(keep / 16)]
+  const int* dst; long dst_stride;      // fresh pages [S][>= ceil(keep / 16)]
   int Hkv, keep;
 };
 
@@ -283,8 +283,6 @@ __global__ void __launch_bounds__(128) compact_kernel(const CompactParams p) {
   }
 }
 
-bool table_ok(const void* table, int slots, int width, int pages) { return table && slots >= 1 && width >= 1 && width <= kMaxWidth && pages >= 1; }
-
 }  // namespace
 
 #define KV4_DISPATCH(D, CALL)                                   \
@@ -295,46 +293,68 @@ bool table_ok(const void* table, int slots, int width, int pages) { return table
     default: return -2;                                         \
   }
 
-// data: uint8 [pages][Hkv][18 * D]; mass: fp32 [pages][Hkv][16] or null; k / v: bf16 rows of Hkv * D; vec: rows 8-byte aligned.
-GRM_API int grm_kv4_append(void* data, void* mass, const void* k, const void* v, long ld_k, long ld_v, const void* row_pos, const void* row_seq,
-                           const void* table, int slots, int width, long stride, int pages, int M, int Hkv, int D, int vec, void* stream) {
-  if (M < 1 || Hkv < 1 || !table_ok(table, slots, width, pages)) return -2;
-  AppendParams p{(uint8_t*)data, (float*)mass, (const bf16*)k, (const bf16*)v, ld_k, ld_v, (const int*)row_pos, (const int*)row_seq,
-                 Table{(const int*)table, slots, width, stride, pages}, M, Hkv, vec};
-  const long blocks = ((long)M * Hkv + 3) / 4;
+// Every entry point takes its arguments as one record of 64-bit words (kv4::Args), in the order of the list above it.
+
+// data, mass (or 0), table, slots, width, stride, pages, k, v, ld_k, ld_v, row_pos, row_seq, M, Hkv, D, vec (rows 8-byte aligned)
+// data: uint8 [pages][Hkv][18 * D]; mass: fp32 [pages][Hkv][16]; k / v: bf16 rows of Hkv * D.
+GRM_API int grm_kv4_append(const void* words, void* stream) {
+  Args a(words);
+  AppendParams p;
+  p.data = a.ptr<uint8_t>(); p.mass = a.ptr<float>();
+  if (!read_table(a, p.t)) return -2;
+  p.k = a.ptr<const bf16>(); p.v = a.ptr<const bf16>(); p.ld_k = a.num(); p.ld_v = a.num();
+  p.row_pos = a.ptr<const int>(); p.row_seq = a.ptr<const int>();
+  const long M = a.num(), Hkv = a.num(), D = a.num();
+  p.vec = a.num() != 0;
+  if (!fits(M, 1, 0x7fffffff) || !fits(Hkv, 1, 0x7fffffff) || (M * Hkv + 3) / 4 > 0x7fffffffL) return -2;
+  p.M = (int)M; p.Hkv = (int)Hkv;
+  KV4_DISPATCH(D, (append_kernel<DD><<<(unsigned)((M * Hkv + 3) / 4), 128, 0, (cudaStream_t)stream>>>(p)));
+  GRM_LAUNCH_RET();
+}
+
+// data, table, slots, width, stride, pages, seq (or 0), lengths (or 0), out_k, out_v, ld_k, ld_v, batch_k, batch_v, S, T, Hkv, D,
+// vec (rows 16-byte aligned).  out_k / out_v: bf16 [S][T][Hkv * D], strides in elements.
+GRM_API int grm_kv4_gather(const void* words, void* stream) {
+  Args a(words);
+  GatherParams p;
+  p.data = a.ptr<const uint8_t>();
+  if (!read_table(a, p.t)) return -2;
+  p.slots = a.ptr<const int>(); p.lengths = a.ptr<const int>(); p.out_k = a.ptr<bf16>(); p.out_v = a.ptr<bf16>();
+  p.ld_k = a.num(); p.ld_v = a.num(); p.batch_k = a.num(); p.batch_v = a.num();
+  const long S = a.num(), T = a.num(), Hkv = a.num(), D = a.num();
+  p.vec = a.num() != 0;
+  if (!fits(S, 1, 65535) || !fits(T, 1, 0x7fffffff) || !fits(Hkv, 1, 0x7fffffff)) return -2;
+  p.T = (int)T; p.Hkv = (int)Hkv;
+  const long blocks = (T * Hkv * (D / 4) + 255) / 256;
   if (blocks > 0x7fffffffL) return -2;
-  KV4_DISPATCH(D, (append_kernel<DD><<<(unsigned)blocks, 128, 0, (cudaStream_t)stream>>>(p)));
+  KV4_DISPATCH(D, (gather_kernel<DD><<<dim3((unsigned)blocks, (unsigned)S), 256, 0, (cudaStream_t)stream>>>(p)));
   GRM_LAUNCH_RET();
 }
 
-// out_k / out_v: bf16 [S][T][Hkv * D] with row strides ld_* and batch strides batch_* in elements; vec: every row 16-byte aligned.
-GRM_API int grm_kv4_gather(const void* data, const void* table, int slots_n, int width, long stride, int pages, const void* slots, const void* lengths,
-                           void* out_k, void* out_v, long ld_k, long ld_v, long batch_k, long batch_v, int S, int T, int Hkv, int D, int vec,
-                           void* stream) {
-  if (S < 1 || S > 65535 || T < 1 || Hkv < 1 || !table_ok(table, slots_n, width, pages)) return -2;
-  GatherParams p{(const uint8_t*)data, Table{(const int*)table, slots_n, width, stride, pages}, (const int*)slots, (const int*)lengths,
-                 (bf16*)out_k, (bf16*)out_v, ld_k, ld_v, batch_k, batch_v, T, Hkv, vec};
-  const long blocks = ((long)T * Hkv * (D / 4) + 255) / 256;
-  if (blocks > 0x7fffffffL) return -2;
-  KV4_DISPATCH(D, (gather_kernel<DD><<<dim3((unsigned)blocks, S), 256, 0, (cudaStream_t)stream>>>(p)));
+// mass, table, slots, width, stride, pages, seq (or 0), lengths, idx (int32 [S][Hkv][keep]), S, Hkv, keep, recent, sink
+GRM_API int grm_kv4_select(const void* words, void* stream) {
+  Args a(words);
+  SelectParams p;
+  p.mass = a.ptr<const float>();
+  if (!read_table(a, p.t)) return -2;
+  p.slots = a.ptr<const int>(); p.lengths = a.ptr<const int>(); p.idx = a.ptr<int>();
+  const long S = a.num(), Hkv = a.num(), keep = a.num(), recent = a.num(), sink = a.num();
+  if (!fits(S, 1, 65535) || !fits(Hkv, 1, 0x7fffffff) || !fits(keep, 1, 0x7fffffff) || !fits(recent, 0, keep) || !fits(sink, 0, keep - recent)) return -2;
+  p.Hkv = (int)Hkv; p.keep = (int)keep; p.recent = (int)recent; p.sink = (int)sink;
+  select_kernel<<<dim3((unsigned)Hkv, (unsigned)S), kSelThreads, 0, (cudaStream_t)stream>>>(p);
   GRM_LAUNCH_RET();
 }
 
-GRM_API int grm_kv4_select(const void* mass, const void* table, int slots_n, int width, long stride, int pages, const void* slots, const void* lengths,
-                           void* idx, int S, int Hkv, int keep, int recent, int sink, void* stream) {
-  if (S < 1 || S > 65535 || Hkv < 1 || keep < 1 || recent < 0 || sink < 0 || (long)recent + sink > keep || !table_ok(table, slots_n, width, pages)) return -2;
-  SelectParams p{(const float*)mass, Table{(const int*)table, slots_n, width, stride, pages}, (const int*)slots, (const int*)lengths, (int*)idx, Hkv,
-                 keep, recent, sink};
-  select_kernel<<<dim3(Hkv, S), kSelThreads, 0, (cudaStream_t)stream>>>(p);
-  GRM_LAUNCH_RET();
-}
-
-GRM_API int grm_kv4_compact(void* data, void* mass, const void* table, int slots_n, int width, long stride, int pages, const void* slots,
-                            const void* idx, const void* dst, long dst_stride, int dst_width, int S, int Hkv, int D, int keep, void* stream) {
-  const int need = (keep + kPage - 1) / kPage;
-  if (S < 1 || S > 65535 || Hkv < 1 || Hkv > 65535 || keep < 1 || dst_width < need || !table_ok(table, slots_n, width, pages)) return -2;
-  CompactParams p{(uint8_t*)data, (float*)mass, Table{(const int*)table, slots_n, width, stride, pages}, (const int*)slots, (const int*)idx,
-                  (const int*)dst, dst_stride, dst_width, Hkv, keep};
-  KV4_DISPATCH(D, (compact_kernel<DD><<<dim3(need, Hkv, S), 128, 0, (cudaStream_t)stream>>>(p)));
+// data, mass (or 0), table, slots, width, stride, pages, seq (or 0), idx, dst (int32 [S][>= ceil(keep / 16)]), dst_stride, S, Hkv, D, keep
+GRM_API int grm_kv4_compact(const void* words, void* stream) {
+  Args a(words);
+  CompactParams p;
+  p.data = a.ptr<uint8_t>(); p.mass = a.ptr<float>();
+  if (!read_table(a, p.src)) return -2;
+  p.slots = a.ptr<const int>(); p.idx = a.ptr<const int>(); p.dst = a.ptr<const int>(); p.dst_stride = a.num();
+  const long S = a.num(), Hkv = a.num(), D = a.num(), keep = a.num();
+  if (!fits(S, 1, 65535) || !fits(Hkv, 1, 65535) || !fits(keep, 1, 0x7fffffff - kPage)) return -2;
+  p.Hkv = (int)Hkv; p.keep = (int)keep;
+  KV4_DISPATCH(D, (compact_kernel<DD><<<dim3((unsigned)((keep + kPage - 1) / kPage), (unsigned)Hkv, (unsigned)S), 128, 0, (cudaStream_t)stream>>>(p)));
   GRM_LAUNCH_RET();
 }

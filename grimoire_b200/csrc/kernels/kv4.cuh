@@ -39,4 +39,31 @@ __device__ __forceinline__ int page_of(const Table& t, int slot, int index) {
   return (unsigned)p < (unsigned)t.pages ? p : -1;
 }
 
+// Arguments of a call as 64-bit words (pointers, integers; the one fraction as the bits of a double) in the order of the entry
+// point's list: a record that the caller packs at once costs it a third of what thirty separate arguments do.
+struct Args {
+  const long long* w;
+  int at = 0;
+  explicit Args(const void* words) : w((const long long*)words) {}
+  template <typename T>
+  T* ptr() { return (T*)(uintptr_t)w[at++]; }
+  long num() { return (long)w[at++]; }
+  double real() {
+    union { long long i; double d; } u;
+    u.i = w[at++];
+    return u.d;
+  }
+};
+inline bool fits(long v, long lo, long hi) { return v >= lo && v <= hi; }
+// table, slots, width, stride, pages
+inline bool read_table(Args& a, Table& t) {
+  t.table = a.ptr<const int>();
+  const long slots = a.num(), width = a.num();
+  t.stride = a.num();
+  const long pages = a.num();
+  if (!t.table || !fits(slots, 1, 0x7fffffff) || !fits(width, 1, kMaxWidth) || !fits(pages, 1, 0x7fffffff)) return false;
+  t.slots = (int)slots; t.width = (int)width; t.pages = (int)pages;
+  return true;
+}
+
 }  // namespace kv4

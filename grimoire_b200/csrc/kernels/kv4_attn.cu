@@ -861,30 +861,38 @@ __global__ void __launch_bounds__(kThreads) mass_kernel(const AttnParams p, int 
 struct Plan {
   int heads, subs, rows, groups, units, uheads, pairs, splits, ctas, sms;
   long slots;               // parts that are stored
-  long floats(int M, int Hq, int D, int observe) const {
-    return (splits == 1 ? 0 : slots * pairs * (D + 2)) + (splits == 0 ? 2L * (units + 2) : 0) + (observe ? 2L * M * Hq : 0);
+  long floats(long M, long Hq, long D, long observe) const {
+    return (splits == 1 ? 0 : slots * pairs * (D + 2)) + (splits == 0 ? 2L * (units + 2) : 0) + (observe ? 2 * M * Hq : 0);
   }
 };
 
-int plan(Plan& pl, int M, int Hq, int Hkv, int D, int block, int max_len) {
-  if (M < 1 || M > 65535 || Hkv < 1 || Hq < 1 || Hq % Hkv || Hq / Hkv > 16 || block < 1 || M % block || max_len < 1) return -2;
+// The multiprocessors of the current device (0 where that fails).
+int sm_count() {
+  static int known[64] = {0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  if (!known[dev] && cudaDeviceGetAttribute(&known[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  return known[dev];
+}
+
+int plan(Plan& pl, long M, long Hq, long Hkv, long D, long block, long max_len) {
+  if (!fits(M, 1, 65535) || !fits(Hkv, 1, 65535) || !fits(Hq, 1, 16 * Hkv) || Hq % Hkv || !fits(block, 1, M) || M % block || !fits(max_len, 1, 0x7fffffff)) return -2;
   if (D != 64 && D != 128 && D != 256) return -2;
-  const int G = Hq / Hkv;
+  const int G = (int)(Hq / Hkv), sms = sm_count();
+  if (!sms) return -2;
   // (row, head) pairs of a CTA: one MMA column tile holds 8.  Two tiles where more pairs than that share the keys, except at
   // head_dim 256, whose accumulators fill the registers with one.
   const int most = D == 256 ? 8 : 16;
   pl.heads = G < most ? G : most;
   pl.subs = (G + pl.heads - 1) / pl.heads;
   pl.rows = pl.subs > 1 ? 1 : most / G;
-  if (pl.rows > block) pl.rows = block;
-  pl.groups = (block + pl.rows - 1) / pl.rows;
+  if (pl.rows > block) pl.rows = (int)block;
+  pl.groups = (int)((block + pl.rows - 1) / pl.rows);
   pl.pairs = pl.rows * pl.heads <= 8 ? 8 : 16;
-  pl.uheads = Hkv * pl.subs;
-  const long units = (long)(M / block) * pl.groups;
-  if (units > 65535 || pl.uheads > 65535) return -2;
+  const long units = M / block * pl.groups;
+  if (units > 65535 || Hkv * pl.subs > 65535) return -2;
   pl.units = (int)units;
-  int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return -2;
+  pl.uheads = (int)Hkv * pl.subs;
   pl.sms = sms;
   pl.ctas = sms * (pl.pairs == 16 || D == 256 ? 3 : 4);
   const long cells = units * pl.uheads, pages = (max_len + kPage - 1) / kPage;
@@ -900,11 +908,22 @@ int plan(Plan& pl, int M, int Hq, int Hkv, int D, int block, int max_len) {
   return 0;
 }
 
+// Opts a kernel in to its dynamic shared memory, once per device (bit of ``ready``; setting it twice does no harm).
+cudaError_t allow_smem(unsigned long long& ready, const void* kernel, int bytes) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (ready >> (dev & 63) & 1)) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) ready |= 1ull << (dev & 63);
+  return e;
+}
+
 template <int D, int HH>
 int launch_attn(const AttnParams& p, cudaStream_t st) {
   constexpr int kMerge = kWarps * 8 * HH * (D + 4) * 4;
   constexpr int kSmem = Ring<D>::kBytes > kMerge ? Ring<D>::kBytes : kMerge;
-  cudaError_t e = cudaFuncSetAttribute(attn_kernel<D, HH>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem);
+  static unsigned long long ready = 0;
+  const cudaError_t e = allow_smem(ready, (const void*)attn_kernel<D, HH>, kSmem);
   if (e != cudaSuccess) return (int)e;
   attn_kernel<D, HH><<<p.splits ? dim3(p.splits, p.uheads, p.units) : dim3(p.ctas), kThreads, kSmem, st>>>(p);
   GRM_LAUNCH_RET();
@@ -925,7 +944,8 @@ int launch(const AttnParams& p, int nblocks, int mass_pages, cudaStream_t st) {
     const long cells = (long)mass_pages * p.Hkv * nblocks;
     long per = (cells + 4L * p.sms - 1) / (4L * p.sms);
     per = (per + kWarps - 1) / kWarps * kWarps;
-    const cudaError_t e = cudaFuncSetAttribute(mass_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, MassTile<D>::kBytes);
+    static unsigned long long ready = 0;
+    const cudaError_t e = allow_smem(ready, (const void*)mass_kernel<D>, MassTile<D>::kBytes);
     if (e != cudaSuccess) return (int)e;
     mass_kernel<D><<<dim3((unsigned)((mass_pages + per - 1) / per), p.Hkv, nblocks), kThreads, MassTile<D>::kBytes, st>>>(p, nblocks, mass_pages, (int)per);
   }
@@ -941,28 +961,35 @@ GRM_API long grm_kv4_attn_scratch(int M, int Hq, int Hkv, int D, int block, int 
   return rc ? rc : pl.floats(M, Hq, D, observe);
 }
 
-// observe: 0 nothing, 1 set, 2 add.  max_len bounds the positions of the call's rows for the observed weight and sets how the
-// keys are cut.  scratch: 8-byte aligned.
-GRM_API int grm_kv4_attn(const void* data, void* mass, const void* table, int slots_n, int width, long stride, int pages, const void* q, long ld_q,
-                         const void* row_seq, const void* row_pos, const void* gate, long ld_gate, void* out, long ld_o, void* scratch, int M, int Hq,
-                         int Hkv, int D, int window, float scale, int block, int observe, int max_len, void* stream) {
+// One record of 64-bit words (kv4::Args):
+//   data, mass (or 0), table, slots, width, stride, pages, q, ld_q, row_seq, row_pos, gate (or 0), ld_gate, out, ld_o, scratch
+//   (8-byte aligned, or 0 where none is needed), M, Hq, Hkv, D, window, scale, block, observe (0 nothing, 1 set, 2 add), max_len
+// max_len bounds the positions of the call's rows for the observed weight and sets how the keys are cut.
+GRM_API int grm_kv4_attn(const void* words, void* stream) {
+  Args a(words);
+  AttnParams p;
+  p.data = a.ptr<const uint8_t>(); p.mass = a.ptr<float>();
+  if (!read_table(a, p.t)) return -2;
+  p.q = a.ptr<const bf16>(); p.ld_q = a.num();
+  p.row_seq = a.ptr<const int>(); p.row_pos = a.ptr<const int>();
+  p.gate = a.ptr<const bf16>(); p.ld_gate = a.num();
+  p.out = a.ptr<bf16>(); p.ld_o = a.num();
+  float* s = a.ptr<float>();
+  const long M = a.num(), Hq = a.num(), Hkv = a.num(), D = a.num(), window = a.num();
+  p.scale_log2 = (float)(a.real() * 1.4426950408889634);
+  const long block = a.num(), observe = a.num(), max_len = a.num();
   Plan pl;
   const int rc = plan(pl, M, Hq, Hkv, D, block, max_len);
   if (rc) return rc;
-  if (!table || slots_n < 1 || width < 1 || width > kMaxWidth || pages < 1 || !scratch || (observe && !mass)) return -2;
-  AttnParams p;
-  p.data = (const uint8_t*)data; p.mass = observe ? (float*)mass : nullptr;
-  p.t = Table{(const int*)table, slots_n, width, stride, pages};
-  p.q = (const bf16*)q; p.ld_q = ld_q; p.row_seq = (const int*)row_seq; p.row_pos = (const int*)row_pos;
-  p.gate = (const bf16*)gate; p.ld_gate = ld_gate; p.out = (bf16*)out; p.ld_o = ld_o;
-  p.M = M; p.Hkv = Hkv; p.G = Hq / Hkv; p.window = window; p.block = block; p.add = observe == 2;
+  if (!fits(observe, 0, 2) || (observe && !p.mass) || (!s && pl.floats(M, Hq, D, observe))) return -2;
+  if (!observe) p.mass = nullptr;
+  p.M = (int)M; p.Hkv = (int)Hkv; p.G = (int)(Hq / Hkv); p.window = (int)(fits(window, 1, 0x7fffffff) ? window : 0); p.block = (int)block;
+  p.add = observe == 2;
   p.heads = pl.heads; p.subs = pl.subs; p.rows = pl.rows; p.groups = pl.groups;
   p.units = pl.units; p.uheads = pl.uheads; p.splits = pl.splits; p.ctas = pl.ctas; p.pairs = pl.pairs; p.sms = pl.sms;
-  p.scale_log2 = scale * 1.4426950408889634f;
   p.status = grm_status_ptr();
-  p.vec = ((uintptr_t)q | (uintptr_t)(2 * ld_q)) % 8 == 0;
-  p.vec_out = ((uintptr_t)out | (uintptr_t)(2 * ld_o)) % 4 == 0;
-  float* s = (float*)scratch;
+  p.vec = ((uintptr_t)p.q | (uintptr_t)(2 * p.ld_q)) % 8 == 0;
+  p.vec_out = ((uintptr_t)p.out | (uintptr_t)(2 * p.ld_o)) % 4 == 0;
   p.sched = (long long*)s;
   if (pl.splits == 0) s += 2L * (pl.units + 2);
   p.part_o = s;
@@ -970,10 +997,10 @@ GRM_API int grm_kv4_attn(const void* data, void* mass, const void* table, int sl
   p.part_ml = s;
   if (pl.splits != 1) s += pl.slots * pl.pairs * 2;
   p.fin = observe ? s : nullptr;
-  const int mass_pages = (max_len + kPage - 1) / kPage < width ? (max_len + kPage - 1) / kPage : width;
+  const int mass_pages = (int)((max_len + kPage - 1) / kPage < p.t.width ? (max_len + kPage - 1) / kPage : p.t.width);
   switch (D) {
-    case 64: return launch<64>(p, M / block, mass_pages, (cudaStream_t)stream);
-    case 128: return launch<128>(p, M / block, mass_pages, (cudaStream_t)stream);
-    default: return launch<256>(p, M / block, mass_pages, (cudaStream_t)stream);
+    case 64: return launch<64>(p, p.M / p.block, mass_pages, (cudaStream_t)stream);
+    case 128: return launch<128>(p, p.M / p.block, mass_pages, (cudaStream_t)stream);
+    default: return launch<256>(p, p.M / p.block, mass_pages, (cudaStream_t)stream);
   }
 }

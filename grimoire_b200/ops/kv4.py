@@ -14,6 +14,8 @@ synchronise.  Lengths, positions and tables are read on the device; values outsi
 from __future__ import annotations
 
 import ctypes
+import struct
+from contextlib import nullcontext
 from dataclasses import dataclass
 from typing import Optional
 
@@ -28,13 +30,23 @@ MAX_GROUP = 16          # query heads of a kv head
 MAX_PAGES = 1 << 20     # pages of a sequence
 
 
-@dataclass
+@dataclass(frozen=True)
 class Kv4Layer:
     """4-bit K / V pages of one layer: ``data`` uint8 [P][Hkv][18 * D]; ``mass`` (optional) fp32 [P][Hkv][16], the attention
     weight drawn by every cached token."""
 
     data: torch.Tensor
     mass: Optional[torch.Tensor] = None
+
+    def __post_init__(self):
+        data, mass = self.data, self.mass
+        if data.dim() != 3 or data.dtype != torch.uint8 or not data.is_contiguous() or data.shape[2] not in (1152, 2304, 4608):
+            raise ValueError(f"4-bit KV pages: data must be a contiguous uint8 [pages][kv heads][18 * head_dim] with head_dim in {HEAD_DIMS}")
+        if data.numel() == 0 or data.data_ptr() % 16:
+            raise ValueError("4-bit KV pages: data must hold a page and start on a 16-byte boundary")
+        if mass is not None and (mass.dtype != torch.float32 or not mass.is_contiguous() or mass.shape != (data.shape[0], data.shape[1], PAGE)
+                                 or mass.device != data.device):
+            raise ValueError("4-bit KV pages: mass must be a contiguous fp32 [pages][kv heads][16] on the device of the data")
 
     @staticmethod
     def alloc(pages: int, Hkv: int, D: int, device, mass: bool = False) -> "Kv4Layer":
@@ -52,60 +64,71 @@ class Kv4Layer:
         return Hkv * rec // PAGE + (4 * Hkv if self.mass is not None else 0)
 
 
+# The calls are short (a decode step makes some per layer): arguments travel as one record of 64-bit words, and tensors are
+# checked with as few attribute reads as that takes.
+_pack = {n: struct.Struct(f"{n}q").pack for n in (14, 15, 17, 19)}
+_pack_attn = struct.Struct("21qd3q").pack
 _lib = None
+_INT, _BF16 = torch.int32, torch.bfloat16
+_OBSERVE = {None: 0, "set": 1, "add": 2}
 
 
 def _cuda():
-    """The kernel library with the argument types of this module's entry points declared (numbers need no wrapping then)."""
+    """The kernel library with the argument types of this module's entry points declared."""
     global _lib
     if _lib is None:
         lib = _native.cuda()
-        p, i, l, f = ctypes.c_void_p, ctypes.c_int, ctypes.c_long, ctypes.c_float
-        lib.grm_kv4_append.argtypes = [p, p, p, p, l, l, p, p, p, i, i, l, i, i, i, i, i, p]
-        lib.grm_kv4_gather.argtypes = [p, p, i, i, l, i, p, p, p, p, l, l, l, l, i, i, i, i, i, p]
-        lib.grm_kv4_select.argtypes = [p, p, i, i, l, i, p, p, p, i, i, i, i, i, p]
-        lib.grm_kv4_compact.argtypes = [p, p, p, i, i, l, i, p, p, p, l, i, i, i, i, i, p]
-        lib.grm_kv4_attn_scratch.argtypes = [i, i, i, i, i, i, i]
-        lib.grm_kv4_attn_scratch.restype = l
-        lib.grm_kv4_attn.argtypes = [p, p, p, i, i, l, i, p, l, p, p, p, l, p, l, p, i, i, i, i, i, f, i, i, i, p]
+        for fn in (lib.grm_kv4_append, lib.grm_kv4_gather, lib.grm_kv4_select, lib.grm_kv4_compact, lib.grm_kv4_attn):
+            fn.argtypes = [ctypes.c_char_p, ctypes.c_void_p]
+        lib.grm_kv4_attn_scratch.argtypes = [ctypes.c_int] * 7
+        lib.grm_kv4_attn_scratch.restype = ctypes.c_long
         _lib = lib
     return _lib
 
 
-def _check(kv: Kv4Layer, block_table: torch.Tensor, *ints: Optional[torch.Tensor], what: str) -> None:
-    data, mass = kv.data, kv.mass
-    if data.dim() != 3 or data.dtype != torch.uint8 or not data.is_contiguous() or data.shape[2] not in (1152, 2304, 4608):
-        raise ValueError(f"{what}: data must be a contiguous uint8 [pages][kv heads][18 * head_dim] with head_dim in {HEAD_DIMS}")
-    if data.numel() == 0 or data.data_ptr() % 16:
-        raise ValueError(f"{what}: data must hold a page and start on a 16-byte boundary")
-    if mass is not None and (mass.dtype != torch.float32 or not mass.is_contiguous() or tuple(mass.shape) != (data.shape[0], data.shape[1], PAGE)
-                             or mass.device != data.device):
-        raise ValueError(f"{what}: mass must be a contiguous fp32 [pages][kv heads][16] on the cache's device")
-    if block_table.dim() != 2 or block_table.dtype != torch.int32 or (block_table.stride(1) != 1 and block_table.shape[1] > 1) or block_table.numel() == 0 or block_table.device != data.device:
-        raise ValueError(f"{what}: block_table must be a non-empty int32 [slots][pages] with contiguous rows on the cache's device")
-    if block_table.shape[1] > MAX_PAGES:
+def _check_table(table: torch.Tensor, dev: int, what: str):
+    """(pointer, slots, pages of a slot, stride) of a block table."""
+    if table.dtype is not _INT or table.dim() != 2 or table.get_device() != dev:
+        raise ValueError(f"{what}: block_table must be int32 [slots][pages] on the cache's device")
+    slots, width = table.shape
+    stride = table.stride()
+    if not slots or not width or (stride[1] != 1 and width > 1):
+        raise ValueError(f"{what}: block_table must be non-empty with contiguous rows")
+    if width > MAX_PAGES:
         raise ValueError(f"{what}: at most {MAX_PAGES} pages a sequence are served")
-    for t in ints:
-        if t is not None and (t.dim() != 1 or t.dtype != torch.int32 or not t.is_contiguous() or t.device != data.device):
-            raise ValueError(f"{what}: rows, positions, slots and lengths must be contiguous int32 vectors on the cache's device")
+    return table.data_ptr(), slots, width, stride[0]
 
 
-def _check_rows(t: torch.Tensor, kv: Kv4Layer, M: int, width: int, name: str, what: str) -> None:
-    if t.dim() != 2 or t.shape[0] != M or t.shape[1] != width or t.dtype != torch.bfloat16 or (t.stride(1) != 1 and width > 1) or t.device != kv.data.device:
-        raise ValueError(f"{what}: {name} must be bf16 [{M}][{width}] with contiguous rows on the cache's device")
+def _check_ints(t: Optional[torch.Tensor], n: int, dev: int, what: str) -> int:
+    if t is None:
+        return 0
+    if t.dtype is not _INT or t.dim() != 1 or t.shape[0] != n or t.get_device() != dev or not t.is_contiguous():
+        raise ValueError(f"{what}: rows, positions, slots and lengths must be contiguous int32 vectors on the cache's device, an entry per row or sequence")
+    return t.data_ptr()
 
 
-def _here(kv: Kv4Layer):
-    """Makes the cache's device the current one for the launch."""
-    return torch.cuda.device(kv.data.device)
+def _check_rows(t: torch.Tensor, M: int, W: int, dev: int, name: str, what: str):
+    """(pointer, row stride) of bf16 rows."""
+    if t.dtype is not _BF16 or t.dim() != 2 or t.shape[0] != M or t.shape[1] != W or t.get_device() != dev:
+        raise ValueError(f"{what}: {name} must be bf16 [{M}][{W}] on the cache's device")
+    stride = t.stride()
+    if stride[1] != 1:
+        raise ValueError(f"{what}: the rows of {name} must be contiguous")
+    return t.data_ptr(), stride[0]
 
 
-def _slots(block_table: torch.Tensor):
-    return block_table.data_ptr(), block_table.shape[0], block_table.shape[1], block_table.stride(0)
+def _ptr(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
-def _ptr(t: Optional[torch.Tensor]):
-    return None if t is None else t.data_ptr()
+def _on(dev: int):
+    """Makes ``dev`` the current device, where it is not already."""
+    return nullcontext() if torch._C._cuda_getDevice() == dev else torch.cuda.device(dev)
+
+
+def _launch(fn, words: bytes, dev: int, what: str) -> None:
+    with _on(dev):
+        _native.check(fn(words, _native.raw_stream(dev)), what)
 
 
 # ---------------------------------------------------------------------------------------------
@@ -118,15 +141,16 @@ def kv4_append(kv: Kv4Layer, k: torch.Tensor, v: torch.Tensor, row_pos: torch.Te
 
     Per group of 32 elements ``code = round(7 x / max|x|)``, ties to even, exactly as in 64-bit arithmetic.  A group with an
     infinity or a NaN reads back as NaN."""
-    M, Hkv, D = k.shape[0], kv.data.shape[1], kv.D
-    _check(kv, block_table, row_pos, row_seq, what="kv4_append")
-    _check_rows(k, kv, M, Hkv * D, "k", "kv4_append")
-    _check_rows(v, kv, M, Hkv * D, "v", "kv4_append")
-    if row_pos.numel() != M or row_seq.numel() != M:
-        raise ValueError("kv4_append: row_pos and row_seq need an entry per row")
+    data = kv.data
+    P, Hkv, rec = data.shape
+    D, M, dev, what = rec // 18, k.shape[0], data.get_device(), "kv4_append"
+    table = _check_table(block_table, dev, what)
+    kp, ks = _check_rows(k, M, Hkv * D, dev, "k", what)
+    vp, vs = _check_rows(v, M, Hkv * D, dev, "v", what)
+    pos, seq = _check_ints(row_pos, M, dev, what), _check_ints(row_seq, M, dev, what)
     if M == 0:
         return
-    if not kv.data.is_cuda:
+    if dev < 0:
         codes, amax = ref.kv4_views(kv.data)
         for m in range(M):
             page, slot, ok = ref.kv4_place(block_table, int(row_seq[m]), row_pos[m: m + 1], kv.data.shape[0])
@@ -138,11 +162,8 @@ def kv4_append(kv: Kv4Layer, k: torch.Tensor, v: torch.Tensor, row_pos: torch.Te
                 if kv.mass is not None:
                     kv.mass[page[0], :, slot[0]] = 0
         return
-    vec = int((k.data_ptr() | v.data_ptr() | 2 * k.stride(0) | 2 * v.stride(0)) % 8 == 0)
-    with _here(kv):
-        code = _cuda().grm_kv4_append(kv.data.data_ptr(), _ptr(kv.mass), k.data_ptr(), v.data_ptr(), k.stride(0), v.stride(0), row_pos.data_ptr(),
-                                      row_seq.data_ptr(), *_slots(block_table), kv.data.shape[0], M, Hkv, D, vec, _native.stream_ptr())
-    _native.check(code, "kv4_append")
+    words = _pack[17](data.data_ptr(), _ptr(kv.mass), *table, P, kp, vp, ks, vs, pos, seq, M, Hkv, D, (kp | vp | 2 * ks | 2 * vs) % 8 == 0)
+    _launch(_cuda().grm_kv4_append, words, dev, what)
 
 
 def kv4_gather(kv: Kv4Layer, block_table: torch.Tensor, slots: Optional[torch.Tensor], lengths: Optional[torch.Tensor], out_k: torch.Tensor,
@@ -150,19 +171,22 @@ def kv4_gather(kv: Kv4Layer, block_table: torch.Tensor, slots: Optional[torch.Te
     """Dequantise the first ``min(lengths[i], T)`` cached tokens of sequence slot ``slots[i]`` into ``out_k[i]`` / ``out_v[i]``
     (bf16 [S][T][Hkv * D], rounded once).  ``slots`` None: sequence i is row i of the table; ``lengths`` None: all T tokens.
     Rows past a sequence's length, and those of pages that are not mapped, stay as they are."""
-    _check(kv, block_table, slots, lengths, what="kv4_gather")
-    P, Hkv, D = kv.data.shape[0], kv.data.shape[1], kv.D
+    data = kv.data
+    P, Hkv, rec = data.shape
+    D, dev, what = rec // 18, data.get_device(), "kv4_gather"
+    table = _check_table(block_table, dev, what)
     for t in (out_k, out_v):
-        if t.dim() != 3 or t.dtype != torch.bfloat16 or t.shape[2] != Hkv * D or t.shape[:2] != out_k.shape[:2] or t.stride(2) != 1 or t.device != kv.data.device:
+        if t.dtype is not _BF16 or t.dim() != 3 or t.shape[2] != Hkv * D or t.shape[:2] != out_k.shape[:2] or t.get_device() != dev or t.stride(2) != 1:
             raise ValueError("kv4_gather: out_k / out_v must be bf16 [sequences][tokens][kv heads * head_dim] with contiguous rows on the cache's device")
     S, T = out_k.shape[:2]
-    if (slots is None and S > block_table.shape[0]) or any(t is not None and t.numel() != S for t in (slots, lengths)):
-        raise ValueError("kv4_gather: slots and lengths need an entry per sequence")
+    seq, length = _check_ints(slots, S, dev, what), _check_ints(lengths, S, dev, what)
+    if slots is None and S > table[1]:
+        raise ValueError("kv4_gather: more sequences than the table has rows")
     if S > 65535:
         raise ValueError("kv4_gather: at most 65535 sequences")
     if S == 0 or T == 0:
         return
-    if not kv.data.is_cuda:
+    if dev < 0:
         for i in range(S):
             n = max(0, T if lengths is None else min(T, int(lengths[i])))
             t = torch.arange(n)
@@ -170,14 +194,10 @@ def kv4_gather(kv: Kv4Layer, block_table: torch.Tensor, slots: Optional[torch.Te
             for out, x in zip((out_k, out_v), ref.kv4_rows(kv.data, page, slot)):
                 out[i, :n][ok] = x[ok].reshape(-1, Hkv * D).to(torch.bfloat16)
         return
-    align = out_k.data_ptr() | out_v.data_ptr()
-    for t in (out_k, out_v):
-        align |= 2 * t.stride(0) | 2 * t.stride(1)
-    with _here(kv):
-        code = _cuda().grm_kv4_gather(kv.data.data_ptr(), *_slots(block_table), P, _ptr(slots), _ptr(lengths), out_k.data_ptr(), out_v.data_ptr(),
-                                      out_k.stride(1), out_v.stride(1), out_k.stride(0), out_v.stride(0), S, T, Hkv, D, int(align % 16 == 0),
-                                      _native.stream_ptr())
-    _native.check(code, "kv4_gather")
+    kp, vp = out_k.data_ptr(), out_v.data_ptr()
+    (kb, ks, _), (vb, vs, _) = out_k.stride(), out_v.stride()
+    words = _pack[19](data.data_ptr(), *table, P, seq, length, kp, vp, ks, vs, kb, vb, S, T, Hkv, D, (kp | vp | 2 * (ks | vs | kb | vb)) % 16 == 0)
+    _launch(_cuda().grm_kv4_gather, words, dev, what)
 
 
 # ---------------------------------------------------------------------------------------------
@@ -195,29 +215,30 @@ def kv4_attn(q: torch.Tensor, row_seq: torch.Tensor, row_pos: torch.Tensor, bloc
     ``observe``: "set" or "add" the softmax weight that every token drew from the rows of its sequence in this call, summed
     over the rows and the query heads of a kv head, to ``kv.mass``; "set" covers all tokens up to the block's last position.
     """
-    M, Hq, D, Hkv = q.shape[0], geom.Hq, geom.D, geom.Hkv
-    _check(kv, block_table, row_seq, row_pos, what="kv4_attn")
-    if kv.D != D or kv.data.shape[1] != Hkv:
-        raise ValueError(f"kv4_attn: the cache holds {kv.data.shape[1]} kv heads of {kv.D}, the geometry says {Hkv} of {D}")
-    if Hkv < 1 or Hq % Hkv or not 1 <= Hq // Hkv <= MAX_GROUP:
+    data = kv.data
+    P, heads, rec = data.shape
+    M, Hq, D, Hkv, dev, what = q.shape[0], geom.Hq, geom.D, geom.Hkv, data.get_device(), "kv4_attn"
+    table = _check_table(block_table, dev, what)
+    if rec != 18 * D or heads != Hkv:
+        raise ValueError(f"kv4_attn: the cache holds {heads} kv heads of {rec // 18}, the geometry says {Hkv} of {D}")
+    if Hq % Hkv or not 1 <= Hq // Hkv <= MAX_GROUP:
         raise ValueError(f"kv4_attn: {Hq} query heads over {Hkv} kv heads: 1 to {MAX_GROUP} query heads a kv head are served")
-    _check_rows(q, kv, M, Hq * D, "q", "kv4_attn")
-    _check_rows(out, kv, M, Hq * D, "out", "kv4_attn")
-    if gate is not None:
-        _check_rows(gate, kv, M, Hq * D, "gate", "kv4_attn")
-    if row_seq.numel() != M or row_pos.numel() != M:
-        raise ValueError("kv4_attn: row_seq and row_pos need an entry per row")
+    qp, qs = _check_rows(q, M, Hq * D, dev, "q", what)
+    op, os_ = _check_rows(out, M, Hq * D, dev, "out", what)
+    gp, gs = (0, 0) if gate is None else _check_rows(gate, M, Hq * D, dev, "gate", what)
+    seq, pos = _check_ints(row_seq, M, dev, what), _check_ints(row_pos, M, dev, what)
     if block < 1 or M % block or M > 65535:
         raise ValueError(f"kv4_attn: {M} rows in blocks of {block}: a whole number of blocks and at most 65535 rows are served")
-    if observe not in (None, "set", "add"):
+    mode = _OBSERVE.get(observe, -1)
+    if mode < 0:
         raise ValueError(f"kv4_attn: observe must be None, 'set' or 'add', got {observe!r}")
-    if observe is not None and kv.mass is None:
+    if mode and kv.mass is None:
         raise ValueError("kv4_attn: observe needs a cache with mass")
-    if max_len < 1:
-        raise ValueError("kv4_attn: max_len must be at least 1")
+    if not 1 <= max_len <= MAX_PAGES * PAGE:
+        raise ValueError(f"kv4_attn: max_len must lie in 1 .. {MAX_PAGES * PAGE}")
     if M == 0:
         return out
-    if not kv.data.is_cuda:
+    if dev < 0:
         o, weights = ref.kv4_attention(q, row_seq, row_pos, block_table, kv.data, Hq, geom.scale, geom.window)
         if gate is not None:
             o = o * torch.sigmoid(gate.float())
@@ -236,16 +257,14 @@ def kv4_attn(q: torch.Tensor, row_seq: torch.Tensor, row_pos: torch.Tensor, bloc
                 kv.mass[page[ok], :, place[ok]] = old + w[:, ok].t()
         return out
     lib = _cuda()
-    mode = 0 if observe is None else (1 if observe == "set" else 2)
-    with _here(kv):
+    with _on(dev):
         floats = lib.grm_kv4_attn_scratch(M, Hq, Hkv, D, block, max_len, mode)
         if floats < 0:
-            _native.check(int(floats), "kv4_attn")
-        scratch = torch.empty(max(1, floats), dtype=torch.float32, device=kv.data.device)
-        code = lib.grm_kv4_attn(kv.data.data_ptr(), _ptr(kv.mass), *_slots(block_table), kv.data.shape[0], q.data_ptr(), q.stride(0), row_seq.data_ptr(),
-                                row_pos.data_ptr(), _ptr(gate), 0 if gate is None else gate.stride(0), out.data_ptr(), out.stride(0), scratch.data_ptr(),
-                                M, Hq, Hkv, D, geom.window, geom.scale, block, mode, max_len, _native.stream_ptr())
-    _native.check(code, "kv4_attn")
+            _native.check(int(floats), what)
+        scratch = torch.empty(floats, dtype=torch.float32, device=data.device) if floats else None
+        words = _pack_attn(data.data_ptr(), _ptr(kv.mass), *table, P, qp, qs, seq, pos, gp, gs, op, os_, _ptr(scratch), M, Hq, Hkv, D, geom.window,
+                           geom.scale, block, mode, max_len)
+        _native.check(lib.grm_kv4_attn(words, _native.raw_stream(dev)), what)
     return out
 
 
@@ -258,20 +277,22 @@ def kv4_select(kv: Kv4Layer, slots: Optional[torch.Tensor], lengths: torch.Tenso
     last ``recent`` and, per kv head, those of the rest with the most mass (ties to the earlier token; NaN and tokens without
     a page come last).  Returns int32 [S][Hkv][keep], positions in ascending order, -1 behind the last one of a sequence
     that is not longer than ``keep``."""
-    _check(kv, block_table, slots, lengths, what="kv4_select")
-    S, Hkv = lengths.numel(), kv.data.shape[1]
+    P, Hkv, _ = kv.data.shape
+    S, dev, what = lengths.numel(), kv.data.get_device(), "kv4_select"
+    table = _check_table(block_table, dev, what)
+    seq, length = _check_ints(slots, S, dev, what), _check_ints(lengths, S, dev, what)
     if kv.mass is None:
         raise ValueError("kv4_select needs a cache with mass")
     if keep < 1 or recent < 0 or sink < 0 or recent + sink > keep:
         raise ValueError(f"kv4_select: keep {keep} >= 1, recent {recent} and sink {sink} >= 0 and recent + sink <= keep are wanted")
-    if (slots is None and S > block_table.shape[0]) or (slots is not None and slots.numel() != S):
-        raise ValueError("kv4_select: slots and lengths need an entry per sequence")
+    if slots is None and S > table[1]:
+        raise ValueError("kv4_select: more sequences than the table has rows")
     if S > 65535:
         raise ValueError("kv4_select: at most 65535 sequences")
     idx = torch.empty(S, Hkv, keep, dtype=torch.int32, device=kv.data.device)
     if S == 0:
         return idx
-    if not kv.data.is_cuda:
+    if dev < 0:
         idx.fill_(-1)
         for i in range(S):
             n = max(0, min(int(lengths[i]), block_table.shape[1] * PAGE))
@@ -287,10 +308,8 @@ def kv4_select(kv: Kv4Layer, slots: Optional[torch.Tensor], lengths: torch.Tenso
                 got = order[:keep].sort().values
                 idx[i, h, : got.numel()] = got.to(torch.int32)
         return idx
-    with _here(kv):
-        code = _cuda().grm_kv4_select(kv.mass.data_ptr(), *_slots(block_table), kv.data.shape[0], _ptr(slots), lengths.data_ptr(), idx.data_ptr(), S, Hkv,
-                                      keep, recent, sink, _native.stream_ptr())
-    _native.check(code, "kv4_select")
+    words = _pack[14](kv.mass.data_ptr(), *table, P, seq, length, idx.data_ptr(), S, Hkv, keep, recent, sink)
+    _launch(_cuda().grm_kv4_select, words, dev, what)
     return idx
 
 
@@ -299,20 +318,24 @@ def kv4_compact(kv: Kv4Layer, slots: Optional[torch.Tensor], idx: torch.Tensor, 
     pages ``dst_table[i]`` (int32 [S][>= ceil(keep / 16)]).  The destination pages must not be among the sources: pages that
     other sequences share stay intact, and the caller swaps the tables afterwards.  Places whose ``idx`` is -1 stay as they
     are."""
-    _check(kv, block_table, slots, what="kv4_compact")
-    if idx.dim() != 3 or idx.dtype != torch.int32 or not idx.is_contiguous() or idx.shape[1] != kv.data.shape[1] or idx.device != kv.data.device:
+    data = kv.data
+    P, Hkv, rec = data.shape
+    dev, what = data.get_device(), "kv4_compact"
+    table = _check_table(block_table, dev, what)
+    if idx.dtype is not _INT or idx.dim() != 3 or not idx.is_contiguous() or idx.shape[1] != Hkv or idx.get_device() != dev:
         raise ValueError("kv4_compact: idx must be a contiguous int32 [sequences][kv heads][keep] on the cache's device")
-    S, Hkv, keep = idx.shape
-    if dst_table.dim() != 2 or dst_table.dtype != torch.int32 or dst_table.shape[0] != S or dst_table.shape[1] * PAGE < keep or \
-            (dst_table.stride(1) != 1 and dst_table.shape[1] > 1) or dst_table.device != kv.data.device:
+    S, _, keep = idx.shape
+    if dst_table.dtype is not _INT or dst_table.dim() != 2 or dst_table.shape[0] != S or dst_table.shape[1] * PAGE < keep or \
+            (dst_table.stride(1) != 1 and dst_table.shape[1] > 1) or dst_table.get_device() != dev:
         raise ValueError("kv4_compact: dst_table must be int32 [sequences][>= keep / 16 pages] with contiguous rows on the cache's device")
-    if (slots is None and S > block_table.shape[0]) or (slots is not None and slots.numel() != S):
-        raise ValueError("kv4_compact: slots needs an entry per sequence")
+    seq = _check_ints(slots, S, dev, what)
+    if slots is None and S > table[1]:
+        raise ValueError("kv4_compact: more sequences than the table has rows")
     if S > 65535:
         raise ValueError("kv4_compact: at most 65535 sequences")
     if S == 0 or keep == 0:
         return
-    if not kv.data.is_cuda:
+    if dev < 0:
         codes, amax = ref.kv4_views(kv.data)
         P = kv.data.shape[0]
         for i in range(S):
@@ -325,7 +348,5 @@ def kv4_compact(kv: Kv4Layer, slots: Optional[torch.Tensor], idx: torch.Tensor, 
                 if kv.mass is not None:
                     kv.mass[c, h, d] = kv.mass[a, h, b]
         return
-    with _here(kv):
-        code = _cuda().grm_kv4_compact(kv.data.data_ptr(), _ptr(kv.mass), *_slots(block_table), kv.data.shape[0], _ptr(slots), idx.data_ptr(),
-                                       dst_table.data_ptr(), dst_table.stride(0), dst_table.shape[1], S, Hkv, kv.D, keep, _native.stream_ptr())
-    _native.check(code, "kv4_compact")
+    words = _pack[15](data.data_ptr(), _ptr(kv.mass), *table, P, seq, idx.data_ptr(), dst_table.data_ptr(), dst_table.stride(0), S, Hkv, rec // 18, keep)
+    _launch(_cuda().grm_kv4_compact, words, dev, what)
