@@ -20,74 +20,89 @@ struct AppendParams {
   int M, Hkv, vec;
 };
 
-// One warp per (row, kv head): the 2 * D / 4 quads of K and V go round the lanes, so a lane's quads all lie in one group and
-// the group's maximum is a butterfly over the lanes with the same (K / V, quad mod groups).  7 x / maximum is a quotient of an
-// 11-bit and an 8-bit integer (times powers of two; 7 / 8 and 1 / 8 so that nothing overflows): a correctly rounded fp32
-// division never lands on another side of a rounding boundary than the exact quotient, so the codes equal those of 64-bit
-// arithmetic.
-template <int D>
+// A warp per row and head: the 2 * D / 4 quads of K and V go round the lanes, so a lane's quads all lie in one group and
+// the group's maximum is a butterfly over the lanes with the same (K / V, quad mod groups).
+//
+// The codes equal those of 64-bit arithmetic.  7 x / maximum is a quotient of an 11-bit and an 8-bit integer (times a power of
+// two): it either is a multiple of one half, or at least 2^-13 away from one.  Both are first scaled by a power of two that brings
+// the maximum near one (exact, nothing overflows); x7 times the approximate reciprocal, corrected by its exact residual once, is
+// within an ulp of the quotient and equals it where it is a multiple of one half; adding 1.5 * 2^23 rounds to even.
+//
+// kHeads heads of a row a warp: one where there are few rows, four (their loads in flight together, one look into the table) where
+// there are many.
+template <int D, int kHeads>
 __global__ void __launch_bounds__(128) append_kernel(const AppendParams p) {
   using G = Geo<D>;
   constexpr int kQuads = D / 4, kRegs = (2 * kQuads + 31) / 32;
   const long wid = ((long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31;
-  if (wid >= (long)p.M * p.Hkv) return;
-  const int row = (int)(wid / p.Hkv), h = (int)(wid % p.Hkv);
+  const int sets = (p.Hkv + kHeads - 1) / kHeads;
+  if (wid >= (long)p.M * sets) return;
+  const int row = (int)(wid / sets), h0 = (int)(wid % sets) * kHeads;
   const int pos = p.row_pos[row];
   const int page = pos < 0 ? -1 : page_of(p.t, p.row_seq[row], pos / kPage);
   if (page < 0) return;
   const int slot = pos % kPage;
-  uint2 x[kRegs];          // 4 bf16 each
+  uint2 x[kHeads][kRegs];          // 4 bf16 each
 #pragma unroll
-  for (int i = 0; i < kRegs; ++i) {
-    const int idx = lane + 32 * i, which = idx / kQuads, quad = idx % kQuads;
-    const bf16* src = (which ? p.v + (size_t)row * p.ld_v : p.k + (size_t)row * p.ld_k) + (size_t)h * D + 4 * quad;
-    if (p.vec) {
-      x[i] = *reinterpret_cast<const uint2*>(src);
-    } else {
-      const unsigned short* s = reinterpret_cast<const unsigned short*>(src);
-      x[i].x = s[0] | ((uint32_t)s[1] << 16);
-      x[i].y = s[2] | ((uint32_t)s[3] << 16);
+  for (int n = 0; n < kHeads; ++n)
+#pragma unroll
+    for (int i = 0; i < kRegs; ++i) {
+      const int idx = lane + 32 * i, which = idx / kQuads, quad = idx % kQuads;
+      const bf16* src = (which ? p.v + (size_t)row * p.ld_v : p.k + (size_t)row * p.ld_k) + (size_t)min(h0 + n, p.Hkv - 1) * D + 4 * quad;
+      if (p.vec) {
+        x[n][i] = *reinterpret_cast<const uint2*>(src);
+      } else {
+        const unsigned short* s = reinterpret_cast<const unsigned short*>(src);
+        x[n][i].x = s[0] | ((uint32_t)s[1] << 16);
+        x[n][i].y = s[2] | ((uint32_t)s[3] << 16);
+      }
     }
-  }
-  // magnitude bits order like the values, with infinity and then NaN on top
-  uint32_t mx[kRegs];
 #pragma unroll
-  for (int i = 0; i < kRegs; ++i) {
-    const uint32_t a = x[i].x & 0x7fff7fffu, b = x[i].y & 0x7fff7fffu;
-    const uint32_t m = __vmaxu2(a, b);
-    mx[i] = max(m & 0xffffu, m >> 16);
-  }
-  if constexpr (D == 256) {                       // registers 0, 1 are K, 2, 3 are V; both quads of a lane are in group lane % 8
-    mx[0] = mx[1] = max(mx[0], mx[1]);
-    mx[2] = mx[3] = max(mx[2], mx[3]);
-  }
+  for (int n = 0; n < kHeads; ++n) {
+    if (h0 + n >= p.Hkv) break;
+    // magnitude bits order like the values, with infinity and then NaN on top
+    uint32_t mx[kRegs];
 #pragma unroll
-  for (int i = 0; i < kRegs; ++i) {
-    if (D == 256 && (i & 1)) { mx[i] = mx[i - 1]; continue; }
-#pragma unroll
-    for (int o = G::kGroups; o < (kQuads < 32 ? kQuads : 32); o <<= 1) mx[i] = max(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], o));
-  }
-  uint8_t* rec = p.data + ((size_t)page * p.Hkv + h) * G::kRecord;
-#pragma unroll
-  for (int i = 0; i < kRegs; ++i) {
-    const int idx = lane + 32 * i, which = idx / kQuads, quad = idx % kQuads;
-    const float amax = __uint_as_float(mx[i] << 16);
-    const bool ok = mx[i] > 0u && mx[i] < 0x7f80u;        // an empty group has codes of zero; one that is not finite reads back as NaN
-    uint32_t word = 0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t b = j < 2 ? x[i].x : x[i].y;
-      const float f = (j & 1) ? bf16hi_to_f(b) : bf16lo_to_f(b);
-      const int q = ok ? __float2int_rn(__fdiv_rn(0.875f * f, 0.125f * amax)) : 0;
-      word |= (uint32_t)(q + 8) << (4 * j);
+    for (int i = 0; i < kRegs; ++i) {
+      const uint32_t m = __vmaxu2(x[n][i].x & 0x7fff7fffu, x[n][i].y & 0x7fff7fffu);
+      mx[i] = max(m & 0xffffu, m >> 16);
     }
-    const uint32_t other = __shfl_xor_sync(0xffffffffu, word, 1);
-    if (!(lane & 1)) *reinterpret_cast<uint32_t*>(rec + which * G::kV + slot * G::kRow + 2 * quad) = word | (other << 16);
-    if (quad < G::kGroups)
-      *reinterpret_cast<unsigned short*>(rec + G::kAmax + slot * G::kAmaxTok + 2 * (which * G::kGroups + quad)) = (unsigned short)mx[i];
+    if constexpr (D == 256) {                     // registers 0, 1 are K, 2, 3 are V; both quads of a lane are in group lane % 8
+      mx[0] = mx[1] = max(mx[0], mx[1]);
+      mx[2] = mx[3] = max(mx[2], mx[3]);
+    }
+#pragma unroll
+    for (int i = 0; i < kRegs; ++i) {
+      if (D == 256 && (i & 1)) { mx[i] = mx[i - 1]; continue; }
+#pragma unroll
+      for (int o = G::kGroups; o < (kQuads < 32 ? kQuads : 32); o <<= 1) mx[i] = max(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], o));
+    }
+    uint8_t* rec = p.data + ((size_t)page * p.Hkv + h0 + n) * G::kRecord;
+#pragma unroll
+    for (int i = 0; i < kRegs; ++i) {
+      const int idx = lane + 32 * i, which = idx / kQuads, quad = idx % kQuads;
+      const int e = (int)(mx[i] >> 7);                    // biased exponent of the maximum
+      const float scale = __uint_as_float((uint32_t)max(254 - e, 1) << 23), top = __uint_as_float(mx[i] << 16) * scale;
+      float r;
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(top));
+      const bool ok = mx[i] > 0u && mx[i] < 0x7f80u;      // an empty group has codes of zero; one that is not finite reads back as NaN
+      uint32_t word = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const uint32_t b = j < 2 ? x[n][i].x : x[n][i].y;
+        const float f = (j & 1) ? bf16hi_to_f(b) : bf16lo_to_f(b);
+        const float x7 = f * scale * 7.f, t = x7 * r;
+        const float q = fmaf(fmaf(-t, top, x7), r, t) + 12582920.f;      // 1.5 * 2^23 + 8: the code in the last bits
+        word |= (ok ? __float_as_uint(q) & 15u : 8u) << (4 * j);
+      }
+      const uint32_t other = __shfl_xor_sync(0xffffffffu, word, 1);
+      if (!(lane & 1)) *reinterpret_cast<uint32_t*>(rec + which * G::kV + slot * G::kRow + 2 * quad) = word | (other << 16);
+      if (quad < G::kGroups)
+        *reinterpret_cast<unsigned short*>(rec + G::kAmax + slot * G::kAmaxTok + 2 * (which * G::kGroups + quad)) = (unsigned short)mx[i];
+    }
+    if (p.mass && lane == 0) p.mass[((size_t)page * p.Hkv + h0 + n) * kPage + slot] = 0.f;
   }
-  if (p.mass && lane == 0) p.mass[((size_t)page * p.Hkv + h) * kPage + slot] = 0.f;
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -102,52 +117,48 @@ struct GatherParams {
   int T, Hkv, vec;
 };
 
-// x / 7 rounded correctly: one Newton correction of the product with the rounded reciprocal (Markstein).
-__device__ __forceinline__ float div7(float x) {
-  constexpr float r = 1.f / 7.f;
-  const float y = x * r;
-  const float z = fmaf(fmaf(-7.f, y, x), r, y);
-  return isfinite(z) ? z : y;
-}
-
-// One thread per 8 elements (a word of codes) of K or V: T * Hkv * 2 * D / 8 words a sequence.
+// One CTA per (page, kv head, sequence): the record is read once, 8 elements (a word of codes) a thread and turn.  code * maximum / 7
+// is a ratio of integers of 11 and 3 bits: it is a bf16 or lies at least 2^-12 from a rounding boundary, so the product with the
+// rounded seventh of the maximum rounds to the same bf16 as the exact value.
 template <int D>
-__global__ void __launch_bounds__(256) gather_kernel(const GatherParams p) {
+__global__ void __launch_bounds__(128) gather_kernel(const GatherParams p) {
   using G = Geo<D>;
-  constexpr int kWords = D / 8;
-  const int s = blockIdx.y;
+  constexpr int kWords = D / 8, kTurns = 2 * kPage * kWords / 128;
+  const int s = blockIdx.z, h = blockIdx.y, pg = blockIdx.x;
   const int slot = p.slots ? p.slots[s] : s;
   const int len = p.lengths ? min(p.lengths[s], p.T) : p.T;
-  const long i = (long)blockIdx.x * blockDim.x + threadIdx.x;
-  const int w = (int)(i % kWords);
-  const int which = (int)(i / kWords % 2);
-  const long th = i / (2 * kWords);
-  const int h = (int)(th % p.Hkv);
-  const long tok = th / p.Hkv;
-  if (tok >= len) return;
-  const int page = page_of(p.t, slot, (int)(tok / kPage));
+  if (pg * kPage >= len) return;
+  const int page = page_of(p.t, slot, pg);
   if (page < 0) return;
-  const int in = (int)(tok % kPage);
   const uint8_t* rec = p.data + ((size_t)page * p.Hkv + h) * G::kRecord;
-  const uint32_t c = *reinterpret_cast<const uint32_t*>(rec + which * G::kV + in * G::kRow + 4 * w);
-  const unsigned short* am = reinterpret_cast<const unsigned short*>(rec + G::kAmax + in * G::kAmaxTok) + which * G::kGroups;
-  const float a0 = __uint_as_float((uint32_t)am[(2 * w) % G::kGroups] << 16);
-  const float a1 = __uint_as_float((uint32_t)am[(2 * w + 1) % G::kGroups] << 16);
-  uint32_t o[4];
+  uint32_t c[kTurns];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float a = j < 2 ? a0 : a1;
-    const float lo = 0.125f * (float)((int)((c >> (8 * j)) & 15u) - 8), hi = 0.125f * (float)((int)((c >> (8 * j + 4)) & 15u) - 8);
-    o[j] = pack_bf16x2(8.f * div7(lo * a), 8.f * div7(hi * a));      // an eighth on the way: code * maximum may exceed fp32
-  }
-  bf16* dst = which ? p.out_v + s * p.batch_v + tok * p.ld_v : p.out_k + s * p.batch_k + tok * p.ld_k;
-  dst += (size_t)h * D + 8 * w;
-  if (p.vec) {
-    *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
-  } else {
-    unsigned short* d = reinterpret_cast<unsigned short*>(dst);
+  for (int k = 0; k < kTurns; ++k) c[k] = __ldg(reinterpret_cast<const uint32_t*>(rec) + threadIdx.x + 128 * k);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) { d[2 * j] = (unsigned short)o[j]; d[2 * j + 1] = (unsigned short)(o[j] >> 16); }
+  for (int k = 0; k < kTurns; ++k) {
+    const int i = threadIdx.x + 128 * k, which = i / (kPage * kWords), in = i / kWords % kPage, w = i % kWords;
+    const int tok = pg * kPage + in;
+    if (tok >= len) continue;
+    const uint32_t am = __ldg(reinterpret_cast<const uint32_t*>(rec + G::kAmax + in * G::kAmaxTok + 2 * which * G::kGroups) + w % (G::kGroups / 2));
+    const float a[2] = {bf16lo_to_f(am) * (1.f / 7.f), bf16hi_to_f(am) * (1.f / 7.f)};
+    uint32_t o[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      float v[2];
+#pragma unroll
+      for (int y = 0; y < 2; ++y)                        // 2^23 + code, less 2^23 + 8
+        v[y] = (__uint_as_float(((c[k] >> (8 * j + 4 * y)) & 15u) | 0x4b000000u) - 8388616.f) * a[j >> 1];
+      o[j] = pack_bf16x2(v[0], v[1]);
+    }
+    bf16* dst = which ? p.out_v + s * p.batch_v + tok * p.ld_v : p.out_k + s * p.batch_k + tok * p.ld_k;
+    dst += (size_t)h * D + 8 * w;
+    if (p.vec) {
+      *reinterpret_cast<uint4*>(dst) = make_uint4(o[0], o[1], o[2], o[3]);
+    } else {
+      unsigned short* d = reinterpret_cast<unsigned short*>(dst);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) { d[2 * j] = (unsigned short)o[j]; d[2 * j + 1] = (unsigned short)(o[j] >> 16); }
+    }
   }
 }
 
@@ -170,75 +181,149 @@ __device__ __forceinline__ uint32_t order_key(float f) {
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
-constexpr int kSelThreads = 1024;
+constexpr int kSelThreads = 1024, kSelBins = 2048;
+constexpr int kSelKeys = 16384;          // keys that a CTA keeps in shared memory
 
-// One CTA per (kv head, sequence).  Radix selection: four passes of 8 bits over the tokens that are neither among the first
-// `sink` nor the last `recent` find the key of the last token that stays and how many tokens of exactly that key do; one
-// more pass writes the kept positions in order.
-__global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectParams p) {
-  __shared__ int hist[256];
-  __shared__ uint32_t s_prefix;
-  __shared__ int s_need;
-  __shared__ int w_eq[kSelThreads / 32], w_keep[kSelThreads / 32];
-  const int h = blockIdx.x, s = blockIdx.y;
+__device__ __forceinline__ void cluster_sync_() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ int cluster_load(const int* local, int rank) {      // the same variable of another CTA of the cluster
+  uint32_t a;
+  int v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(local)), "r"(rank));
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+// Inclusive sums over the CTA's threads.
+__device__ __forceinline__ int block_scan(int v, int* warp_sums) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += y;
+  }
+  if (lane == 31) warp_sums[warp] = v;
+  __syncthreads();
+  int before = lane < warp ? warp_sums[lane] : 0;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+  __syncthreads();
+  return v + before;
+}
+
+// One cluster of CTAs per (kv head, sequence), each with a stretch of the tokens whose keys it reads once into shared memory (a
+// stretch too long for that is read again in every pass).  Radix selection: three passes of 11, 11 and 10 bits over the tokens
+// that are neither among the first `sink` nor the last `recent` find the key of the last token that stays and how many tokens
+// of exactly that key do, the earliest ones; the histograms of the cluster are added through distributed shared memory.  Then
+// every warp writes the kept positions of its own stretch behind those of the stretches before it.
+__global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectParams p, int nctas) {
+  extern __shared__ __align__(16) uint32_t keys[];       // [kSelKeys]
+  __shared__ int hist[kSelBins];
+  __shared__ int warp_sums[32], w_eq[33], w_gt[33], s_bin, s_left, tot[2];
+  const int rank = (int)(blockIdx.x % nctas), h = blockIdx.x / nctas, s = blockIdx.y;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int slot = p.slots ? p.slots[s] : s;
   const int n = max(0, min(p.lengths[s], p.t.width * kPage));
   int* out = p.idx + ((size_t)s * p.Hkv + h) * p.keep;
   if (n <= p.keep) {
-    for (int i = tid; i < p.keep; i += kSelThreads) out[i] = i < n ? i : -1;
+    for (int i = rank * kSelThreads + tid; i < p.keep; i += nctas * kSelThreads) out[i] = i < n ? i : -1;
     return;
   }
   const int lo = min(p.sink, n), hi = max(n - p.recent, lo);
-  auto key = [&](int t) -> uint32_t {
+  const int per = (n + nctas * kPage - 1) / (nctas * kPage) * kPage;
+  const int beg = min(rank * per, n), end = min(beg + per, n), len = end - beg;
+  const bool cached = per <= kSelKeys;
+  auto key_of = [&](int t) -> uint32_t {
     const int page = page_of(p.t, slot, t / kPage);
     return page < 0 ? 0u : order_key(__ldg(p.mass + ((size_t)page * p.Hkv + h) * kPage + t % kPage));
   };
+  if (cached) {                                          // four tokens of a page a thread
+    for (int i = 4 * tid; i < len; i += 4 * kSelThreads) {
+      const int page = page_of(p.t, slot, (beg + i) / kPage);
+      uint4 k = make_uint4(0u, 0u, 0u, 0u);
+      if (page >= 0) {
+        const float4 m = __ldg(reinterpret_cast<const float4*>(p.mass + ((size_t)page * p.Hkv + h) * kPage + (beg + i) % kPage));
+        k = make_uint4(order_key(m.x), order_key(m.y), order_key(m.z), order_key(m.w));
+      }
+      *reinterpret_cast<uint4*>(keys + i) = k;
+    }
+  }
+  auto key = [&](int t) -> uint32_t { return cached ? keys[t - beg] : key_of(t); };
+  const int want = p.keep - lo - (n - hi);               // tokens to take from [lo, hi); fewer than there are
   uint32_t prefix = 0;
-  int need = p.keep - lo - (n - hi);                        // tokens to take from [lo, hi); fewer than there are
-  for (int shift = 24; shift >= 0 && need > 0; shift -= 8) {
-    if (tid < 256) hist[tid] = 0;
+  int need = want;
+  const int from = max(beg, lo), to = min(end, hi);
+#pragma unroll 1
+  for (int pass = 0; pass < 3 && want > 0; ++pass) {
+    const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
+    const uint32_t digits = pass == 2 ? 1023u : 2047u;
+    const int above = pass == 1 ? 21 : 10;               // bits below those that are settled
+    for (int b = tid; b < kSelBins; b += kSelThreads) hist[b] = 0;
     __syncthreads();
-    for (int t = lo + tid; t < hi; t += kSelThreads) {
-      const uint32_t k = key(t);
-      if (shift == 24 || (k >> (shift + 8)) == prefix) atomicAdd(&hist[(k >> shift) & 255u], 1);
+    for (int base = from; base < to; base += kSelThreads) {
+      const int t = base + tid;
+      const uint32_t k = t < to ? key(t) : 0u;
+      const bool in = t < to && (pass == 0 || (k >> above) == prefix);
+      // tokens that were never looked at share one key: a warp counts them together
+      const bool zero = in && k == 0x80000000u;
+      const uint32_t zeros = __ballot_sync(0xffffffffu, zero);
+      if (in && !zero) atomicAdd(&hist[(k >> shift) & digits], 1);
+      if (zeros && lane == 0) atomicAdd(&hist[(0x80000000u >> shift) & digits], __popc(zeros));
     }
-    __syncthreads();
-    if (tid == 0) {
-      int left = need, b = 255;
-      while (b > 0 && hist[b] < left) left -= hist[b--];
-      s_prefix = (prefix << 8) | (uint32_t)b;
-      s_need = left;
+    cluster_sync_();
+    // bins in falling order, two a thread
+    const int b1 = kSelBins - 1 - 2 * tid, b0 = b1 - 1;
+    int c1 = 0, c0 = 0;
+    for (int r = 0; r < nctas; ++r) { c1 += cluster_load(&hist[b1], r); c0 += cluster_load(&hist[b0], r); }
+    const int sum = block_scan(c1 + c0, warp_sums), before = sum - c1 - c0;
+    if (before < need && need <= sum) {
+      const bool first = need <= before + c1;
+      s_bin = first ? b1 : b0;
+      s_left = need - before - (first ? 0 : c1);
     }
-    __syncthreads();
-    prefix = s_prefix;
-    need = s_need;
+    cluster_sync_();                                     // s_bin is there; nobody reads this pass's histogram any more
+    prefix = pass == 2 ? (prefix << 10) | (uint32_t)s_bin : (prefix << 11) | (uint32_t)s_bin;
+    need = s_left;
   }
-  // prefix: the key of the last kept token; need: how many tokens with that key stay, the earliest ones
-  const bool none = p.keep - lo - (n - hi) == 0;
-  int eq0 = 0, out0 = 0;
-  for (int t0 = 0; t0 < n; t0 += kSelThreads) {
-    const int t = t0 + tid;
+  if (cached) __syncthreads();                           // (no pass has run where nothing is wanted)
+  // prefix: the key of the last kept token; need: how many tokens with that key stay
+  auto judge = [&](int t, bool& gt, bool& eq) {
     const bool cand = t >= lo && t < hi;
-    const uint32_t k = (cand && !none) ? key(t) : 0u;
-    const bool eq = cand && !none && k == prefix;
-    const uint32_t eqs = __ballot_sync(0xffffffffu, eq);
-    if (lane == 0) w_eq[warp] = __popc(eqs);
-    __syncthreads();
-    int before = eq0, all_eq = 0;
-    for (int w = 0; w < kSelThreads / 32; ++w) { before += w < warp ? w_eq[w] : 0; all_eq += w_eq[w]; }
-    before += __popc(eqs & ((1u << lane) - 1u));
-    const bool keep = t < n && (!cand || (!none && (k > prefix || (eq && before < need))));
-    const uint32_t ks = __ballot_sync(0xffffffffu, keep);
-    if (lane == 0) w_keep[warp] = __popc(ks);
-    __syncthreads();
-    int at = out0, all_keep = 0;
-    for (int w = 0; w < kSelThreads / 32; ++w) { at += w < warp ? w_keep[w] : 0; all_keep += w_keep[w]; }
-    at += __popc(ks & ((1u << lane) - 1u));
-    if (keep && at < p.keep) out[at] = t;
-    eq0 += all_eq;
-    out0 += all_keep;
+    const uint32_t k = (cand && want > 0) ? key(t) : 0u;
+    gt = !cand || (want > 0 && k > prefix);
+    eq = cand && want > 0 && k == prefix;
+  };
+  const int wper = (len + 32 * 32 - 1) / (32 * 32) * 32, wbeg = beg + min(warp * wper, len), wend = min(wbeg + wper, end);
+  int n_gt = 0, n_eq = 0;
+  for (int t = wbeg + lane; t < wend; t += 32) {
+    bool gt, eq;
+    judge(t, gt, eq);
+    n_gt += gt; n_eq += eq;
   }
+  n_gt = __reduce_add_sync(0xffffffffu, n_gt);
+  n_eq = __reduce_add_sync(0xffffffffu, n_eq);
+  if (lane == 0) { w_gt[warp] = n_gt; w_eq[warp] = n_eq; }
+  __syncthreads();
+  if (tid == 0) {
+    int a = 0, b = 0;
+    for (int w = 0; w < 32; ++w) { a += w_gt[w]; b += w_eq[w]; }
+    tot[0] = a; tot[1] = b;
+  }
+  cluster_sync_();
+  int gt_before = 0, eq_before = 0;
+  for (int r = 0; r < rank; ++r) { gt_before += cluster_load(&tot[0], r); eq_before += cluster_load(&tot[1], r); }
+  for (int w = 0; w < warp; ++w) { gt_before += w_gt[w]; eq_before += w_eq[w]; }
+  for (int t0 = wbeg; t0 < wend; t0 += 32) {
+    const int t = t0 + lane;
+    bool gt = false, eq = false;
+    if (t < wend) judge(t, gt, eq);
+    const uint32_t gts = __ballot_sync(0xffffffffu, gt), eqs = __ballot_sync(0xffffffffu, eq), under = (1u << lane) - 1u;
+    const int eq_here = eq_before + __popc(eqs & under);
+    if (gt || (eq && eq_here < need)) out[gt_before + __popc(gts & under) + min(eq_here, need)] = t;
+    gt_before += __popc(gts);
+    eq_before += __popc(eqs);
+  }
+  cluster_sync_();                                       // the totals stay readable until everybody has read them
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -253,34 +338,50 @@ struct CompactParams {
   int Hkv, keep;
 };
 
-// One CTA of 8-byte movers per (page of 16 kept tokens, kv head, sequence): codes and maxima are copied as they are.
+// One CTA per (four pages of kept tokens, kv head, sequence): the sources of its 64 tokens are looked up side by side, then codes and
+// maxima are copied as they are, 16 bytes (the maxima at head_dim 64: 8) a thread and turn, loads ahead of stores.
+constexpr int kMoveTokens = 64;
 template <int D>
-__global__ void __launch_bounds__(128) compact_kernel(const CompactParams p) {
+__global__ void __launch_bounds__(256) compact_kernel(const CompactParams p) {
   using G = Geo<D>;
-  constexpr int kUnits = (2 * G::kRow + G::kAmaxTok) / 8;   // 8-byte units of a token
-  const int s = blockIdx.z, h = blockIdx.y, pg = blockIdx.x;
-  const int dst = p.dst[(size_t)s * p.dst_stride + pg];
-  if ((unsigned)dst >= (unsigned)p.src.pages) return;
-  const int slot = p.slots ? p.slots[s] : s;
-  const int* idx = p.idx + ((size_t)s * p.Hkv + h) * p.keep + (size_t)pg * kPage;
-  const size_t dbase = (size_t)dst * p.Hkv + h;
-  for (int i = threadIdx.x; i < kPage * kUnits; i += blockDim.x) {
-    const int tok = i / kUnits, u = i % kUnits;
-    if (pg * kPage + tok >= p.keep) continue;
-    const int from = idx[tok];
-    if (from < 0) continue;
-    const int page = page_of(p.src, slot, from / kPage);
-    if (page < 0) continue;
-    const size_t sbase = (size_t)page * p.Hkv + h;
-    const int in = from % kPage;
-    constexpr int kRowUnits = G::kRow / 8;
-    auto off = [&](int r) {
-      return u < kRowUnits ? r * G::kRow + 8 * u
-                           : (u < 2 * kRowUnits ? G::kV + r * G::kRow + 8 * (u - kRowUnits) : G::kAmax + r * G::kAmaxTok + 8 * (u - 2 * kRowUnits));
-    };
-    *reinterpret_cast<uint2*>(p.data + dbase * G::kRecord + off(tok)) = *reinterpret_cast<const uint2*>(p.data + sbase * G::kRecord + off(in));
-    if (u == 0 && p.mass) p.mass[dbase * kPage + tok] = p.mass[sbase * kPage + in];
+  constexpr int kRowUnits = G::kRow / 16;                // units of a token's K (or V) codes
+  constexpr int kTurns = kMoveTokens * 2 * kRowUnits / 256;
+  __shared__ long long from[kMoveTokens], to[kMoveTokens];       // (page * kv heads + head) * 16 + place; -1: nothing to move
+  const int s = blockIdx.z, h = blockIdx.y, j0 = blockIdx.x * kMoveTokens;
+  if (threadIdx.x < kMoveTokens) {
+    const int j = j0 + threadIdx.x;
+    long long a = -1, b = -1;
+    if (j < p.keep) {
+      const int t = p.idx[((size_t)s * p.Hkv + h) * p.keep + j], dst = p.dst[(size_t)s * p.dst_stride + j / kPage];
+      const int page = t < 0 ? -1 : page_of(p.src, p.slots ? p.slots[s] : s, t / kPage);
+      if (page >= 0 && (unsigned)dst < (unsigned)p.src.pages) {
+        a = ((long long)page * p.Hkv + h) * kPage + t % kPage;
+        b = ((long long)dst * p.Hkv + h) * kPage + j % kPage;
+        if (p.mass) p.mass[b] = p.mass[a];
+      }
+    }
+    from[threadIdx.x] = a; to[threadIdx.x] = b;
   }
+  __syncthreads();
+  auto record = [&](long long at) { return p.data + (size_t)(at / kPage) * G::kRecord; };
+  uint4 v[kTurns];
+#pragma unroll
+  for (int k = 0; k < kTurns; ++k) {
+    const int i = threadIdx.x + 256 * k, tok = i / (2 * kRowUnits), u = i % (2 * kRowUnits);
+    const long long a = from[tok];
+    if (a >= 0) v[k] = *reinterpret_cast<const uint4*>(record(a) + (u / kRowUnits) * G::kV + (int)(a % kPage) * G::kRow + 16 * (u % kRowUnits));
+  }
+  constexpr int kAmaxUnits = G::kAmaxTok / 8;
+  uint2 m;
+  const int mt = threadIdx.x / kAmaxUnits, mu = threadIdx.x % kAmaxUnits;
+  if (mt < kMoveTokens && from[mt] >= 0) m = *reinterpret_cast<const uint2*>(record(from[mt]) + G::kAmax + (int)(from[mt] % kPage) * G::kAmaxTok + 8 * mu);
+#pragma unroll
+  for (int k = 0; k < kTurns; ++k) {
+    const int i = threadIdx.x + 256 * k, tok = i / (2 * kRowUnits), u = i % (2 * kRowUnits);
+    const long long b = to[tok];
+    if (b >= 0) *reinterpret_cast<uint4*>(record(b) + (u / kRowUnits) * G::kV + (int)(b % kPage) * G::kRow + 16 * (u % kRowUnits)) = v[k];
+  }
+  if (mt < kMoveTokens && from[mt] >= 0) *reinterpret_cast<uint2*>(record(to[mt]) + G::kAmax + (int)(to[mt] % kPage) * G::kAmaxTok + 8 * mu) = m;
 }
 
 }  // namespace
@@ -308,7 +409,11 @@ GRM_API int grm_kv4_append(const void* words, void* stream) {
   p.vec = a.num() != 0;
   if (!fits(M, 1, 0x7fffffff) || !fits(Hkv, 1, 0x7fffffff) || (M * Hkv + 3) / 4 > 0x7fffffffL) return -2;
   p.M = (int)M; p.Hkv = (int)Hkv;
-  KV4_DISPATCH(D, (append_kernel<DD><<<(unsigned)((M * Hkv + 3) / 4), 128, 0, (cudaStream_t)stream>>>(p)));
+  if (M * Hkv < 8192) {
+    KV4_DISPATCH(D, (append_kernel<DD, 1><<<(unsigned)((M * Hkv + 3) / 4), 128, 0, (cudaStream_t)stream>>>(p)));
+  } else {
+    KV4_DISPATCH(D, (append_kernel<DD, 4><<<(unsigned)((M * ((Hkv + 3) / 4) + 3) / 4), 128, 0, (cudaStream_t)stream>>>(p)));
+  }
   GRM_LAUNCH_RET();
 }
 
@@ -323,11 +428,9 @@ GRM_API int grm_kv4_gather(const void* words, void* stream) {
   p.ld_k = a.num(); p.ld_v = a.num(); p.batch_k = a.num(); p.batch_v = a.num();
   const long S = a.num(), T = a.num(), Hkv = a.num(), D = a.num();
   p.vec = a.num() != 0;
-  if (!fits(S, 1, 65535) || !fits(T, 1, 0x7fffffff) || !fits(Hkv, 1, 0x7fffffff)) return -2;
+  if (!fits(S, 1, 65535) || !fits(T, 1, 0x7fffffff - kPage) || !fits(Hkv, 1, 65535)) return -2;
   p.T = (int)T; p.Hkv = (int)Hkv;
-  const long blocks = (T * Hkv * (D / 4) + 255) / 256;
-  if (blocks > 0x7fffffffL) return -2;
-  KV4_DISPATCH(D, (gather_kernel<DD><<<dim3((unsigned)blocks, (unsigned)S), 256, 0, (cudaStream_t)stream>>>(p)));
+  KV4_DISPATCH(D, (gather_kernel<DD><<<dim3((unsigned)((T + kPage - 1) / kPage), (unsigned)Hkv, (unsigned)S), 128, 0, (cudaStream_t)stream>>>(p)));
   GRM_LAUNCH_RET();
 }
 
@@ -341,7 +444,25 @@ GRM_API int grm_kv4_select(const void* words, void* stream) {
   const long S = a.num(), Hkv = a.num(), keep = a.num(), recent = a.num(), sink = a.num();
   if (!fits(S, 1, 65535) || !fits(Hkv, 1, 0x7fffffff) || !fits(keep, 1, 0x7fffffff) || !fits(recent, 0, keep) || !fits(sink, 0, keep - recent)) return -2;
   p.Hkv = (int)Hkv; p.keep = (int)keep; p.recent = (int)recent; p.sink = (int)sink;
-  select_kernel<<<dim3((unsigned)Hkv, (unsigned)S), kSelThreads, 0, (cudaStream_t)stream>>>(p);
+  // CTAs a (kv head, sequence): a stretch of up to 4096 tokens is quickest in one (no sums across CTAs); longer ones are shared by up
+  // to eight, as many as leave every CTA a place on the GPU at once
+  int dev = 0, sms = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (e != cudaSuccess) return (int)e;
+  int n = 1;
+  while (n < 8 && (long)p.t.width * kPage > 4096L * n && (S * Hkv * n < sms || (long)p.t.width * kPage > (long)kSelKeys * n)) n *= 2;
+  if (Hkv * n > 0x7fffffffL) return -2;
+  e = cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelKeys * 4);
+  if (e != cudaSuccess) return (int)e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(Hkv * n), (unsigned)S); cfg.blockDim = dim3(kSelThreads); cfg.dynamicSmemBytes = kSelKeys * 4; cfg.stream = (cudaStream_t)stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)n; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+  cfg.attrs = at; cfg.numAttrs = 1;
+  e = cudaLaunchKernelEx(&cfg, select_kernel, p, n);
+  if (e != cudaSuccess) return (int)e;
   GRM_LAUNCH_RET();
 }
 
@@ -353,8 +474,8 @@ GRM_API int grm_kv4_compact(const void* words, void* stream) {
   if (!read_table(a, p.src)) return -2;
   p.slots = a.ptr<const int>(); p.idx = a.ptr<const int>(); p.dst = a.ptr<const int>(); p.dst_stride = a.num();
   const long S = a.num(), Hkv = a.num(), D = a.num(), keep = a.num();
-  if (!fits(S, 1, 65535) || !fits(Hkv, 1, 65535) || !fits(keep, 1, 0x7fffffff - kPage)) return -2;
+  if (!fits(S, 1, 65535) || !fits(Hkv, 1, 65535) || !fits(keep, 1, 0x7fffffff - kMoveTokens)) return -2;
   p.Hkv = (int)Hkv; p.keep = (int)keep;
-  KV4_DISPATCH(D, (compact_kernel<DD><<<dim3((unsigned)((keep + kPage - 1) / kPage), (unsigned)Hkv, (unsigned)S), 128, 0, (cudaStream_t)stream>>>(p)));
+  KV4_DISPATCH(D, (compact_kernel<DD><<<dim3((unsigned)((keep + kMoveTokens - 1) / kMoveTokens), (unsigned)Hkv, (unsigned)S), 256, 0, (cudaStream_t)stream>>>(p)));
   GRM_LAUNCH_RET();
 }

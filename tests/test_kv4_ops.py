@@ -645,3 +645,46 @@ def test_offsets_beyond_32_bits():
     kv4.kv4_attn(q.cuda(), pos[:1], pos[39:], table, kv, AttnGeom(Hkv * G, Hkv, D, D, 1 / 16), out, 40)
     r = [attend64(q.reshape(Hkv, G, D)[h], k4[:, h], v4[:, h], 39, 1 / 16, 0) for h in range(Hkv)]
     close(out.cpu(), torch.cat([x[0].flatten() for x in r])[None], torch.cat([x[1].flatten() for x in r])[None])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("width,n,keep", [(700, 1500, 300), (1300, 9000, 4000), (4000, 40000, 777)])
+def test_selection_of_long_sequences_and_wide_tables(device, width, n, keep):
+    """Sequences that several CTAs share, short ones in a wide table among them."""
+    g = torch.Generator().manual_seed(n)
+    P = (n + PAGE - 1) // PAGE + 2
+    kv = kv4.Kv4Layer.alloc(P, 1, 64, device, mass=True)
+    m = torch.exp(3 * torch.randn(P, 1, PAGE, generator=g)) * (torch.rand(P, 1, PAGE, generator=g) < 0.6)
+    kv.mass.copy_(m)
+    table = torch.full((3, width), -1, dtype=torch.int32)
+    pages = (n + PAGE - 1) // PAGE
+    table[1, :pages] = torch.randperm(P, generator=g)[:pages].to(torch.int32)
+    table[2, :20] = table[1, :20]
+    lens = [n, 300, 5]
+    idx = kv4.kv4_select(kv, torch.tensor([1, 2, 2], dtype=torch.int32, device=device), torch.tensor(lens, dtype=torch.int32, device=device),
+                         table.to(device), keep, 16, 4)
+    for s, (slot, k) in enumerate(zip((1, 2, 2), lens)):
+        t = torch.arange(k)
+        mass = m[table[slot, t // PAGE].long(), 0, t % PAGE]
+        assert idx[s, 0].tolist() == expected_kept(mass.tolist(), k, keep, 16, 4)
+
+
+@pytest.mark.gpu
+def test_selection_of_a_sequence_longer_than_the_cluster_keeps():
+    n, keep = 150_000, 5000
+    P = n // PAGE + 1
+    kv = kv4.Kv4Layer.alloc(P, 1, 64, "cuda", mass=True)
+    kv.mass.copy_(torch.randint(0, 40, kv.mass.shape, generator=torch.Generator().manual_seed(2)).float())
+    table = torch.arange(P, dtype=torch.int32, device="cuda")[None]
+    idx = kv4.kv4_select(kv, None, torch.tensor([n], dtype=torch.int32, device="cuda"), table, keep, 100, 4)
+    assert idx[0, 0].tolist() == expected_kept(kv.mass.flatten()[:n].tolist(), n, keep, 100, 4)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_append_of_many_rows_over_an_odd_number_of_heads(device, D):
+    n, Hkv = 2800, 3
+    c = Cache([n], Hkv, D, device, seed=D)
+    ok, ov = (torch.zeros(1, n, Hkv * D, dtype=torch.bfloat16, device=device) for _ in range(2))
+    kv4.kv4_gather(c.kv, c.table, c.slots.to(device), None, ok, ov)
+    assert torch.equal(ok[0].cpu(), c.k[0].reshape(n, -1).bfloat16()) and torch.equal(ov[0].cpu(), c.v[0].reshape(n, -1).bfloat16())
