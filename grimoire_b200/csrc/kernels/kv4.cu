@@ -34,6 +34,7 @@ template <int D, int kHeads>
 __global__ void __launch_bounds__(128) append_kernel(const AppendParams p) {
   using G = Geo<D>;
   constexpr int kQuads = D / 4, kRegs = (2 * kQuads + 31) / 32;
+  grm_pdl_wait();
   const long wid = ((long)blockIdx.x * blockDim.x + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31;
   const int sets = (p.Hkv + kHeads - 1) / kHeads;
@@ -125,6 +126,7 @@ __global__ void __launch_bounds__(128) gather_kernel(const GatherParams p) {
   using G = Geo<D>;
   constexpr int kWords = D / 8, kTurns = 2 * kPage * kWords / 128;
   const int s = blockIdx.z, h = blockIdx.y, pg = blockIdx.x;
+  grm_pdl_wait();
   const int slot = p.slots ? p.slots[s] : s;
   const int len = p.lengths ? min(p.lengths[s], p.T) : p.T;
   if (pg * kPage >= len) return;
@@ -222,6 +224,7 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectParams 
   __shared__ int warp_sums[32], w_eq[33], w_gt[33], s_bin, s_left, tot[2];
   const int rank = (int)(blockIdx.x % nctas), h = blockIdx.x / nctas, s = blockIdx.y;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  grm_pdl_wait();
   const int slot = p.slots ? p.slots[s] : s;
   const int n = max(0, min(p.lengths[s], p.t.width * kPage));
   int* out = p.idx + ((size_t)s * p.Hkv + h) * p.keep;
@@ -348,6 +351,7 @@ __global__ void __launch_bounds__(256) compact_kernel(const CompactParams p) {
   constexpr int kTurns = kMoveTokens * 2 * kRowUnits / 256;
   __shared__ long long from[kMoveTokens], to[kMoveTokens];       // (page * kv heads + head) * 16 + place; -1: nothing to move
   const int s = blockIdx.z, h = blockIdx.y, j0 = blockIdx.x * kMoveTokens;
+  grm_pdl_wait();
   if (threadIdx.x < kMoveTokens) {
     const int j = j0 + threadIdx.x;
     long long a = -1, b = -1;
@@ -386,11 +390,12 @@ __global__ void __launch_bounds__(256) compact_kernel(const CompactParams p) {
 
 }  // namespace
 
-#define KV4_DISPATCH(D, CALL)                                   \
+// CALL, which returns, with DD for the head dimension
+#define KV4_DISPATCH(D, ...)                                    \
   switch (D) {                                                  \
-    case 64: { constexpr int DD = 64; CALL; break; }            \
-    case 128: { constexpr int DD = 128; CALL; break; }          \
-    case 256: { constexpr int DD = 256; CALL; break; }          \
+    case 64: { constexpr int DD = 64; __VA_ARGS__; }            \
+    case 128: { constexpr int DD = 128; __VA_ARGS__; }          \
+    case 256: { constexpr int DD = 256; __VA_ARGS__; }          \
     default: return -2;                                         \
   }
 
@@ -410,11 +415,10 @@ GRM_API int grm_kv4_append(const void* words, void* stream) {
   if (!fits(M, 1, 0x7fffffff) || !fits(Hkv, 1, 0x7fffffff) || (M * Hkv + 3) / 4 > 0x7fffffffL) return -2;
   p.M = (int)M; p.Hkv = (int)Hkv;
   if (M * Hkv < 8192) {
-    KV4_DISPATCH(D, (append_kernel<DD, 1><<<(unsigned)((M * Hkv + 3) / 4), 128, 0, (cudaStream_t)stream>>>(p)));
+    KV4_DISPATCH(D, return (int)grm_launch_pdl(GRM_PDL_ATTN, append_kernel<DD, 1>, dim3((unsigned)((M * Hkv + 3) / 4)), dim3(128), 0, (cudaStream_t)stream, p));
   } else {
-    KV4_DISPATCH(D, (append_kernel<DD, 4><<<(unsigned)((M * ((Hkv + 3) / 4) + 3) / 4), 128, 0, (cudaStream_t)stream>>>(p)));
+    KV4_DISPATCH(D, return (int)grm_launch_pdl(GRM_PDL_ATTN, append_kernel<DD, 4>, dim3((unsigned)((M * ((Hkv + 3) / 4) + 3) / 4)), dim3(128), 0, (cudaStream_t)stream, p));
   }
-  GRM_LAUNCH_RET();
 }
 
 // data, table, slots, width, stride, pages, seq (or 0), lengths (or 0), out_k, out_v, ld_k, ld_v, batch_k, batch_v, S, T, Hkv, D,
@@ -430,8 +434,7 @@ GRM_API int grm_kv4_gather(const void* words, void* stream) {
   p.vec = a.num() != 0;
   if (!fits(S, 1, 65535) || !fits(T, 1, 0x7fffffff - kPage) || !fits(Hkv, 1, 65535)) return -2;
   p.T = (int)T; p.Hkv = (int)Hkv;
-  KV4_DISPATCH(D, (gather_kernel<DD><<<dim3((unsigned)((T + kPage - 1) / kPage), (unsigned)Hkv, (unsigned)S), 128, 0, (cudaStream_t)stream>>>(p)));
-  GRM_LAUNCH_RET();
+  KV4_DISPATCH(D, return (int)grm_launch_pdl(GRM_PDL_ATTN, gather_kernel<DD>, dim3((unsigned)((T + kPage - 1) / kPage), (unsigned)Hkv, (unsigned)S), dim3(128), 0, (cudaStream_t)stream, p));
 }
 
 // mass, table, slots, width, stride, pages, seq (or 0), lengths, idx (int32 [S][Hkv][keep]), S, Hkv, keep, recent, sink
@@ -457,13 +460,13 @@ GRM_API int grm_kv4_select(const void* words, void* stream) {
   if (e != cudaSuccess) return (int)e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(Hkv * n), (unsigned)S); cfg.blockDim = dim3(kSelThreads); cfg.dynamicSmemBytes = kSelKeys * 4; cfg.stream = (cudaStream_t)stream;
-  cudaLaunchAttribute at[1];
+  cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = (unsigned)n; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
-  cfg.attrs = at; cfg.numAttrs = 1;
-  e = cudaLaunchKernelEx(&cfg, select_kernel, p, n);
-  if (e != cudaSuccess) return (int)e;
-  GRM_LAUNCH_RET();
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = (grm_pdl_enabled() & GRM_PDL_ATTN) ? 1 : 0;
+  cfg.attrs = at; cfg.numAttrs = 2;
+  return (int)cudaLaunchKernelEx(&cfg, select_kernel, p, n);
 }
 
 // data, mass (or 0), table, slots, width, stride, pages, seq (or 0), idx, dst (int32 [S][>= ceil(keep / 16)]), dst_stride, S, Hkv, D, keep
@@ -476,6 +479,5 @@ GRM_API int grm_kv4_compact(const void* words, void* stream) {
   const long S = a.num(), Hkv = a.num(), D = a.num(), keep = a.num();
   if (!fits(S, 1, 65535) || !fits(Hkv, 1, 65535) || !fits(keep, 1, 0x7fffffff - kMoveTokens)) return -2;
   p.Hkv = (int)Hkv; p.keep = (int)keep;
-  KV4_DISPATCH(D, (compact_kernel<DD><<<dim3((unsigned)((keep + kMoveTokens - 1) / kMoveTokens), (unsigned)Hkv, (unsigned)S), 256, 0, (cudaStream_t)stream>>>(p)));
-  GRM_LAUNCH_RET();
+  KV4_DISPATCH(D, return (int)grm_launch_pdl(GRM_PDL_ATTN, compact_kernel<DD>, dim3((unsigned)((keep + kMoveTokens - 1) / kMoveTokens), (unsigned)Hkv, (unsigned)S), dim3(256), 0, (cudaStream_t)stream, p));
 }

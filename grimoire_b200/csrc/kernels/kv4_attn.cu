@@ -42,7 +42,8 @@ __device__ __forceinline__ int row_first(const AttnParams& p, int len) { return 
 
 template <int D>
 struct Ring {
-  static constexpr int kStages = D == 64 ? 3 : 2;        // of two page records each
+  static constexpr int kStages = D == 256 ? 2 : 3;       // of two page records each
+  static constexpr int kCtas = D == 256 ? 2 : 3;         // an SM: as many as the accumulators leave registers for without spills
   static constexpr int kWarpBytes = kStages * 2 * Geo<D>::kRecord + 2 * 32 * 4 * Geo<D>::kGroups;
   static constexpr int kBytes = kWarps * kWarpBytes;
 };
@@ -254,11 +255,31 @@ __device__ __forceinline__ Rows rows_of(const AttnParams& p, int u) {
   return r;
 }
 
-// Pages before each group of rows, in shared memory, by one CTA; returns the pages per CTA of the streamed schedule.
+// Pages before each group of rows, in shared memory; returns the pages per CTA of the streamed schedule.  Up to 32 groups: every
+// warp scans them in its lanes and writes the same values, so that no barrier is needed before its own reads.
+__device__ __forceinline__ int pages_per_cta(const AttnParams& p, int run) {
+  const long long total = (long long)run * p.uheads;
+  const int per = total < 0x7fffffffLL - p.ctas ? ((int)total + p.ctas - 1) / p.ctas : (int)((total + p.ctas - 1) / p.ctas);
+  return max(8, (per + 7) / 8 * 8);                      // whole steps of the four warps
+}
 __device__ __forceinline__ int stream_schedule(const AttnParams& p, int (&before)[kMaxUnits + 1]) {
   __shared__ int warp_sum_[kWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   int run = 0;
+  if (p.units <= 32) {
+    const int n = lane < p.units ? rows_of(p, lane).pages : 0;
+    int x = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    run = __shfl_sync(0xffffffffu, x, 31);
+    if (lane < p.units) before[lane] = x - n;
+    if (lane == 0) before[p.units] = run;
+    __syncwarp();
+    return pages_per_cta(p, run);
+  }
   for (int base = 0; base < p.units; base += kThreads) {
     int n = base + tid < p.units ? rows_of(p, base + tid).pages : 0, x = n;
 #pragma unroll
@@ -278,12 +299,11 @@ __device__ __forceinline__ int stream_schedule(const AttnParams& p, int (&before
   }
   if (tid == 0) before[p.units] = run;
   __syncthreads();
-  const long long total = (long long)run * p.uheads;
-  return max(8, (int)((total + p.ctas - 1) / p.ctas + 7) / 8 * 8);       // whole steps of the four warps
+  return pages_per_cta(p, run);
 }
 
 template <int D, int HH>
-__global__ void __launch_bounds__(kThreads, HH == 2 ? 3 : (D == 256 ? 3 : 4)) attn_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(kThreads, Ring<D>::kCtas) attn_kernel(const AttnParams p) {
   using Gm = Geo<D>;
   constexpr int NG = Gm::kGroups, WT = D / 64, PP = 8 * HH;
   constexpr int kStages = Ring<D>::kStages;
@@ -293,7 +313,6 @@ __global__ void __launch_bounds__(kThreads, HH == 2 ? 3 : (D == 256 ? 3 : 4)) at
   __shared__ float sm_ml[kWarps][PP][2];
   __shared__ int before[kMaxUnits + 1];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  grm_pdl_trigger();
   const Magic mg;
   uint8_t* ring = smem + (size_t)warp * Ring<D>::kWarpBytes;
   float* am_k = reinterpret_cast<float*>(ring + kStages * 2 * Gm::kRecord);                  // [32 tokens][NG]
@@ -304,6 +323,7 @@ __global__ void __launch_bounds__(kThreads, HH == 2 ? 3 : (D == 256 ? 3 : 4)) at
     mbar_fence_init();
   }
   __syncwarp();
+  grm_pdl_wait();
   uint32_t step = 0;                                     // steps of this warp so far: ring stage and barrier phase
   uint32_t limit = 4000000u;
 
@@ -640,12 +660,15 @@ __global__ void __launch_bounds__(kThreads, HH == 2 ? 3 : (D == 256 ? 3 : 4)) at
 }
 
 // Joins the parts of a unit: one CTA per (query head, row).  Groups of D / 2 threads (two dims each) take every n-th part and are
-// joined in order: the result does not depend on timing.
-constexpr int kMergeThreads = 256, kMergeParts = 512;
-template <int D>
+// joined in order: the result does not depend on timing.  Bound by the latency of its dependent loads: the parts' statistics are
+// read once, and a group keeps eight parts in flight.
+// kMergeThreads: 512 where a unit has many parts (74 of one row over 131072 tokens: 4 us less than with 256), 128 where it has few.
+constexpr int kMergeParts = 512;
+template <int D, int kMergeThreads>
 __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const AttnParams p) {
-  constexpr int kGroups = kMergeThreads / (D / 2);
-  __shared__ float wt[kMergeParts], red[kMergeThreads / 32];
+  constexpr int kGroups = kMergeThreads / (D / 2), kMergeWarps = kMergeThreads / 32;
+  __shared__ float2 wt[kMergeParts];                     // (weight, sum) of a part; a part without keys has a sum of zero
+  __shared__ float red[kMergeWarps];
   __shared__ float2 so[kGroups][D / 2];
   __shared__ float sl[kGroups];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, grp = tid / (D / 2), d = 2 * (tid % (D / 2));
@@ -658,34 +681,44 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const AttnParams p
   int n = p.splits;
   if (p.splits == 0) {
     const long long q = p.sched[0], lo = p.sched[1 + u], pages = p.sched[2 + u] - lo;
-    const long long beg = lo * p.uheads + uh * pages;
-    first = beg / q + (long)u * p.uheads + uh;
-    n = pages > 0 ? (int)((beg + pages - 1) / q - beg / q) + 1 : 0;
+    const long long beg = lo * p.uheads + uh * pages, last = beg + pages - 1;
+    long long c0, c1;
+    if (last < 0xffffffffLL) {                           // 32-bit division where it will do
+      c0 = (uint32_t)beg / (uint32_t)q; c1 = (uint32_t)last / (uint32_t)q;
+    } else {
+      c0 = beg / q; c1 = last / q;
+    }
+    first = c0 + (long)u * p.uheads + uh;
+    n = pages > 0 ? (int)(c1 - c0) + 1 : 0;
   }
   const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + first * p.pairs + pr;
   const float* po = p.part_o + (first * p.pairs + pr) * D + d;
   float mx = -INFINITY;
-  for (int s = tid; s < n; s += kMergeThreads) mx = fmaxf(mx, ml[(size_t)s * p.pairs].x);
+  for (int s = tid; s < n; s += kMergeThreads) {
+    const float2 v = ml[(size_t)s * p.pairs];
+    if (n <= kMergeParts) wt[s] = v;
+    mx = fmaxf(mx, v.x);
+  }
   mx = warp_max(mx);
   if (lane == 0) red[warp] = mx;
   __syncthreads();
 #pragma unroll
-  for (int w = 0; w < kMergeThreads / 32; ++w) mx = fmaxf(mx, red[w]);
+  for (int w = 0; w < kMergeWarps; ++w) mx = fmaxf(mx, red[w]);
   float l = 0.f, o0 = 0.f, o1 = 0.f;
-  for (int base = 0; base < n; base += kMergeParts) {    // weights of the parts; a part without keys has a sum of zero
+  for (int base = 0; base < n; base += kMergeParts) {
     const int here = min(kMergeParts, n - base);
-    __syncthreads();
     for (int s = tid; s < here; s += kMergeThreads) {
-      const float2 v = ml[(size_t)(base + s) * p.pairs];
-      wt[s] = v.y == 0.f ? 0.f : (v.x == -INFINITY ? 1.f : exp2f(v.x - mx));
+      const float2 v = n <= kMergeParts ? wt[s] : ml[(size_t)(base + s) * p.pairs];
+      wt[s] = make_float2(v.x == -INFINITY ? 1.f : exp2f(v.x - mx), v.y);
     }
     __syncthreads();
-#pragma unroll 4
+#pragma unroll 8
     for (int s = grp; s < here; s += kGroups) {
       const float2 v = *reinterpret_cast<const float2*>(po + (size_t)(base + s) * p.pairs * D);
-      const float f = wt[s], ls = ml[(size_t)(base + s) * p.pairs].y;
-      if (ls != 0.f) { l = fmaf(f, ls, l); o0 = fmaf(f, v.x, o0); o1 = fmaf(f, v.y, o1); }      // a NaN sum counts
+      const float2 f = wt[s];
+      if (f.y != 0.f) { l = fmaf(f.x, f.y, l); o0 = fmaf(f.x, v.x, o0); o1 = fmaf(f.x, v.y, o1); }      // a NaN sum counts
     }
+    __syncthreads();
   }
   so[grp][d / 2] = make_float2(o0, o1);
   if (d == 0) sl[grp] = l;
@@ -710,7 +743,8 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const AttnParams p
 // two blocks of one sequence neither race nor depend on timing.
 template <int D>
 struct MassTile {
-  static constexpr int kTiles = 2560 / D;                // tiles in shared memory at a time
+  static constexpr int kSide = D == 256 ? 2 : 4;         // tiles worked on side by side: independent chains of MMAs
+  static constexpr int kTiles = 2560 / D / kSide * kSide;       // tiles in shared memory at a time
   static constexpr int kBytes = kTiles * (32 * D / 2 + 8 * 24);       // operands, (factor, maximum, 1 / sum), (seen, first)
 };
 // The weights that a page's tokens g and g + 8 draw from the lane's pairs of every tile.
@@ -719,27 +753,33 @@ __device__ __forceinline__ void page_sums(const uint32_t (&ka)[D / 32][2][4], co
                                           int tok0, int lane, float (&sum)[2]) {
   constexpr int NG = D / 32;
   const int g = lane >> 2, t = lane & 3;
-#pragma unroll 2
-  for (int i = 0; i < tiles; ++i) {
-    float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+  for (int i0 = 0; i0 < tiles; i0 += MassTile<D>::kSide) {
+    float c[MassTile<D>::kSide][4];
 #pragma unroll
-    for (int gi = 0; gi < NG; ++gi) {
-      const uint4 q = sq[(i * NG + gi) * 32 + lane];
-      mma(c, ka[gi][0][0], ka[gi][0][1], ka[gi][0][2], ka[gi][0][3], q.x, q.y);
-      mma(c, ka[gi][1][0], ka[gi][1][1], ka[gi][1][2], ka[gi][1][3], q.z, q.w);
-    }
+    for (int i = 0; i < MassTile<D>::kSide; ++i) c[i][0] = c[i][1] = c[i][2] = c[i][3] = 0.f;
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const float4 f = sf[8 * i + 2 * t + j];
-      const int2 lim = kEdge ? sl[8 * i + 2 * t + j] : make_int2(0, 0);
-      const float k = f.x * pf;
+    for (int gi = 0; gi < NG; ++gi)
 #pragma unroll
-      for (int r = 0; r < 2; ++r) {
-        const float e = exp2_fast(fmaf(c[2 * r + j], k, -f.y));
-        const int at = tok0 + g + 8 * r;
-        if (!kEdge || (at < lim.x && at >= lim.y)) sum[r] = fmaf(e, f.z, sum[r]);
+      for (int i = 0; i < MassTile<D>::kSide; ++i) {
+        const uint4 q = sq[((i0 + i) * NG + gi) * 32 + lane];
+        mma(c[i], ka[gi][0][0], ka[gi][0][1], ka[gi][0][2], ka[gi][0][3], q.x, q.y);
+        mma(c[i], ka[gi][1][0], ka[gi][1][1], ka[gi][1][2], ka[gi][1][3], q.z, q.w);
       }
-    }
+#pragma unroll
+    for (int i = 0; i < MassTile<D>::kSide; ++i)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const float4 f = sf[8 * (i0 + i) + 2 * t + j];
+        const int2 lim = kEdge ? sl[8 * (i0 + i) + 2 * t + j] : make_int2(0, 0);
+        const float k = f.x * pf;
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float e = exp2_fast(fmaf(c[i][2 * r + j], k, -f.y));
+          const int at = tok0 + g + 8 * r;
+          if (!kEdge || (at < lim.x && at >= lim.y)) sum[r] = fmaf(e, f.z, sum[r]);
+        }
+      }
   }
 }
 
@@ -754,9 +794,10 @@ __global__ void __launch_bounds__(kThreads) mass_kernel(const AttnParams p, int 
   __shared__ int s_len, s_dup;
   const int kvh = blockIdx.y, blk = blockIdx.z;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  const int slot = p.row_seq[blk * p.block];
   const Magic mg;
   if (tid == 0) { s_len = 0; s_dup = 0; }
+  grm_pdl_wait();
+  const int slot = p.row_seq[blk * p.block];
   __syncthreads();
   for (int b = tid; b < blk; b += kThreads)
     if (p.row_seq[b * p.block] == slot) s_dup = 1;
@@ -775,7 +816,7 @@ __global__ void __launch_bounds__(kThreads) mass_kernel(const AttnParams p, int 
     if (p.row_seq[b * p.block] != slot) continue;
     const int np = p.block * p.G;
     for (int pair0 = 0; pair0 < np; pair0 += 8 * kTiles) {
-      const int tiles = min(kTiles, (np - pair0 + 7) / 8);
+      const int tiles = min(kTiles, ((np - pair0 + 7) / 8 + MassTile<D>::kSide - 1) / MassTile<D>::kSide * MassTile<D>::kSide);
       __syncthreads();
       for (int i = warp; i < tiles; i += kWarps) {
         const int pr = pair0 + 8 * i + g;
@@ -894,13 +935,15 @@ int plan(Plan& pl, long M, long Hq, long Hkv, long D, long block, long max_len) 
   pl.units = (int)units;
   pl.uheads = (int)Hkv * pl.subs;
   pl.sms = sms;
-  pl.ctas = sms * (pl.pairs == 16 || D == 256 ? 3 : 4);
+  pl.ctas = sms * (D == 256 ? Ring<256>::kCtas : Ring<128>::kCtas);
   const long cells = units * pl.uheads, pages = (max_len + kPage - 1) / kPage;
   // Streamed: every CTA gets the same number of pages of the flat list, whatever the rows' lengths, at the price of a scan over
   // the rows and of parts that begin anywhere.  Split: a fixed number of CTAs a unit, at least eight pages (a step of the four
-  // warps) each.
+  // warps) each.  Measured, us split / streamed: 8 rows of up to 4999 tokens x 8 heads (45 pages a CTA) 20.7 / 24.5, 16 rows of
+  // up to 8191 at head_dim 256 (110 pages) 51.0 / 54.1, one row of 131072 (147 pages) 47.9 / 52.7, 32 rows of up to 32768 (900
+  // pages) 320 / 231.
   pl.splits = 0;
-  if (units > kMaxUnits || cells * pages < 32L * pl.ctas) {
+  if (units > kMaxUnits || cells * pages < 256L * pl.ctas) {
     long s = pages / 8 < pl.ctas / cells ? pages / 8 : pl.ctas / cells;
     pl.splits = (int)(s < 1 ? 1 : s);
   }
@@ -925,8 +968,7 @@ int launch_attn(const AttnParams& p, cudaStream_t st) {
   static unsigned long long ready = 0;
   const cudaError_t e = allow_smem(ready, (const void*)attn_kernel<D, HH>, kSmem);
   if (e != cudaSuccess) return (int)e;
-  attn_kernel<D, HH><<<p.splits ? dim3(p.splits, p.uheads, p.units) : dim3(p.ctas), kThreads, kSmem, st>>>(p);
-  GRM_LAUNCH_RET();
+  return (int)grm_launch_pdl(GRM_PDL_ATTN, attn_kernel<D, HH>, p.splits ? dim3(p.splits, p.uheads, p.units) : dim3(p.ctas), dim3(kThreads), kSmem, st, p);
 }
 
 template <int D>
@@ -936,7 +978,10 @@ int launch(const AttnParams& p, int nblocks, int mass_pages, cudaStream_t st) {
   else rc = p.pairs == 8 ? launch_attn<D, 1>(p, st) : launch_attn<D, 2>(p, st);
   if (rc) return rc;
   if (p.splits != 1) {
-    const cudaError_t e = grm_launch_pdl(GRM_PDL_ATTN, merge_kernel<D>, dim3(p.Hkv * p.G, p.M), dim3(kMergeThreads), 0, st, p);
+    const dim3 grid(p.Hkv * p.G, p.M);
+    const bool many = (p.splits ? p.splits : p.ctas / ((long)p.units * p.uheads)) >= 16;
+    const cudaError_t e = many ? grm_launch_pdl(GRM_PDL_ATTN, merge_kernel<D, 512>, grid, dim3(512), 0, st, p)
+                               : grm_launch_pdl(GRM_PDL_ATTN, merge_kernel<D, 128>, grid, dim3(128), 0, st, p);
     if (e != cudaSuccess) return (int)e;
   }
   if (p.mass) {
@@ -947,9 +992,10 @@ int launch(const AttnParams& p, int nblocks, int mass_pages, cudaStream_t st) {
     static unsigned long long ready = 0;
     const cudaError_t e = allow_smem(ready, (const void*)mass_kernel<D>, MassTile<D>::kBytes);
     if (e != cudaSuccess) return (int)e;
-    mass_kernel<D><<<dim3((unsigned)((mass_pages + per - 1) / per), p.Hkv, nblocks), kThreads, MassTile<D>::kBytes, st>>>(p, nblocks, mass_pages, (int)per);
+    return (int)grm_launch_pdl(GRM_PDL_ATTN, mass_kernel<D>, dim3((unsigned)((mass_pages + per - 1) / per), p.Hkv, nblocks), dim3(kThreads), MassTile<D>::kBytes,
+                               st, p, nblocks, mass_pages, (int)per);
   }
-  GRM_LAUNCH_RET();
+  return 0;
 }
 
 }  // namespace
