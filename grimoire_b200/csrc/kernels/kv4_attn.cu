@@ -747,40 +747,48 @@ struct MassTile {
   static constexpr int kTiles = 2560 / D / kSide * kSide;       // tiles in shared memory at a time
   static constexpr int kBytes = kTiles * (32 * D / 2 + 8 * 24);       // operands, (factor, maximum, 1 / sum), (seen, first)
 };
-// The weights that a page's tokens g and g + 8 draw from the lane's pairs of every tile.
-template <int D, bool kEdge>
-__device__ __forceinline__ void page_sums(const uint32_t (&ka)[D / 32][2][4], const uint4* sq, const float4* sf, const int2* sl, int tiles, float pf,
+// The weights that a page's tokens g and g + 8 draw from the lane's pairs of tiles i0 .. i0 + kSide - 1, worked on side by side:
+// independent chains of MMAs.
+template <int D, bool kEdge, int kSide>
+__device__ __forceinline__ void tile_sums(const uint32_t (&ka)[D / 32][2][4], const uint4* sq, const float4* sf, const int2* sl, int i0, float pf,
                                           int tok0, int lane, float (&sum)[2]) {
   constexpr int NG = D / 32;
   const int g = lane >> 2, t = lane & 3;
+  float c[kSide][4];
+#pragma unroll
+  for (int i = 0; i < kSide; ++i) c[i][0] = c[i][1] = c[i][2] = c[i][3] = 0.f;
+#pragma unroll
+  for (int gi = 0; gi < NG; ++gi)
+#pragma unroll
+    for (int i = 0; i < kSide; ++i) {
+      const uint4 q = sq[((i0 + i) * NG + gi) * 32 + lane];
+      mma(c[i], ka[gi][0][0], ka[gi][0][1], ka[gi][0][2], ka[gi][0][3], q.x, q.y);
+      mma(c[i], ka[gi][1][0], ka[gi][1][1], ka[gi][1][2], ka[gi][1][3], q.z, q.w);
+    }
+#pragma unroll
+  for (int i = 0; i < kSide; ++i)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float4 f = sf[8 * (i0 + i) + 2 * t + j];
+      const int2 lim = kEdge ? sl[8 * (i0 + i) + 2 * t + j] : make_int2(0, 0);
+      const float k = f.x * pf;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        const float e = exp2_fast(fmaf(c[i][2 * r + j], k, -f.y));
+        const int at = tok0 + g + 8 * r;
+        if (!kEdge || (at < lim.x && at >= lim.y)) sum[r] = fmaf(e, f.z, sum[r]);
+      }
+    }
+}
+template <int D, bool kEdge>
+__device__ __forceinline__ void page_sums(const uint32_t (&ka)[D / 32][2][4], const uint4* sq, const float4* sf, const int2* sl, int tiles, float pf,
+                                          int tok0, int lane, float (&sum)[2]) {
+  constexpr int kSide = MassTile<D>::kSide;
+  int i = 0;
 #pragma unroll 1
-  for (int i0 = 0; i0 < tiles; i0 += MassTile<D>::kSide) {
-    float c[MassTile<D>::kSide][4];
-#pragma unroll
-    for (int i = 0; i < MassTile<D>::kSide; ++i) c[i][0] = c[i][1] = c[i][2] = c[i][3] = 0.f;
-#pragma unroll
-    for (int gi = 0; gi < NG; ++gi)
-#pragma unroll
-      for (int i = 0; i < MassTile<D>::kSide; ++i) {
-        const uint4 q = sq[((i0 + i) * NG + gi) * 32 + lane];
-        mma(c[i], ka[gi][0][0], ka[gi][0][1], ka[gi][0][2], ka[gi][0][3], q.x, q.y);
-        mma(c[i], ka[gi][1][0], ka[gi][1][1], ka[gi][1][2], ka[gi][1][3], q.z, q.w);
-      }
-#pragma unroll
-    for (int i = 0; i < MassTile<D>::kSide; ++i)
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const float4 f = sf[8 * (i0 + i) + 2 * t + j];
-        const int2 lim = kEdge ? sl[8 * (i0 + i) + 2 * t + j] : make_int2(0, 0);
-        const float k = f.x * pf;
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          const float e = exp2_fast(fmaf(c[i][2 * r + j], k, -f.y));
-          const int at = tok0 + g + 8 * r;
-          if (!kEdge || (at < lim.x && at >= lim.y)) sum[r] = fmaf(e, f.z, sum[r]);
-        }
-      }
-  }
+  for (; i + kSide <= tiles; i += kSide) tile_sums<D, kEdge, kSide>(ka, sq, sf, sl, i, pf, tok0, lane, sum);
+#pragma unroll 1
+  for (; i < tiles; ++i) tile_sums<D, kEdge, 1>(ka, sq, sf, sl, i, pf, tok0, lane, sum);
 }
 
 template <int D>
@@ -816,7 +824,7 @@ __global__ void __launch_bounds__(kThreads) mass_kernel(const AttnParams p, int 
     if (p.row_seq[b * p.block] != slot) continue;
     const int np = p.block * p.G;
     for (int pair0 = 0; pair0 < np; pair0 += 8 * kTiles) {
-      const int tiles = min(kTiles, ((np - pair0 + 7) / 8 + MassTile<D>::kSide - 1) / MassTile<D>::kSide * MassTile<D>::kSide);
+      const int tiles = min(kTiles, (np - pair0 + 7) / 8);
       __syncthreads();
       for (int i = warp; i < tiles; i += kWarps) {
         const int pr = pair0 + 8 * i + g;
@@ -999,10 +1007,10 @@ int launch(const AttnParams& p, int nblocks, int mass_pages, cudaStream_t st) {
     if (e != cudaSuccess) return (int)e;
   }
   if (p.mass) {
-    // pages of a CTA: at least a page a warp, otherwise one wave of CTAs (three waves lay the pairs out
-    // more often: 398 against 386 us for four prompts of 16384 tokens with 32 observed rows)
-    const long cells = (long)mass_pages * p.Hkv * nblocks;
-    long per = cells / (4L * p.sms);
+    // pages of a CTA: at least a page a warp; three waves of CTAs, which even out sequences of different lengths, where the pairs are
+    // quickly laid out, one where that costs more (32 rows x 5 heads, four prompts of 16384 tokens: 398 against 386 us)
+    const long cells = (long)mass_pages * p.Hkv * nblocks, ctas = (p.block * p.G <= 32 ? 12L : 4L) * p.sms;
+    long per = cells / ctas;
     per = per < 1 ? 1 : per;
     per = (per + kWarps - 1) / kWarps * kWarps;
     static unsigned long long ready = 0;

@@ -688,3 +688,79 @@ def test_append_of_many_rows_over_an_odd_number_of_heads(device, D):
     ok, ov = (torch.zeros(1, n, Hkv * D, dtype=torch.bfloat16, device=device) for _ in range(2))
     kv4.kv4_gather(c.kv, c.table, c.slots.to(device), None, ok, ov)
     assert torch.equal(ok[0].cpu(), c.k[0].reshape(n, -1).bfloat16()) and torch.equal(ov[0].cpu(), c.v[0].reshape(n, -1).bfloat16())
+
+
+# ---------------------------------------------------------------------------------------------
+# blocks of many rows: the unpacked keys are shared by all their pairs
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("D,G,block,window", [(64, 16, 9, 0), (64, 1, 40, 33), (128, 5, 32, 0), (128, 16, 5, 70), (256, 12, 1, 0), (256, 3, 20, 0), (256, 16, 3, 25)])
+def test_blocks_of_many_rows(device, D, G, block, window):
+    lens, Hkv = [200, 65, 700], 2
+    c = Cache(lens, Hkv, D, device, seed=D + G)
+    seqs = [s for s in range(3) for _ in range(block)]
+    pos = [lens[s] - block + r for s in range(3) for r in range(block)]
+    pos[0] = -1
+    q = torch.randn(len(seqs), Hkv * G * D, generator=torch.Generator().manual_seed(G)).bfloat16()
+    gate = torch.randn(len(seqs), Hkv * G * D, generator=torch.Generator().manual_seed(G + 1)).bfloat16()
+    scale = -1 / math.sqrt(D) if window else 1 / math.sqrt(D)
+    out = c.attend(seqs, pos, q, G, scale, window, gate=gate, block=block)
+    ref, size, _, _ = c.expect(seqs, pos, q, G, scale, window)
+    top = c.expect(seqs, pos, q, G, abs(scale), window)[3]
+    scores_in_range(D, top)
+    sg = torch.sigmoid(gate.double())
+    close(out, ref * sg, size * sg)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_block_keeps_nan_from_rows_and_channels_that_do_not_see_it(device, D):
+    n, G, block = 60, 6, 8
+    c = Cache([n], 1, D, device, seed=6)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=device)
+    k, v = c.kx[0][55:57].clone(), c.vx[0][55:57].clone()
+    v[0, 5], k[1, 3] = math.inf, math.nan                                             # token 55: a value, token 56: a key
+    kv4.kv4_append(c.kv, k.to(device), v.to(device), i32([55, 56]), i32([int(c.slots[0])] * 2), c.table)
+    c.v[0][55] = quantised(c.vx[0][55:56].reshape(1, 1, D))[0]
+    q = torch.randn(block, G * D, generator=torch.Generator().manual_seed(2)).bfloat16()
+    pos = list(range(50, 58))
+    out = c.attend([0] * block, pos, q, G, 0.1, block=block).reshape(block, G, D)
+    ref, size, _, top = c.expect([0] * block, pos, q, G, 0.1)
+    scores_in_range(D, top)
+    ref, size = ref.reshape(block, G, D), size.reshape(block, G, D)
+    bad = (torch.arange(D) // 4) % (D // 32) == (5 // 4) % (D // 32)
+    close(out[:5].flatten(1), ref[:5].flatten(1), size[:5].flatten(1))                # rows 50 .. 54 see neither
+    assert bool(torch.isnan(out[5][:, bad]).all())                                    # row 55: 32 channels
+    close(out[5][:, ~bad], ref[5][:, ~bad], size[5][:, ~bad])
+    assert bool(torch.isnan(out[6:]).all())                                           # rows that see the key
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("amp", [2.0 ** -60, 1e-4, 300.0, 2.0 ** 50])
+def test_block_over_small_and_large_values(device, amp):
+    D, G, n, block = 128, 3, 150, 12
+    c = Cache([n], 1, D, device, seed=8, amp=amp)
+    q = (torch.randn(block, G * D, generator=torch.Generator().manual_seed(3)) / amp).bfloat16()
+    pos = list(range(n - block, n))
+    ref, size, w, top = c.expect([0] * block, pos, q, G, 0.1)
+    scores_in_range(D, top)
+    close(c.attend([0] * block, pos, q, G, 0.1, block=block, observe="set"), ref, size)
+    want = sum(torch.nn.functional.pad(x, (0, n - x.shape[1])) for x in w)
+    eps = 2 * (D + 16) * 2 ** -24 * top + 2 ** -19
+    assert bool(((c.mass_of(0).double() - want).abs() <= eps * want + 1e-35).all())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_block_with_tokens_of_far_larger_values(device):
+    D, n, G, block = 64, 400, 4, 9
+    c = Cache([n], 1, D, device, seed=12)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=device)
+    big = (c.vx[0][210:211].float() * 2.0 ** 30).bfloat16()
+    kv4.kv4_append(c.kv, c.kx[0][210:211].to(device), big.to(device), i32([210]), i32([int(c.slots[0])]), c.table)
+    c.v[0][210] = quantised(big.reshape(1, 1, D))[0]
+    q = torch.randn(block, G * D, generator=torch.Generator().manual_seed(5)).bfloat16()
+    for last in (209, 212, 399):
+        pos = list(range(last - block + 1, last + 1))
+        ref, size, _, top = c.expect([0] * block, pos, q, G, 0.1)
+        scores_in_range(D, top)
+        close(c.attend([0] * block, pos, q, G, 0.1, block=block), ref, size)
