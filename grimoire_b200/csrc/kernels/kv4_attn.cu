@@ -1007,9 +1007,10 @@ int launch(const AttnParams& p, int nblocks, int mass_pages, cudaStream_t st) {
     if (e != cudaSuccess) return (int)e;
   }
   if (p.mass) {
-    // pages of a CTA: at least a page a warp; three waves of CTAs, which even out sequences of different lengths, where the pairs are
-    // quickly laid out, one where that costs more (32 rows x 5 heads, four prompts of 16384 tokens: 398 against 386 us)
-    const long cells = (long)mass_pages * p.Hkv * nblocks, ctas = (p.block * p.G <= 32 ? 12L : 4L) * p.sms;
+    // pages of a CTA: at least a page a warp, and about a wave of CTAs, four an SM; a quarter more where the pairs are quickly laid out,
+    // since CTAs behind the end of a shorter sequence leave at once (one observed row, four sequences of 8192 to 16384 tokens: 92 us
+    // of a call that sets and one that adds, against 104 with three waves and 108 with three quarters of one)
+    const long cells = (long)mass_pages * p.Hkv * nblocks, ctas = (p.block * p.G <= 32 ? 5L : 4L) * p.sms;
     long per = cells / ctas;
     per = per < 1 ? 1 : per;
     per = (per + kWarps - 1) / kWarps * kWarps;
