@@ -244,9 +244,9 @@ class Grimoire:
         # draft head: on a single-stage, single-rank dense model or dense-FFN hybrid (the reference drafts on the last stage)
         want_mtp = mtp_src is not None and ec.tp_world == 1 and ec.pp_world == 1
         lim = EngineLimits(max_slots=ec.seq_slots, max_ctx=ec.ctx, prefill_chunk=ec.prefill_chunk, max_decode_rows=64,
-                           kv_pages=ec.kv_pages, extra_kv_layers=1 if want_mtp else 0)
+                           kv_pages=ec.kv_pages, extra_kv_layers=1 if want_mtp else 0, kv_bits=ec.kv_bits, kv_keep=ec.kv_keep, kv_recent=ec.kv_recent)
         eng = Engine(model, lim)
-        if ec.prefix_cache and not cfg.is_qwen4_exp:       # that family's n-gram history and convolution tails are not snapshotted
+        if ec.prefix_cache and not cfg.is_qwen4_exp and not ec.kv_keep:       # that family's n-gram history and convolution tails are not snapshotted
             eng.enable_prefix_cache()
         g = cls(model, eng, tok, ec)
         if want_mtp:
@@ -273,7 +273,8 @@ class Grimoire:
             f"ep={getattr(m, 'ep_world', 1)} dp={ec.dp_world}",
             f"  weights    : {'block-scaled fp8 (e4m3, 1x128)' if getattr(m, 'kv_layer_count', None) is not None else ec.proj + ' g' + str(m.cfg.quant_group)} "
             f"({m.weight_bytes() / 1e9:.2f} GB on this rank), draft head={type(self.drafter).__name__ if self.drafter is not None else 'none'}",
-            f"  kv cache   : int8 paged, {self.engine.kv.num_pages} pages x 16 tokens, {self.engine.kv.bytes_per_token()} B/token",
+            f"  kv cache   : {'int8' if self.engine.kv.bits == 8 else '4-bit'} paged, {self.engine.kv.num_pages} pages x 16 tokens, {self.engine.kv.bytes_per_token()} B/token"
+            + (f", cut to {ec.kv_keep} tokens a conversation" if ec.kv_keep else ""),
             f"  batching   : width {ec.width()}, prefill chunk {ec.prefill_chunk}, interleave chunk {ec.interleave_chunk}",
             f"  speculation: copy drafts={'on' if ec.copy_drafts else 'off'} depth table {ec.spec_depth_table()}",
             f"  prefix     : {'on' if self.engine.prefix_cache is not None else 'off'}",

@@ -25,6 +25,9 @@ _ENV = {
     "GRIMOIRE_MTP_DRAFT_VOCAB": ("mtp_draft_vocab", int),
     "GRIMOIRE_KV_POOL": ("kv_pool", int),
     "GRIMOIRE_KV_PAGES": ("kv_pages", int),
+    "GRIMOIRE_KV_BITS": ("kv_bits", int),
+    "GRIMOIRE_KV_KEEP": ("kv_keep", int),
+    "GRIMOIRE_KV_RECENT": ("kv_recent", int),
     "GRIMOIRE_PREFIX_CACHE": ("prefix_cache", int),
     "GRIMOIRE_PREFILL_CHUNK": ("prefill_chunk", int),
     "GRIMOIRE_INTERLEAVE_CHUNK": ("interleave_chunk", int),
@@ -73,6 +76,9 @@ class EngineConfig:
     admit_hold_long_ms: float = 100.0
     kv_pool: int = 1
     kv_pages: int = 0
+    kv_bits: int = 8                   # --kv-bits {8,4}
+    kv_keep: int = 0                   # --kv-keep: cached tokens a conversation is cut to (0: never)
+    kv_recent: int = 0                 # the last tokens that always stay (0: half of kv_keep)
     prefix_cache: int = 1
     # speculation
     mtp: int = 1
@@ -114,6 +120,10 @@ class EngineConfig:
                 raise ValueError(f"{name} must be >= 1")
         if not (0 <= self.tp_rank < self.tp_world) or not (0 <= self.pp_rank < self.pp_world) or not (0 <= self.ep_rank < self.ep_world):
             raise ValueError("rank outside its world size")
+        if self.kv_bits not in (4, 8):
+            raise ValueError("--kv-bits must be 8 or 4")
+        if self.kv_keep < 0 or self.kv_recent < 0 or (self.kv_keep and self.kv_bits != 4):
+            raise ValueError("--kv-keep needs --kv-bits 4 and a number of tokens >= 0")
         if self.mtp_k < 0 or self.mtp_k > 16:
             raise ValueError("GRIMOIRE_MTP_K must be in 0..16")
         return self
@@ -132,6 +142,8 @@ def add_engine_flags(ap: argparse.ArgumentParser) -> None:
     ap.add_argument("--model", "-m", default="", help="HF directory, .gguf file or pre-quantized artifact")
     ap.add_argument("--proj", default="int4", help="projection format: int4 int8 mxfp4 mxfp8 fp8 (block-scaled) fp8_e4m3 fp8_e5m2 bf16 native")
     ap.add_argument("--ctx", type=int, default=8192, help="context cap per request")
+    ap.add_argument("--kv-bits", type=int, default=8, help="bits of a cached K / V element: 8 or 4")
+    ap.add_argument("--kv-keep", type=int, default=0, help="cut a conversation's cache to this many tokens, by accumulated attention weight (needs --kv-bits 4)")
     ap.add_argument("--dflash-model", default="", help="optional block drafter checkpoint")
     ap.add_argument("--defer-moe-gather", action="store_true")
     ap.add_argument("--bf16-qkv", action="store_true")

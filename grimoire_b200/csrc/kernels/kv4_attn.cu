@@ -938,7 +938,7 @@ int sm_count() {
   return known[dev];
 }
 
-int plan(Plan& pl, long M, long Hq, long Hkv, long D, long block, long max_len) {
+int plan(Plan& pl, long M, long Hq, long Hkv, long D, long block, long max_len, long alone) {
   if (!fits(M, 1, 65535) || !fits(Hkv, 1, 65535) || !fits(Hq, 1, 16 * Hkv) || Hq % Hkv || !fits(block, 1, M) || M % block || !fits(max_len, 1, 0x7fffffff)) return -2;
   if (D != 64 && D != 128 && D != 256) return -2;
   const int G = (int)(Hq / Hkv), sms = sm_count();
@@ -958,18 +958,19 @@ int plan(Plan& pl, long M, long Hq, long Hkv, long D, long block, long max_len) 
   pl.uheads = (int)Hkv * pl.subs;
   pl.sms = sms;
   pl.ctas = sms * (D == 256 ? Ring<256>::kCtas : Ring<128>::kCtas);
-  const long cells = units * pl.uheads, pages = (max_len + kPage - 1) / kPage;
+  // alone: the keys of a block are cut as in a call of that block only, so that its rows get the same bits in both
+  const long cells = (alone ? pl.groups : units) * pl.uheads, pages = (max_len + kPage - 1) / kPage;
   // Streamed: every CTA gets the same number of pages of the flat list, whatever the rows' lengths, at the price of a scan over
   // the rows and of parts that begin anywhere.  Split: a fixed number of CTAs a unit, at least eight pages (a step of the four
   // warps) each.  Measured, us split / streamed: 8 rows of up to 4999 tokens x 8 heads (45 pages a CTA) 20.7 / 24.5, 16 rows of
   // up to 8191 at head_dim 256 (110 pages) 51.0 / 54.1, one row of 131072 (147 pages) 47.9 / 52.7, 32 rows of up to 32768 (900
   // pages) 320 / 231.
   pl.splits = 0;
-  if (units > kMaxUnits || cells * pages < 256L * pl.ctas) {
+  if (alone || units > kMaxUnits || cells * pages < 256L * pl.ctas) {
     long s = pages / 8 < pl.ctas / cells ? pages / 8 : pl.ctas / cells;
     pl.splits = (int)(s < 1 ? 1 : s);
   }
-  pl.slots = pl.splits == 0 ? pl.ctas + cells : cells * pl.splits;
+  pl.slots = pl.splits == 0 ? pl.ctas + cells : units * pl.uheads * pl.splits;
   return 0;
 }
 
@@ -1026,15 +1027,16 @@ int launch(const AttnParams& p, int nblocks, int mass_pages, cudaStream_t st) {
 }  // namespace
 
 // Scratch of a call in fp32 words, or -2 for arguments that are not served.
-GRM_API long grm_kv4_attn_scratch(int M, int Hq, int Hkv, int D, int block, int max_len, int observe) {
+GRM_API long grm_kv4_attn_scratch(int M, int Hq, int Hkv, int D, int block, int max_len, int observe, int alone) {
   Plan pl;
-  const int rc = plan(pl, M, Hq, Hkv, D, block, max_len);
+  const int rc = plan(pl, M, Hq, Hkv, D, block, max_len, alone);
   return rc ? rc : pl.floats(M, Hq, D, observe);
 }
 
 // One record of 64-bit words (kv4::Args):
 //   data, mass (or 0), table, slots, width, stride, pages, q, ld_q, row_seq, row_pos, gate (or 0), ld_gate, out, ld_o, scratch
-//   (8-byte aligned, or 0 where none is needed), M, Hq, Hkv, D, window, scale, block, observe (0 nothing, 1 set, 2 add), max_len
+//   (8-byte aligned, or 0 where none is needed), M, Hq, Hkv, D, window, scale, block, observe (0 nothing, 1 set, 2 add), max_len,
+//   alone
 // max_len bounds the positions of the call's rows for the observed weight and sets how the keys are cut.
 GRM_API int grm_kv4_attn(const void* words, void* stream) {
   Args a(words);
@@ -1048,9 +1050,9 @@ GRM_API int grm_kv4_attn(const void* words, void* stream) {
   float* s = a.ptr<float>();
   const long M = a.num(), Hq = a.num(), Hkv = a.num(), D = a.num(), window = a.num();
   p.scale_log2 = (float)(a.real() * 1.4426950408889634);
-  const long block = a.num(), observe = a.num(), max_len = a.num();
+  const long block = a.num(), observe = a.num(), max_len = a.num(), alone = a.num();
   Plan pl;
-  const int rc = plan(pl, M, Hq, Hkv, D, block, max_len);
+  const int rc = plan(pl, M, Hq, Hkv, D, block, max_len, alone);
   if (rc) return rc;
   if (!fits(observe, 0, 2) || (observe && !p.mass) || (!s && pl.floats(M, Hq, D, observe))) return -2;
   if (!observe) p.mass = nullptr;

@@ -17,6 +17,7 @@ import torch
 from ..models.dense import Buffers, DenseModel, RowBatch
 from ..ops import core as K
 from ..ops.core import PAGE
+from ..ops.kv4 import length_bucket
 from .kv import KvPool, OutOfPages, SeqSlot
 
 
@@ -28,6 +29,14 @@ class EngineLimits:
     max_decode_rows: int = 64        # rows of one batched decode / verify step
     kv_pages: int = 0                # 0 = max_slots * max_ctx / 16
     extra_kv_layers: int = 0         # KV layers beyond the model's own (1 for an MTP draft head)
+    kv_bits: int = 8                 # bits of a cached K / V element: 8 (a scale per token and head) or 4 (a maximum per 32)
+    # eviction over 4-bit pages: a conversation that has grown to kv_keep + kv_slack cached tokens is cut to kv_keep -- the first
+    # kv_sink, the last kv_recent and those that drew the most attention weight; 0 keeps everything
+    kv_keep: int = 0
+    kv_recent: int = 0               # 0 = half of kv_keep
+    kv_sink: int = 4
+    kv_slack: int = 256
+    kv_observe: int = 32             # last rows of a prompt whose attention weight is kept
 
 
 class Engine:
@@ -41,7 +50,16 @@ class Engine:
         n_attn = getattr(model, "kv_layer_count", len(model.layers)) + lim.extra_kv_layers   # attention layers of this stage
         self.mtp = None                  # models.mtp.MtpDrafter attaches itself here
         pages = lim.kv_pages or (lim.max_slots * ((lim.max_ctx + PAGE - 1) // PAGE))
-        self.kv = KvPool(n_attn, model.geom.Hkv, model.geom.D, pages, lim.max_slots, lim.max_ctx, self.device)
+        if lim.kv_keep:
+            # rows are rotated by positions that are not the cached ones: the one-device dense decoder (full attention) does that
+            if type(model) is not DenseModel or model.geom.window or any(getattr(model, n, None) is not None for n in ("tp", "pp", "cp", "up")):
+                raise ValueError("eviction from the KV cache is served by the dense decoder family with full attention on one device")
+            if lim.kv_bits != 4 or lim.extra_kv_layers:
+                raise ValueError("eviction from the KV cache needs 4-bit pages (kv_bits=4) and no draft head")
+            if lim.kv_keep < 1 or lim.kv_slack < 1 or lim.kv_observe < 1 or lim.kv_sink < 0 or self._kv_recent() + lim.kv_sink > lim.kv_keep or \
+                    self._kv_recent() < 1:
+                raise ValueError("eviction: kv_keep tokens hold kv_sink first and kv_recent last ones, and at least one of the latter")
+        self.kv = KvPool(n_attn, model.geom.Hkv, model.geom.D, pages, lim.max_slots, lim.max_ctx, self.device, lim.kv_bits, lim.kv_keep > 0)
         chunk = min(lim.prefill_chunk, lim.max_ctx)
         self.prefill_buf: Optional[Buffers] = None
         self._prefill_rows = chunk
@@ -51,12 +69,14 @@ class Engine:
         i32 = lambda n: torch.zeros(n, dtype=torch.int32, device=self.device)
         self.d_tokens, self.d_row_seq, self.d_row_pos = i32(lim.max_decode_rows), i32(lim.max_decode_rows), i32(lim.max_decode_rows)
         pin = self.device.type == "cuda"
-        self.h_stage = torch.zeros(3, lim.max_decode_rows, dtype=torch.int32, pin_memory=pin)
+        self.h_stage = torch.zeros(4, lim.max_decode_rows, dtype=torch.int32, pin_memory=pin)
+        self.d_row_rope = i32(lim.max_decode_rows)        # what a row is rotated by (eviction: its cached position + the tokens dropped)
         # verify blocks of a step as groups of rows for the one-pass verify attention: slot, first row, rows, first position
         self.h_groups = torch.zeros(4, lim.max_decode_rows, dtype=torch.int32, pin_memory=pin)
         self.d_groups = torch.zeros(4, lim.max_decode_rows, dtype=torch.int32, device=self.device)
         self.h_next = torch.zeros(lim.max_decode_rows, dtype=torch.int32, pin_memory=pin)
         self.prefix_cache = None
+        self._warming = False             # a run before a capture: its rows are counted once, by the replay
         self._verify: dict = {}           # slot -> (handle, first row, rows, first position) of its last verify block
         self._reused_head_logits = None
         self.graphs: dict[tuple, "torch.cuda.CUDAGraph"] = {}      # (rows, splits, distinct sequences)
@@ -84,12 +104,29 @@ class Engine:
                     self.kv.release(seq)
                     return
                 extra = {"recurrent": snap(seq.slot)}
-            self.prefix_cache.store(seq, head_logits, extra)
+            if not seq.dropped:          # (what is left of a cut conversation is nobody's prefix)
+                self.prefix_cache.store(seq, head_logits, extra)
         self.kv.release(seq)
+
+    def _kv_recent(self) -> int:
+        return self.limits.kv_recent or self.limits.kv_keep // 2
+
+    def trim(self, seq: SeqSlot) -> bool:
+        """Cut a conversation that has outgrown ``kv_keep + kv_slack`` cached tokens (between two steps; see EngineLimits)."""
+        lim = self.limits
+        if not lim.kv_keep or seq.length < lim.kv_keep + lim.kv_slack:
+            return False
+        done = self.kv.evict(seq, lim.kv_keep, self._kv_recent(), lim.kv_sink)
+        if done:
+            del seq.tokens[: len(seq.tokens) - seq.length]      # drafters look for the newest tokens
+            self.counters["kv_evictions"] = self.counters.get("kv_evictions", 0) + 1
+        return done
 
     def enable_prefix_cache(self, max_entries: int = 16):
         from .prefix_cache import PrefixCache
 
+        if self.limits.kv_keep:
+            raise ValueError("cached prefixes and eviction exclude each other: conversations would share the weight of their tokens")
         self.prefix_cache = PrefixCache(self.kv, max_entries)
         return self.prefix_cache
 
@@ -149,6 +186,11 @@ class Engine:
             rb = RowBatch(tok_dev[done: done + m], torch.full((m,), seq.slot, dtype=torch.int32, device=self.device), rows,
                           mode="prefill", q_pos0=pos0, seq_slot=seq.slot,
                           logits_rows=torch.tensor([m - 1], device=self.device))
+            if self.limits.kv_keep:
+                if seq.dropped:
+                    rb.row_rope = rows + seq.dropped
+                if done + m == n:
+                    rb.observe_rows, rb.observe = min(m, self.limits.kv_observe), "add" if seq.tokens else "set"
             out = self.model.forward(rb, self.prefill_buf, self.kv.layers, self.kv.table)
             if self.mtp is not None:
                 self.mtp.warm_chunk(seq, tok_dev, done, m, pos0, self.prefill_buf, last=(done + m == n))
@@ -169,7 +211,7 @@ class Engine:
 
     def can_prefill_batch(self) -> bool:
         """Several fresh prompts in one M-row pass: dense models without a draft head or pipeline stages."""
-        return isinstance(self.model, DenseModel) and self.mtp is None and getattr(self.model, "pp", None) is None
+        return isinstance(self.model, DenseModel) and self.mtp is None and getattr(self.model, "pp", None) is None and not self.limits.kv_keep
 
     def prefill_batch(self, seqs: Sequence[SeqSlot], prompts: Sequence[Sequence[int]]) -> list[torch.Tensor]:
         """Read several whole prompts into fresh slots with ONE forward pass (admit_batch, grimoire.cpp:12071-12146): the
@@ -214,7 +256,7 @@ class Engine:
             _lin.set_batch_invariant(True)
             self.graphs.clear()
 
-    def _stage_rows(self, tokens, slots, positions) -> int:
+    def _stage_rows(self, tokens, slots, positions, seqs=()) -> int:
         M = len(tokens)
         st = self.h_stage
         st[0, :M] = torch.as_tensor(tokens, dtype=torch.int32)
@@ -223,15 +265,24 @@ class Engine:
         self.d_tokens[:M].copy_(st[0, :M], non_blocking=True)
         self.d_row_seq[:M].copy_(st[1, :M], non_blocking=True)
         self.d_row_pos[:M].copy_(st[2, :M], non_blocking=True)
+        if self.limits.kv_keep:
+            st[3, :M] = torch.as_tensor([p + s.dropped for p, s in zip(positions, seqs)], dtype=torch.int32)
+            self.d_row_rope[:M].copy_(st[3, :M], non_blocking=True)
         return M
 
     def _splits_for(self, M: int, max_len: int) -> int:
+        """How the attention of a step cuts the keys, which is also what its graph is keyed by: the split factor over int8 pages,
+        a power of two that bounds the lengths over 4-bit ones."""
+        if self.kv.bits == 4:
+            return length_bucket(max_len)
         return K.decode_splits(max_len, M, self.model.geom.Hkv)
 
     def _run_rows(self, M: int, splits: int, distinct: bool = False, runs=None, full_logits: bool = True, ngroups: int = 0) -> torch.Tensor:
         hs = getattr(self.model, "head_split", None)
         rb = RowBatch(self.d_tokens[:M], self.d_row_seq[:M], self.d_row_pos[:M], mode="decode", splits=splits, distinct=distinct, runs=runs,
                       full_logits=full_logits or hs is None, verify=(self.d_groups, ngroups) if ngroups else None)
+        if self.limits.kv_keep:
+            rb.row_rope, rb.observe = self.d_row_rope[:M], None if self._warming else "add"
         logits = self.model.forward(rb, self.decode_buf, self.kv.layers, self.kv.table)
         pp = getattr(self.model, "pp", None)
         if logits is not None and hs is not None and not rb.full_logits:
@@ -279,7 +330,7 @@ class Engine:
         for s, p in zip(seqs, positions):
             self.kv.ensure(s, p + 1)
             max_len = max(max_len, p + 1)
-        if (runs is None and M > 1 and len({s.slot for s in seqs}) == 1 and max_len < K.VERIFY_ATTN_MIN_CTX
+        if (runs is None and M > 1 and len({s.slot for s in seqs}) == 1 and (max_len < K.VERIFY_ATTN_MIN_CTX or self.kv.bits == 4)
                 and len({self._splits_for(1, p + 1) for p in positions}) > 1):
             # one conversation's verify block whose rows sit on both sides of a length at which the single-row split factor changes (once
             # per doubling of the context): score the rows one launch each, which is what plain decoding would do
@@ -292,11 +343,13 @@ class Engine:
                 else:
                     outs.append(r[0])
             return (outs, torch.stack(lgs)) if return_logits else outs
-        self._stage_rows(tokens, [s.slot for s in seqs], positions)
+        self._stage_rows(tokens, [s.slot for s in seqs], positions, seqs)
         splits = self._splits_for(M, max_len)
         distinct = len({s.slot for s in seqs}) == M      # no verify block: the attention kernel may append K / V itself
         shape = ()
-        if not distinct and max_len < K.VERIFY_ATTN_MIN_CTX:
+        if not distinct and self.kv.bits == 4:
+            splits = -self._splits_for(1, max_len)       # verify blocks over 4-bit pages: every row as in a step of its own
+        elif not distinct and max_len < K.VERIFY_ATTN_MIN_CTX:
             # Short contexts: every row of a verify block is scored exactly as a single-row step at its position would be
             # (the per-row kernel with the single-row split factor, whose page partition depends on the row's own length
             # only), so that speculative output reproduces plain greedy output bit for bit; the one-pass kernel is no
@@ -385,7 +438,9 @@ class Engine:
         # must not keep the warm-up run's update
         saved = self._save_recurrent(M)
         full = getattr(self.model, "head_split", None) is None     # a split head is captured with its (value, index) pick
+        self._warming = True
         self._run_rows(M, splits, distinct, full_logits=full, ngroups=ngroups)
+        self._warming = False
         torch.cuda.current_stream().synchronize()
         self._restore_recurrent(saved)
         g = torch.cuda.CUDAGraph()
@@ -408,7 +463,7 @@ class Engine:
         for s in seqs:
             self.kv.ensure(s, s.length + steps_ahead + 1)
             max_len = max(max_len, s.length + steps_ahead + 1)
-        self._stage_rows(first_tokens, [s.slot for s in seqs], [s.length for s in seqs])
+        self._stage_rows(first_tokens, [s.slot for s in seqs], [s.length for s in seqs], seqs)
         splits = self._splits_for(M, max_len)
         distinct = len({s.slot for s in seqs}) == M
 
@@ -416,17 +471,20 @@ class Engine:
             self._run_rows(M, splits, distinct, full_logits=getattr(self.model, "head_split", None) is None)
             self.d_tokens[:M].copy_(self.decode_buf.next_ids[:M])
             self.d_row_pos[:M].add_(1)
+            self.d_row_rope[:M].add_(1)
 
-        saved = (self.d_tokens[:M].clone(), self.d_row_pos[:M].clone())
+        saved = (self.d_tokens[:M].clone(), self.d_row_pos[:M].clone(), self.d_row_rope[:M].clone())
         rec = self._save_recurrent(M)
+        self._warming = True
         body()                       # warm-up outside capture (also sizes the workspace)
+        self._warming = False
         torch.cuda.current_stream().synchronize()
-        self.d_tokens[:M].copy_(saved[0]); self.d_row_pos[:M].copy_(saved[1])
+        self.d_tokens[:M].copy_(saved[0]); self.d_row_pos[:M].copy_(saved[1]); self.d_row_rope[:M].copy_(saved[2])
         self._restore_recurrent(rec)
         g = torch.cuda.CUDAGraph()
         with torch.cuda.graph(g):
             body()
-        self.d_tokens[:M].copy_(saved[0]); self.d_row_pos[:M].copy_(saved[1])
+        self.d_tokens[:M].copy_(saved[0]); self.d_row_pos[:M].copy_(saved[1]); self.d_row_rope[:M].copy_(saved[2])
         torch.cuda.current_stream().synchronize()
         return g
 
@@ -460,6 +518,7 @@ class Engine:
                 if collect_logits:
                     logit_trace.append(res[1][0].float().cpu().clone())
                 self.commit_rows([seq], [tok], [pos])
+                self.trim(seq)
                 tok = int(nxt[0])
         finally:
             self.release(seq)

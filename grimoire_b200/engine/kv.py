@@ -1,4 +1,4 @@
-"""Pooled paged KV cache: 16-token int8 pages shared by every conversation slot.
+"""Pooled paged KV cache: 16-token int8 (or 4-bit) pages shared by every conversation slot.
 
 Plays the role of the reference's per-slot KV views + on-demand virtual-memory pool
 (bind_seq_slot grimoire.cpp:11872; KvVirtualPool src/kv_vmm.hpp; ensure_kv/admit_kv/release_kv
@@ -14,6 +14,7 @@ from typing import Optional
 import torch
 
 from ..ops.core import PAGE, KvLayer
+from ..ops.kv4 import Kv4Layer, kv4_compact, kv4_select
 
 
 class OutOfPages(RuntimeError):
@@ -26,17 +27,23 @@ class SeqSlot:
     length: int = 0                 # tokens whose K/V are in the cache
     pages: list[int] = field(default_factory=list)
     tokens: list[int] = field(default_factory=list)   # token ids behind the cached positions
+    dropped: int = 0                # tokens evicted so far: a row at cached position p is rotated as position p + dropped
 
 
 class KvPool:
     """Page allocator + per-slot block tables for ``n_layers`` attention layers."""
 
-    def __init__(self, n_layers: int, Hkv: int, D: int, num_pages: int, max_slots: int, max_ctx: int, device):
+    def __init__(self, n_layers: int, Hkv: int, D: int, num_pages: int, max_slots: int, max_ctx: int, device,
+                 bits: int = 8, mass: bool = False):
+        if bits not in (4, 8) or (mass and bits != 4):
+            raise ValueError("KV pages hold 8 or 4 bits an element; the weight of cached tokens is kept with 4-bit pages")
+        self.bits = bits
         self.device = torch.device(device)
         self.num_pages = num_pages
         self.max_slots = max_slots
         self.max_pages_per_seq = (max_ctx + PAGE - 1) // PAGE
-        self.layers = [KvLayer.alloc(num_pages, Hkv, D, device) for _ in range(n_layers)]
+        alloc = (lambda: KvLayer.alloc(num_pages, Hkv, D, device)) if bits == 8 else (lambda: Kv4Layer.alloc(num_pages, Hkv, D, device, mass))
+        self.layers = [alloc() for _ in range(n_layers)]
         self.refcount = [0] * num_pages
         self.free = list(range(num_pages - 1, -1, -1))
         # block table lives on the device (kernels index it) with a pinned host mirror
@@ -104,6 +111,7 @@ class KvPool:
         self._sync_row(seq.slot)
         seq.pages.clear()
         seq.length = 0
+        seq.dropped = 0
         seq.tokens.clear()
         self.slots.pop(seq.slot, None)
 
@@ -119,6 +127,39 @@ class KvPool:
         seq.length = min(seq.length, length)
         del seq.tokens[length:]
         self._sync_row(seq.slot)
+
+    def evict(self, seq: SeqSlot, keep: int, recent: int, sink: int = 0) -> bool:
+        """Cut the sequence to ``keep`` cached tokens: in every layer and kv head the first ``sink``, the last ``recent`` and the
+        others that drew the most attention weight.  They move to fresh pages, so pages shared with other sequences stay as they
+        are.  Returns False, with nothing changed, where the sequence is not longer or the pool has no pages for the copy."""
+        if self.bits != 4 or self.layers[0].mass is None:
+            raise ValueError("eviction needs 4-bit pages that keep the weight of cached tokens")
+        need = (keep + PAGE - 1) // PAGE
+        if seq.length <= keep:
+            return False
+        if need > len(self.free) and self.reclaim is not None:
+            self.reclaim(need)
+        if need > len(self.free):
+            return False
+        fresh = [self.free.pop() for _ in range(need)]
+        i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=self.device)
+        slot, length, dst = i32([seq.slot]), i32([seq.length]), i32([fresh])
+        for layer in self.layers:
+            kept = kv4_select(layer, slot, length, self.table, keep, recent, sink)
+            kv4_compact(layer, slot, kept, self.table, dst)
+        for pg in seq.pages:
+            self.refcount[pg] -= 1
+            if self.refcount[pg] == 0:
+                self.free.append(pg)
+        for pg in fresh:
+            self.refcount[pg] = 1
+        self.table_host[seq.slot].fill_(-1)
+        self.table_host[seq.slot, :need] = torch.tensor(fresh, dtype=torch.int32)
+        seq.pages = fresh
+        seq.dropped += seq.length - keep
+        seq.length = keep
+        self._sync_row(seq.slot)
+        return True
 
     def share_prefix(self, src: SeqSlot, dst: SeqSlot, n_tokens: int) -> int:
         """Point ``dst`` at the first whole pages of ``src`` (copy-on-write is not needed: only

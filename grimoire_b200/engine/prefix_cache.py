@@ -131,7 +131,7 @@ class PrefixCache:
             kv.refcount[new] = 1
             src = ent.pages[n_full]
             for L in kv.layers:
-                L.k[new].copy_(L.k[src]); L.v[new].copy_(L.v[src]); L.ks[new].copy_(L.ks[src]); L.vs[new].copy_(L.vs[src])
+                L.copy_page(src, new)
             kv.table_host[seq.slot, n_full] = new
             seq.pages.append(new)
             reused = n

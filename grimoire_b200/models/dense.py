@@ -22,6 +22,7 @@ from ..formats.codecs import Fmt
 from ..formats.quantize import QuantWeight, quantize, slice_cols, slice_rows
 from ..formats.w4_tile_layout import concat_rows, interleave_gate_up_q
 from ..ops import core as K
+from ..ops import kv4
 from ..ops import ref
 from ..ops.linear import BF16Linear, MXLinear, ROWQ_KIND, RowQLinear, W4Linear
 from ..ops.workspace import Workspace
@@ -71,6 +72,11 @@ class RowBatch:
     # decode step with verify blocks: (int32 device tensor [4][n] of groups -- slot, first row, rows, first position --, n);
     # the attention then reads the cache once per group of rows (attn_verify.cu) instead of once per row
     verify: Optional[tuple] = None
+    # eviction (4-bit pages that keep the weight of cached tokens): the positions that the rows are rotated by, where they are
+    # not the cached ones ``row_pos``; prefill: how many last rows of the chunk are observed, and whether they set or add
+    row_rope: Optional[torch.Tensor] = None
+    observe: Optional[str] = None
+    observe_rows: int = 0
 
 
 class Buffers:
@@ -594,7 +600,7 @@ class DenseModel:
             return self.forward_prefill_sp(rb, buf, kv_layers, block_table)
         cfg, geom = self.cfg, self.geom
         M = rb.tokens.shape[0]
-        if M == 1 and rb.mode == "decode" and not trace.timeline.on and self._mega_ready():
+        if M == 1 and rb.mode == "decode" and not trace.timeline.on and isinstance(kv_layers[0], K.KvLayer) and self._mega_ready():
             return self.forward_mega(rb, buf, kv_layers, block_table)
         eps, off = cfg.rms_norm_eps, cfg.norm_offset
         h, x = buf.h[:M], buf.x[:M]
@@ -607,6 +613,7 @@ class DenseModel:
             self.pp.recv_hidden(h)          # [rows][H] from the previous stage
         prefill = rb.mode == "prefill"
         T = rb.q_pos0 + M
+        rope_pos, row_cache = (rb.row_pos, None) if rb.row_rope is None else (rb.row_rope, rb.row_pos)
         tl = trace.timeline.on
         for li, L in enumerate(self.layers):
             kvl = kv_layers[li]
@@ -624,15 +631,20 @@ class DenseModel:
             elif prefill:
                 if rb.q_pos0 > 0:
                     K.gather_kv_dense(kvl, block_table[rb.seq_slot], rb.q_pos0, buf.dense_k, buf.dense_v)
-                K.rope_kvwrite(qkv, rb.row_pos, rb.row_seq, block_table, self.inv_freq, geom, q, kvl, L.q_norm, L.k_norm,
-                               gate, buf.dense_k[rb.q_pos0: T], buf.dense_v[rb.q_pos0: T])
+                K.rope_kvwrite(qkv, rope_pos, rb.row_seq, block_table, self.inv_freq, geom, q, kvl, L.q_norm, L.k_norm,
+                               gate, buf.dense_k[rb.q_pos0: T], buf.dense_v[rb.q_pos0: T], row_cache=row_cache)
                 K.flash_prefill(q, buf.dense_k, buf.dense_v, geom, attn, rb.q_pos0, gate)
+                if rb.observe_rows:
+                    # what the chunk's last rows look at: the weight that a later eviction goes by (their output is not needed)
+                    w = rb.observe_rows
+                    kv4.kv4_attn(q[M - w: M], rb.row_seq[M - w: M], rb.row_pos[M - w: M], block_table, kvl, geom,
+                                 torch.empty(w, q.shape[1], dtype=q.dtype, device=q.device), T, block=w, observe=rb.observe)
             elif not ((M == 1 or rb.distinct) and gate is None and K.paged_decode_attn_fused(qkv, self.inv_freq, L.q_norm, L.k_norm, rb.row_seq, rb.row_pos,
                                                                           block_table, kvl, geom, attn, rb.splits, self.ws, prefetch=True)):
-                K.rope_kvwrite(qkv, rb.row_pos, rb.row_seq, block_table, self.inv_freq, geom, q, kvl, L.q_norm, L.k_norm, gate)
+                K.rope_kvwrite(qkv, rope_pos, rb.row_seq, block_table, self.inv_freq, geom, q, kvl, L.q_norm, L.k_norm, gate, row_cache=row_cache)
                 if not (rb.verify is not None and K.paged_verify_attn(q, rb.verify[0], rb.verify[1], block_table, kvl, geom, attn,
                                                                       rb.splits, self.ws, gate)):
-                    K.paged_decode_attn(q, rb.row_seq, rb.row_pos, block_table, kvl, geom, attn, rb.splits, self.ws, gate)
+                    K.paged_decode_attn(q, rb.row_seq, rb.row_pos, block_table, kvl, geom, attn, rb.splits, self.ws, gate, rb.observe)
             if tl: trace.mark("o_proj")
             self._row_parallel(L.o, attn, h)
             if tl: trace.mark("norm+gate_up")

@@ -90,9 +90,18 @@ class KvLayer:
         return KvLayer(mk(pages, Hkv, PAGE, D, dt=torch.int8), mk(pages, Hkv, PAGE, D, dt=torch.int8),
                        mk(pages, Hkv, PAGE, dt=torch.float32), mk(pages, Hkv, PAGE, dt=torch.float32))
 
+    def copy_page(self, src: int, dst: int) -> None:
+        for t in (self.k, self.v, self.ks, self.vs):
+            t[dst].copy_(t[src])
+
     def bytes_per_token(self) -> int:
         Hkv, D = self.k.shape[1], self.k.shape[3]
         return 2 * Hkv * D + 2 * Hkv * 4
+
+
+def _four_bit(kv) -> bool:
+    """Whether a layer's pages are the 4-bit ones of ``ops.kv4``."""
+    return kv is not None and not isinstance(kv, KvLayer)
 
 
 @dataclass
@@ -111,13 +120,35 @@ class AttnGeom:
 def rope_kvwrite(qkv: torch.Tensor, row_pos: torch.Tensor, row_seq: Optional[torch.Tensor],
                  block_table: Optional[torch.Tensor], inv_freq: torch.Tensor, geom: AttnGeom, q_out: torch.Tensor,
                  kv: Optional[KvLayer], q_norm_w=None, k_norm_w=None, gate_out=None, k_out=None, v_out=None,
-                 dense_pos0: int = -1, q_rows: Optional[tuple] = None):
+                 dense_pos0: int = -1, q_rows: Optional[tuple] = None, row_cache: Optional[torch.Tensor] = None):
     """Split the fused q|k|v rows, q/k norm, RoPE, write q (bf16) and int8 K/V pages (+ dense bf16
     K/V for the prefill attention of the current chunk).  See rope_kv.cu.  ``dense_pos0`` >= 0: the dense K / V row of a
     token lands at index ``row_pos - dense_pos0`` (rows in any order); ``q_rows`` = (first, count): q / gate are produced
-    for those rows only (the other rows of ``q_out`` are left as they are)."""
+    for those rows only (the other rows of ``q_out`` are left as they are).
+
+    ``kv`` may be a layer of 4-bit pages (``ops.kv4.Kv4Layer``): K / V are then quantised from the bf16 rows, and ``row_cache``
+    (default: ``row_pos``) names the cached position of a row where it is not the one that its rotation takes (tokens before it
+    were evicted)."""
     M = qkv.shape[0]
     Hq, Hkv, D = geom.Hq, geom.Hkv, geom.D
+    if _four_bit(kv):
+        from . import kv4
+
+        if k_out is None:
+            k_rows = torch.empty(M, Hkv * D, dtype=torch.bfloat16, device=qkv.device)
+            v_rows = torch.empty_like(k_rows)
+            rope_kvwrite(qkv, row_pos, row_seq, block_table, inv_freq, geom, q_out, None, q_norm_w, k_norm_w, gate_out, k_rows, v_rows, q_rows=q_rows)
+        else:
+            rope_kvwrite(qkv, row_pos, row_seq, block_table, inv_freq, geom, q_out, None, q_norm_w, k_norm_w, gate_out, k_out, v_out, dense_pos0, q_rows)
+            k_rows, v_rows = k_out, v_out
+            if dense_pos0 >= 0:                     # the dense rows lie at their positions
+                at = row_pos.long() - dense_pos0
+                k_rows, v_rows = k_out.index_select(0, at), v_out.index_select(0, at)
+        if row_seq is not None:
+            kv4.kv4_append(kv, k_rows[:M], v_rows[:M], row_pos if row_cache is None else row_cache, row_seq, block_table)
+        return q_out
+    if row_cache is not None:
+        raise ValueError("rope_kvwrite: row_cache is served over 4-bit pages")
     if not qkv.is_cuda:
         qs = 2 * D if geom.q_gated else D
         x = qkv.float()
@@ -169,9 +200,14 @@ def rope_kvwrite(qkv: torch.Tensor, row_pos: torch.Tensor, row_seq: Optional[tor
 
 def gather_kv_dense(kv: KvLayer, pages_of_seq: torch.Tensor, T: int, out_k: torch.Tensor, out_v: torch.Tensor):
     """Dequantize the first T cached tokens of one sequence into dense bf16 [T][Hkv*D] buffers."""
-    Hkv, D = kv.k.shape[1], kv.k.shape[3]
     if T <= 0:
         return
+    if _four_bit(kv):
+        from . import kv4
+
+        kv4.kv4_gather(kv, pages_of_seq[None], None, None, out_k[None, :T], out_v[None, :T])
+        return
+    Hkv, D = kv.k.shape[1], kv.k.shape[3]
     if not kv.k.is_cuda:
         for name, pages, scales, out in (("k", kv.k, kv.ks, out_k), ("v", kv.v, kv.vs, out_v)):
             npg = (T + PAGE - 1) // PAGE
@@ -205,8 +241,18 @@ def decode_splits(max_len: int, M: int, Hkv: int) -> int:
 
 def paged_decode_attn(q: torch.Tensor, row_seq: torch.Tensor, row_pos: torch.Tensor, block_table: torch.Tensor,
                       kv: KvLayer, geom: AttnGeom, out: torch.Tensor, splits: int, ws: Optional[Workspace],
-                      gate: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """Attention of M (sequence, position) rows over the paged int8 cache; see attn_decode.cu."""
+                      gate: Optional[torch.Tensor] = None, observe: Optional[str] = None) -> torch.Tensor:
+    """Attention of M (sequence, position) rows over the paged int8 cache; see attn_decode.cu.
+
+    Over 4-bit pages (``ops.kv4``) ``splits`` is the bound on the rows' lengths that the step was planned with, negative where a
+    row's result must not depend on the step's other rows (verify blocks), and ``observe`` may keep the weight that every
+    cached token draws."""
+    if _four_bit(kv):
+        from . import kv4
+
+        return kv4.kv4_attn(q, row_seq, row_pos, block_table, kv, geom, out, abs(splits), gate, observe=observe, alone=splits < 0)
+    if observe is not None:
+        raise ValueError("paged_decode_attn: the weight of cached tokens is kept over 4-bit pages")
     M = q.shape[0]
     Hq, Hkv, D = geom.Hq, geom.Hkv, geom.D
     if not q.is_cuda:
@@ -262,7 +308,7 @@ def paged_decode_attn_fused(qkv: torch.Tensor, inv_freq: torch.Tensor, q_norm_w,
     when the case is not served (CPU tensors, gated q, switch off); the caller then runs the two kernels.  ``prefetch``:
     the launch right before this one is the projection that writes ``qkv`` and nothing else this kernel reads, so the
     kernel may fetch the pages of earlier tokens while that launch is still running."""
-    if not (qkv.is_cuda and FUSED_ROPE_ATTN) or geom.q_gated or geom.rot < 64:
+    if not (qkv.is_cuda and FUSED_ROPE_ATTN) or geom.q_gated or geom.rot < 64 or _four_bit(kv):
         return False
     apply_pdl_switch()
     M = qkv.shape[0]
@@ -319,7 +365,7 @@ def paged_verify_attn(q: torch.Tensor, blocks: torch.Tensor, nblocks: int, block
     src/attn_verify.hpp:48-69).  ``blocks`` is an int32 device tensor [4][>= nblocks]: sequence slot, first row, rows,
     first position of every group (``verify_groups``).  K / V of the rows must already be in the cache.  Returns False
     when the case is not served (CPU tensors, switch off); the caller then runs the per-row kernel."""
-    if not (q.is_cuda and VERIFY_ATTN) or verify_rows_per_group(geom) < 1:
+    if not (q.is_cuda and VERIFY_ATTN) or verify_rows_per_group(geom) < 1 or _four_bit(kv):
         return False
     Hq, Hkv, D = geom.Hq, geom.Hkv, geom.D
     part_o = part_ml = counters = None

@@ -59,6 +59,11 @@ class Kv4Layer:
     def D(self) -> int:
         return self.data.shape[2] // 18
 
+    def copy_page(self, src: int, dst: int) -> None:
+        self.data[dst].copy_(self.data[src])
+        if self.mass is not None:
+            self.mass[dst].copy_(self.mass[src])
+
     def bytes_per_token(self) -> int:
         Hkv, rec = self.data.shape[1], self.data.shape[2]
         return Hkv * rec // PAGE + (4 * Hkv if self.mass is not None else 0)
@@ -67,7 +72,7 @@ class Kv4Layer:
 # The calls are short (a decode step makes some per layer): arguments travel as one record of 64-bit words, and tensors are
 # checked with as few attribute reads as that takes.
 _pack = {n: struct.Struct(f"{n}q").pack for n in (14, 15, 17, 19)}
-_pack_attn = struct.Struct("21qd3q").pack
+_pack_attn = struct.Struct("21qd4q").pack
 _lib = None
 _INT, _BF16 = torch.int32, torch.bfloat16
 _OBSERVE = {None: 0, "set": 1, "add": 2}
@@ -80,7 +85,7 @@ def _cuda():
         lib = _native.cuda()
         for fn in (lib.grm_kv4_append, lib.grm_kv4_gather, lib.grm_kv4_select, lib.grm_kv4_compact, lib.grm_kv4_attn):
             fn.argtypes = [ctypes.c_char_p, ctypes.c_void_p]
-        lib.grm_kv4_attn_scratch.argtypes = [ctypes.c_int] * 7
+        lib.grm_kv4_attn_scratch.argtypes = [ctypes.c_int] * 8
         lib.grm_kv4_attn_scratch.restype = ctypes.c_long
         _lib = lib
     return _lib
@@ -203,8 +208,13 @@ def kv4_gather(kv: Kv4Layer, block_table: torch.Tensor, slots: Optional[torch.Te
 # ---------------------------------------------------------------------------------------------
 # attention
 # ---------------------------------------------------------------------------------------------
+def length_bucket(n: int) -> int:
+    """The longest length of a step, rounded up to a power of two: the host's bound that a captured step is keyed by."""
+    return max(PAGE, 1 << (max(1, n) - 1).bit_length())
+
+
 def kv4_attn(q: torch.Tensor, row_seq: torch.Tensor, row_pos: torch.Tensor, block_table: torch.Tensor, kv: Kv4Layer, geom: AttnGeom,
-             out: torch.Tensor, max_len: int, gate: Optional[torch.Tensor] = None, block: int = 1, observe: Optional[str] = None) -> torch.Tensor:
+             out: torch.Tensor, max_len: int, gate: Optional[torch.Tensor] = None, block: int = 1, observe: Optional[str] = None, alone: bool = False) -> torch.Tensor:
     """Attention of M rows over the 4-bit pages: row m (bf16 [Hq * D], after norm and RoPE) of sequence slot ``row_seq[m]`` sees
     the cached positions 0 .. ``row_pos[m]``, the last ``geom.window`` of them with a window, and leaves its output (bf16,
     times sigmoid(``gate[m]``) with a gate) in ``out[m]``.  A row that sees no key (a negative position, no mapped page)
@@ -212,6 +222,8 @@ def kv4_attn(q: torch.Tensor, row_seq: torch.Tensor, row_pos: torch.Tensor, bloc
     bounds the tokens that ``observe`` covers.
 
     ``block`` > 1: every ``block`` consecutive rows belong to one sequence (the last rows of a prompt, a verify block).
+    ``alone``: cut every block's keys as a call of that block alone would (of the same ``max_len``), so that a row's output does
+    not depend on the other rows of the call, to the bit.
     ``observe``: "set" or "add" the softmax weight that every token drew from the rows of its sequence in this call, summed
     over the rows and the query heads of a kv head, to ``kv.mass``; "set" covers all tokens up to the block's last position.
     """
@@ -258,12 +270,12 @@ def kv4_attn(q: torch.Tensor, row_seq: torch.Tensor, row_pos: torch.Tensor, bloc
         return out
     lib = _cuda()
     with _on(dev):
-        floats = lib.grm_kv4_attn_scratch(M, Hq, Hkv, D, block, max_len, mode)
+        floats = lib.grm_kv4_attn_scratch(M, Hq, Hkv, D, block, max_len, mode, alone)
         if floats < 0:
             _native.check(int(floats), what)
         scratch = torch.empty(floats, dtype=torch.float32, device=data.device) if floats else None
         words = _pack_attn(data.data_ptr(), _ptr(kv.mass), *table, P, qp, qs, seq, pos, gp, gs, op, os_, _ptr(scratch), M, Hq, Hkv, D, geom.window,
-                           geom.scale, block, mode, max_len)
+                           geom.scale, block, mode, max_len, alone)
         _native.check(lib.grm_kv4_attn(words, _native.raw_stream(dev)), what)
     return out
 

@@ -357,6 +357,8 @@ class Scheduler:
             eng.commit_rows([job.seq] * len(keep), keep, list(range(pos0, pos0 + len(keep))))
             if n > 1 and hasattr(eng, "rollback"):
                 eng.rollback(job.seq, pos0 + len(keep))
+            if hasattr(eng, "trim"):
+                eng.trim(job.seq)                                      # KV eviction, where the engine is set up for it
             if self.drafter is not None:
                 self.drafter.observe(eng, job.seq, keep, row0=o)       # model drafters track the newest hidden state
             alive = True
