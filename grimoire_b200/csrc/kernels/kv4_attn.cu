@@ -395,7 +395,8 @@ __global__ void __launch_bounds__(kThreads, Ring<D>::kCtas) attn_kernel(const At
 
   // ---- q: column operands of S^T for the pairs g and g + 8 ----
   uint32_t qb[HH][NG][2][2];
-  float fh[HH][2], m[HH][2], l[HH][2];                   // of the pairs 2 t, 2 t + 1 (+ 8 x)
+  constexpr float kLag = 1.f;
+  float fh[HH][2], m[HH][2], l[HH][2], bar[HH][2], off[HH][2];          // of the pairs 2 t, 2 t + 1 (+ 8 x)
   int lim[HH][2], low[HH][2];
 #pragma unroll
   for (int x = 0; x < HH; ++x) {
@@ -409,7 +410,8 @@ __global__ void __launch_bounds__(kThreads, Ring<D>::kCtas) attn_kernel(const At
       fh[x][j] = __shfl_sync(0xffffffffu, f, 8 * t + 4 * j);
       lim[x][j] = __shfl_sync(0xffffffffu, seen, 8 * t + 4 * j);
       low[x][j] = row_first(p, lim[x][j]);
-      m[x][j] = -INFINITY; l[x][j] = 0.f;
+      m[x][j] = bar[x][j] = -INFINITY; l[x][j] = 0.f;
+      off[x][j] = 14.f - kLag;
     }
   }
 
@@ -421,8 +423,6 @@ __global__ void __launch_bounds__(kThreads, Ring<D>::kCtas) attn_kernel(const At
 #pragma unroll
       for (int i = 0; i < 4; ++i) acc[x][gi][0][i] = acc[x][gi][1][i] = 0.f;
   int e_run = 14;                                        // biased exponent of the largest V maximum so far
-  float corr_e = 1.f;
-
   auto step_work = [&](auto edge_tag, const uint8_t* rec, int tok0, int have) {
     constexpr bool kEdge = decltype(edge_tag)::value;    // some token of the step is hidden from some row
     // ---- maxima as fp32, a token per lane; those of V normalised ----
@@ -444,20 +444,24 @@ __global__ void __launch_bounds__(kThreads, Ring<D>::kCtas) attn_kernel(const At
       uint32_t vm = w[NG / 2];
 #pragma unroll
       for (int j = 1; j < NG / 2; ++j) vm = __vmaxu2(vm, w[NG / 2 + j]);
-      int e = (int)(__reduce_max_sync(0xffffffffu, max(vm & 0xffffu, vm >> 16)) >> 7);
-      if (e >= 255) {                                    // a group that is not a number: it must not hide the others
-        e = 0;
+      if (__any_sync(0xffffffffu, max(vm & 0xffffu, vm >> 16) >= (uint32_t)(e_run + 1) << 7)) {
+        int e = e_run;                                   // of the finite ones: a group that is not a number must not hide the others
 #pragma unroll
         for (int j = 0; j < NG / 2; ++j) {
           const int lo = (int)(w[NG / 2 + j] >> 7) & 255, hi = (int)(w[NG / 2 + j] >> 23) & 255;
           e = max(e, max(lo < 255 ? lo : 0, hi < 255 ? hi : 0));
         }
         e = (int)__reduce_max_sync(0xffffffffu, (uint32_t)e);
-      }
-      corr_e = 1.f;
-      if (e > e_run) {
-        corr_e = e - e_run < 127 ? exp2_pos(e_run - e) : 0.f;
+        const float c = e - e_run < 127 ? exp2_pos(e_run - e) : 0.f;
         e_run = e;
+#pragma unroll
+        for (int x = 0; x < HH; ++x)
+#pragma unroll
+          for (int gi = 0; gi < NG; ++gi)
+#pragma unroll
+            for (int ii = 0; ii < 2; ++ii)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) acc[x][gi][ii][i] *= c;
       }
       const float vs = exp2_pos(127 - e_run);            // the largest maximum becomes 1 .. 2
       float vf[NG];
@@ -492,10 +496,10 @@ __global__ void __launch_bounds__(kThreads, Ring<D>::kCtas) attn_kernel(const At
         }
       }
     }
-    // ---- online softmax; the maximum is kept in units of s, P comes with a factor of 2^14 ----
-    float corr[HH][2];
+    // ---- online softmax.  The reference, kept in units of s, follows the maximum when that is 2^kLag times ahead of it (the first
+    // tokens, then hardly ever: no shuffles, no rescaling); P comes with a factor of 2^(14 - kLag) and stays below 2^14 ----
     uint32_t hidden[HH];
-    bool change = corr_e != 1.f;
+    bool ahead = false;
 #pragma unroll
     for (int x = 0; x < HH; ++x) {
       hidden[x] = 0u;
@@ -510,36 +514,46 @@ __global__ void __launch_bounds__(kThreads, Ring<D>::kCtas) attn_kernel(const At
         }
       }
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        float mx = fmaxf(fmaxf(s[x][j], s[x][2 + j]), fmaxf(s[x][4 + j], s[x][6 + j]));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-        const float mn = fmaxf(m[x][j], mx), ref = mn == -INFINITY ? 0.f : mn;
-        corr[x][j] = exp2_fast((m[x][j] - ref) * fh[x][j]);
-        change = change || corr[x][j] != 1.f;
-        m[x][j] = mn;
-        const float off = fmaf(-ref, fh[x][j], 14.f);
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s[x][2 * i + j] = exp2_fast(fmaf(s[x][2 * i + j], fh[x][j], off));
-          sum += s[x][2 * i + j];
-        }
-        l[x][j] = fmaf(l[x][j], corr[x][j], sum);
-        corr[x][j] *= corr_e;
-      }
+      for (int j = 0; j < 2; ++j)
+        ahead = ahead || fmaxf(fmaxf(s[x][j], s[x][2 + j]), fmaxf(s[x][4 + j], s[x][6 + j])) > bar[x][j];
     }
-    if (__any_sync(0xffffffffu, change)) {
+    if (__any_sync(0xffffffffu, ahead)) {
 #pragma unroll
-      for (int x = 0; x < HH; ++x)
+      for (int x = 0; x < HH; ++x) {
+        float corr[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float mx = fmaxf(fmaxf(s[x][j], s[x][2 + j]), fmaxf(s[x][4 + j], s[x][6 + j]));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          const float mn = fmaxf(m[x][j], mx), ref = mn == -INFINITY ? 0.f : mn;
+          corr[j] = exp2_fast((m[x][j] - ref) * fh[x][j]);
+          m[x][j] = mn;
+          bar[x][j] = mn + kLag / fh[x][j];
+          off[x][j] = fmaf(-ref, fh[x][j], 14.f - kLag);
+          l[x][j] *= corr[j];
+        }
 #pragma unroll
         for (int gi = 0; gi < NG; ++gi)
 #pragma unroll
           for (int ii = 0; ii < 2; ++ii)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[x][gi][ii][i] *= corr[x][i & 1];
+            for (int i = 0; i < 4; ++i) acc[x][gi][ii][i] *= corr[i & 1];
+      }
     }
+#pragma unroll
+    for (int x = 0; x < HH; ++x)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[x][2 * i + j] = exp2_fast(fmaf(s[x][2 * i + j], fh[x][j], off[x][j]));
+          sum += s[x][2 * i + j];
+        }
+        l[x][j] += sum;
+      }
     // ---- O^T += V^T P^T ----
 #pragma unroll
     for (int pg = 0; pg < 2; ++pg) {
@@ -605,12 +619,12 @@ __global__ void __launch_bounds__(kThreads, Ring<D>::kCtas) attn_kernel(const At
     for (int j = 0; j < 2; ++j) {
 #pragma unroll
       for (int o = 4; o < 32; o <<= 1) l[x][j] += __shfl_xor_sync(0xffffffffu, l[x][j], o);
-      if (g == 0) { sm_ml[warp][2 * t + j + 8 * x][0] = m[x][j] * fh[x][j]; sm_ml[warp][2 * t + j + 8 * x][1] = l[x][j] * (1.f / 16384.f); }
+      if (g == 0) { sm_ml[warp][2 * t + j + 8 * x][0] = m[x][j] * fh[x][j]; sm_ml[warp][2 * t + j + 8 * x][1] = l[x][j] * (1.f / 8192.f); }
     }
   __syncthreads();                                       // the rings become the merge buffer [warp][pair][nibble of a lane][lane row g]
   float* so = reinterpret_cast<float*>(smem);
   {
-    const float fo = exp2_pos(e_run - 127) * (2.f / 7.f / 16384.f);            // codes' half, maxima's and P's powers of two
+    const float fo = exp2_pos(e_run - 127) * (2.f / 7.f / 8192.f);             // codes' half, maxima's and P's powers of two
 #pragma unroll
     for (int x = 0; x < HH; ++x)
 #pragma unroll
