@@ -341,9 +341,9 @@ struct CompactParams {
   int Hkv, keep;
 };
 
-// One CTA per (four pages of kept tokens, kv head, sequence): the sources of its 64 tokens are looked up side by side, then codes and
+// One CTA per (eight pages of kept tokens, kv head, sequence): the sources of its 128 tokens are looked up side by side, then codes and
 // maxima are copied as they are, 16 bytes (the maxima at head_dim 64: 8) a thread and turn, loads ahead of stores.
-constexpr int kMoveTokens = 64;
+constexpr int kMoveTokens = 128;
 template <int D>
 __global__ void __launch_bounds__(256) compact_kernel(const CompactParams p) {
   using G = Geo<D>;
@@ -375,17 +375,26 @@ __global__ void __launch_bounds__(256) compact_kernel(const CompactParams p) {
     const long long a = from[tok];
     if (a >= 0) v[k] = *reinterpret_cast<const uint4*>(record(a) + (u / kRowUnits) * G::kV + (int)(a % kPage) * G::kRow + 16 * (u % kRowUnits));
   }
-  constexpr int kAmaxUnits = G::kAmaxTok / 8;
-  uint2 m;
-  const int mt = threadIdx.x / kAmaxUnits, mu = threadIdx.x % kAmaxUnits;
-  if (mt < kMoveTokens && from[mt] >= 0) m = *reinterpret_cast<const uint2*>(record(from[mt]) + G::kAmax + (int)(from[mt] % kPage) * G::kAmaxTok + 8 * mu);
+  constexpr int kAmaxUnits = G::kAmaxTok / 8, kMaxTurns = (kMoveTokens * kAmaxUnits + 255) / 256;
+  uint2 m[kMaxTurns];
+#pragma unroll
+  for (int k = 0; k < kMaxTurns; ++k) {
+    const int i = threadIdx.x + 256 * k, tok = i / kAmaxUnits;
+    if (tok < kMoveTokens && from[tok] >= 0)
+      m[k] = *reinterpret_cast<const uint2*>(record(from[tok]) + G::kAmax + (int)(from[tok] % kPage) * G::kAmaxTok + 8 * (i % kAmaxUnits));
+  }
 #pragma unroll
   for (int k = 0; k < kTurns; ++k) {
     const int i = threadIdx.x + 256 * k, tok = i / (2 * kRowUnits), u = i % (2 * kRowUnits);
     const long long b = to[tok];
     if (b >= 0) *reinterpret_cast<uint4*>(record(b) + (u / kRowUnits) * G::kV + (int)(b % kPage) * G::kRow + 16 * (u % kRowUnits)) = v[k];
   }
-  if (mt < kMoveTokens && from[mt] >= 0) *reinterpret_cast<uint2*>(record(to[mt]) + G::kAmax + (int)(to[mt] % kPage) * G::kAmaxTok + 8 * mu) = m;
+#pragma unroll
+  for (int k = 0; k < kMaxTurns; ++k) {
+    const int i = threadIdx.x + 256 * k, tok = i / kAmaxUnits;
+    if (tok < kMoveTokens && to[tok] >= 0)
+      *reinterpret_cast<uint2*>(record(to[tok]) + G::kAmax + (int)(to[tok] % kPage) * G::kAmaxTok + 8 * (i % kAmaxUnits)) = m[k];
+  }
 }
 
 }  // namespace

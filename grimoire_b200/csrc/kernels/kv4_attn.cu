@@ -1040,6 +1040,8 @@ int launch(const AttnParams& p, int nblocks, int mass_pages, cudaStream_t st) {
 
 }  // namespace
 
+constexpr int kNeedsScratch = -3;      // nothing was launched: the call wants grm_kv4_attn_scratch() words
+
 // Scratch of a call in fp32 words, or -2 for arguments that are not served.
 GRM_API long grm_kv4_attn_scratch(int M, int Hq, int Hkv, int D, int block, int max_len, int observe, int alone) {
   Plan pl;
@@ -1049,7 +1051,7 @@ GRM_API long grm_kv4_attn_scratch(int M, int Hq, int Hkv, int D, int block, int 
 
 // One record of 64-bit words (kv4::Args):
 //   data, mass (or 0), table, slots, width, stride, pages, q, ld_q, row_seq, row_pos, gate (or 0), ld_gate, out, ld_o, scratch
-//   (8-byte aligned, or 0 where none is needed), M, Hq, Hkv, D, window, scale, block, observe (0 nothing, 1 set, 2 add), max_len,
+//   (8-byte aligned, or 0: the call returns -3 where it needs some), M, Hq, Hkv, D, window, scale, block, observe (0 nothing, 1 set, 2 add), max_len,
 //   alone
 // max_len bounds the positions of the call's rows for the observed weight and sets how the keys are cut.
 GRM_API int grm_kv4_attn(const void* words, void* stream) {
@@ -1068,7 +1070,8 @@ GRM_API int grm_kv4_attn(const void* words, void* stream) {
   Plan pl;
   const int rc = plan(pl, M, Hq, Hkv, D, block, max_len, alone);
   if (rc) return rc;
-  if (!fits(observe, 0, 2) || (observe && !p.mass) || (!s && pl.floats(M, Hq, D, observe))) return -2;
+  if (!fits(observe, 0, 2) || (observe && !p.mass)) return -2;
+  if (!s && pl.floats(M, Hq, D, observe)) return kNeedsScratch;
   if (!observe) p.mass = nullptr;
   p.M = (int)M; p.Hkv = (int)Hkv; p.G = (int)(Hq / Hkv); p.window = (int)(fits(window, 1, 0x7fffffff) ? window : 0); p.block = (int)block;
   p.add = observe == 2;

@@ -76,6 +76,7 @@ _pack_attn = struct.Struct("21qd4q").pack
 _lib = None
 _INT, _BF16 = torch.int32, torch.bfloat16
 _OBSERVE = {None: 0, "set": 1, "add": 2}
+_NEEDS_SCRATCH = -3                # of grm_kv4_attn: nothing was launched, the keys are cut between CTAs
 
 
 def _cuda():
@@ -269,14 +270,16 @@ def kv4_attn(q: torch.Tensor, row_seq: torch.Tensor, row_pos: torch.Tensor, bloc
                 kv.mass[page[ok], :, place[ok]] = old + w[:, ok].t()
         return out
     lib = _cuda()
+    head = (data.data_ptr(), _ptr(kv.mass), *table, P, qp, qs, seq, pos, gp, gs, op, os_)
+    tail = (M, Hq, Hkv, D, geom.window, geom.scale, block, mode, max_len, alone)
     with _on(dev):
-        floats = lib.grm_kv4_attn_scratch(M, Hq, Hkv, D, block, max_len, mode, alone)
-        if floats < 0:
-            _native.check(int(floats), what)
-        scratch = torch.empty(floats, dtype=torch.float32, device=data.device) if floats else None
-        words = _pack_attn(data.data_ptr(), _ptr(kv.mass), *table, P, qp, qs, seq, pos, gp, gs, op, os_, _ptr(scratch), M, Hq, Hkv, D, geom.window,
-                           geom.scale, block, mode, max_len, alone)
-        _native.check(lib.grm_kv4_attn(words, _native.raw_stream(dev)), what)
+        stream = _native.raw_stream(dev)
+        code = lib.grm_kv4_attn(_pack_attn(*head, 0, *tail), stream)
+        if code == _NEEDS_SCRATCH:
+            floats = lib.grm_kv4_attn_scratch(M, Hq, Hkv, D, block, max_len, mode, alone)
+            scratch = torch.empty(floats, dtype=torch.float32, device=data.device)
+            code = lib.grm_kv4_attn(_pack_attn(*head, scratch.data_ptr(), *tail), stream)
+        _native.check(code, what)
     return out
 
 
