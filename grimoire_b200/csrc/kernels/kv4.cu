@@ -322,7 +322,8 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectParams 
     if (t < wend) judge(t, gt, eq);
     const uint32_t gts = __ballot_sync(0xffffffffu, gt), eqs = __ballot_sync(0xffffffffu, eq), under = (1u << lane) - 1u;
     const int eq_here = eq_before + __popc(eqs & under);
-    if (gt || (eq && eq_here < need)) out[gt_before + __popc(gts & under) + min(eq_here, need)] = t;
+    const int to = gt_before + __popc(gts & under) + min(eq_here, need);
+    if ((gt || (eq && eq_here < need)) && to < p.keep) out[to] = t;          // (more only where the weights change meanwhile)
     gt_before += __popc(gts);
     eq_before += __popc(eqs);
   }

@@ -37,7 +37,7 @@ struct AttnParams {
   float scale_log2;         // softmax scale * log2(e)
 };
 
-__device__ __forceinline__ int row_len(const AttnParams& p, int row) { return max(0, min(p.row_pos[row] + 1, p.t.width * kPage)); }
+__device__ __forceinline__ int row_len(const AttnParams& p, int row) { return max(0, min(p.row_pos[row], p.t.width * kPage - 1) + 1); }
 __device__ __forceinline__ int row_first(const AttnParams& p, int len) { return (p.window > 0 && len > p.window) ? len - p.window : 0; }
 
 template <int D>
@@ -214,21 +214,6 @@ __device__ __forceinline__ float load_q(const AttnParams& p, int row, int head, 
   return fmaxf(fabsf(p.scale_log2) * (2.f / 7.f / 16384.f) * exp2_pos(min(e - 127, 127)), 1e-37f);
 }
 
-// Attention of up to 8 * HH (row, head) pairs of one kv head over one split of the sequence's pages.
-//
-// Bound by the cache's bytes (18 D per 16 tokens and kv head) and, close behind, by issue slots (a record has to cost a warp less
-// than four times the ~100 cycles in which an SM receives it), of them most by the integer pipe that unpacks the codes.  Hence
-//   * a warp owns steps of two pages (32 tokens); a page is ONE bulk copy (the record is contiguous) into a per-warp ring;
-//   * S^T[token][pair] = K Q^T with the codes, as the fp16 integers that they are, as the MMA's row operand: 16 tokens fill its
-//     rows and 8 pairs its columns.  q is scaled by a power of two to fill fp16's range (bf16 has fewer bits: exact); a
-//     quantisation group is two k-steps whose sum is scaled by the group's maximum in fp32;
-//   * O^T[dim][pair] += V^T[dim][token] P^T[token][pair].  P is multiplied by the token's V maximum in fp32, rounded to fp16
-//     (11 bits, against the output's 8) and transposed from the accumulator's layout to the column operand's by one movmatrix
-//     per 8 tokens; a running power of two keeps the largest product at the top of fp16's range, whatever the values'
-//     magnitude.  (Rounding P first and multiplying in fp16 saves 14 instructions a page and loses tokens whose values are
-//     2^-24 of the largest ones.)
-//   * the maxima are unpacked once a step, a token per lane, and handed round through shared memory.
-// Softmax statistics, scores and outputs are fp32.
 // Rows of unit group u and the tokens they see.
 struct Rows {
   int row0, nr, slot;
@@ -302,6 +287,21 @@ __device__ __forceinline__ int stream_schedule(const AttnParams& p, int (&before
   return pages_per_cta(p, run);
 }
 
+// Attention of up to 8 * HH (row, head) pairs of one kv head over one split of the sequence's pages.
+//
+// Bound by the cache's bytes (18 D per 16 tokens and kv head) and, close behind, by issue slots (a record has to cost a warp less
+// than four times the ~100 cycles in which an SM receives it), of them most by the integer pipe that unpacks the codes.  Hence
+//   * a warp owns steps of two pages (32 tokens); a page is ONE bulk copy (the record is contiguous) into a per-warp ring;
+//   * S^T[token][pair] = K Q^T with the codes, as the fp16 integers that they are, as the MMA's row operand: 16 tokens fill its
+//     rows and 8 pairs its columns.  q is scaled by a power of two to fill fp16's range (bf16 has fewer bits: exact); a
+//     quantisation group is two k-steps whose sum is scaled by the group's maximum in fp32;
+//   * O^T[dim][pair] += V^T[dim][token] P^T[token][pair].  P is multiplied by the token's V maximum in fp32, rounded to fp16
+//     (11 bits, against the output's 8) and transposed from the accumulator's layout to the column operand's by one movmatrix
+//     per 8 tokens; a running power of two keeps the largest product at the top of fp16's range, whatever the values'
+//     magnitude.  (Rounding P first and multiplying in fp16 saves 14 instructions a page and loses tokens whose values are
+//     2^-24 of the largest ones.)
+//   * the maxima are unpacked once a step, a token per lane, and handed round through shared memory.
+// Softmax statistics, scores and outputs are fp32.
 template <int D, int HH>
 __global__ void __launch_bounds__(kThreads, Ring<D>::kCtas) attn_kernel(const AttnParams p) {
   using Gm = Geo<D>;

@@ -5,7 +5,7 @@ Same contract as the reference's ``generate_tokens<Engine>`` template (include/b
 82-432), which is written against an engine *concept* so host tests can drive it with fake engines
 (tests/test_generation.cpp).  Here the concept is the ``EngineLike`` protocol: anything that offers
 ``open / release / prefill / decode_rows / commit_rows`` (and optionally ``draft`` / ``rollback`` /
-``prefix_reuse``) can be driven -- the real ``Engine`` or the fakes of tests/test_generation.py.
+``prefix_reuse`` / ``trim``) can be driven -- the real ``Engine`` or the fakes of tests/test_generation.py.
 
 Speculation: K draft tokens come from a drafter (MTP chain, copy / prompt-lookup, or none); ONE
 verify pass scores the candidate block as K+1 rows of the same conversation; the longest prefix
@@ -177,6 +177,8 @@ def generate_tokens(engine: EngineLike, prompt: Sequence[int], opts: GenerationO
                 break
             if len(out) >= opts.max_new:
                 break
+            if hasattr(engine, "trim"):
+                engine.trim(seq)                       # KV eviction, where the engine is set up for it
             pos = seq.length
             drafts: list[int] = []
             if opts.draft_depth > 0 and opts.drafter is not None:

@@ -212,7 +212,7 @@ class MtpDrafter:
             # entry now that its next token (the first of this call) is known
             one = torch.full((1,), seq.slot, dtype=torch.int32, device=eng.device)
             rb1 = RowBatch(tokens_dev[:1], one, torch.full((1,), pos0 - 1, dtype=torch.int32, device=eng.device), mode="decode",
-                           splits=K.decode_splits(pos0, 1, self.head.inner.geom.Hkv))
+                           splits=eng._splits_for(1, pos0))
             self.head.forward(rb1, prev[1].unsqueeze(0), eng.decode_buf, self.kvl, eng.kv.table)
             self.stats["warm_rows"] += 1
         rows = m - 1 if last else m                      # the last prompt position has no next token yet
@@ -242,7 +242,7 @@ class MtpDrafter:
         slot_t = torch.full((1,), seq.slot, dtype=torch.int32, device=dev)
         for j in range(depth):
             rp = torch.full((1,), pos + j, dtype=torch.int32, device=dev)
-            rb = RowBatch(self._ids[:1], slot_t, rp, mode="decode", splits=K.decode_splits(pos + j + 1, 1, self.head.inner.geom.Hkv))
+            rb = RowBatch(self._ids[:1], slot_t, rp, mode="decode", splits=eng._splits_for(1, pos + j + 1))
             logits, h2 = self.head.forward(rb, hidden, eng.decode_buf, self.kvl, eng.kv.table, logits_rows=1, flip=j & 1)
             K.argmax_rows(logits, self._ids[:1])
             self._drafts[j: j + 1].copy_(self._ids[:1])
@@ -262,7 +262,7 @@ class MtpDrafter:
             toks = torch.tensor(keep[1:], dtype=torch.int32, device=dev)
             pos = torch.arange(pos0, pos0 + a, dtype=torch.int32, device=dev)
             rb = RowBatch(toks, torch.full((a,), seq.slot, dtype=torch.int32, device=dev), pos, mode="decode",
-                          splits=K.decode_splits(pos0 + a, a, self.head.inner.geom.Hkv))
+                          splits=eng._splits_for(a, pos0 + a))
             self.head.forward(rb, hid[:a], eng.decode_buf, self.kvl, eng.kv.table)
             self.stats["catchup_rows"] += a
         self.pending[seq.slot] = (pos0 + a, hid[a].clone())

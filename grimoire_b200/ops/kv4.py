@@ -45,8 +45,8 @@ class Kv4Layer:
         if data.numel() == 0 or data.data_ptr() % 16:
             raise ValueError("4-bit KV pages: data must hold a page and start on a 16-byte boundary")
         if mass is not None and (mass.dtype != torch.float32 or not mass.is_contiguous() or mass.shape != (data.shape[0], data.shape[1], PAGE)
-                                 or mass.device != data.device):
-            raise ValueError("4-bit KV pages: mass must be a contiguous fp32 [pages][kv heads][16] on the device of the data")
+                                 or mass.device != data.device or mass.data_ptr() % 16):
+            raise ValueError("4-bit KV pages: mass must be a contiguous fp32 [pages][kv heads][16] on the device of the data, on a 16-byte boundary")
 
     @staticmethod
     def alloc(pages: int, Hkv: int, D: int, device, mass: bool = False) -> "Kv4Layer":
@@ -218,7 +218,7 @@ def kv4_attn(q: torch.Tensor, row_seq: torch.Tensor, row_pos: torch.Tensor, bloc
              out: torch.Tensor, max_len: int, gate: Optional[torch.Tensor] = None, block: int = 1, observe: Optional[str] = None, alone: bool = False) -> torch.Tensor:
     """Attention of M rows over the 4-bit pages: row m (bf16 [Hq * D], after norm and RoPE) of sequence slot ``row_seq[m]`` sees
     the cached positions 0 .. ``row_pos[m]``, the last ``geom.window`` of them with a window, and leaves its output (bf16,
-    times sigmoid(``gate[m]``) with a gate) in ``out[m]``.  A row that sees no key (a negative position, no mapped page)
+    times sigmoid(``gate[m]``) with a gate) in ``out[m]`` (which must not overlap ``q``).  A row that sees no key (a negative position, no mapped page)
     gives zeros.  ``max_len`` is the longest row's ``row_pos + 1`` as the host knows it: it sets how the keys are split, and
     bounds the tokens that ``observe`` covers.
 
@@ -330,8 +330,8 @@ def kv4_select(kv: Kv4Layer, slots: Optional[torch.Tensor], lengths: torch.Tenso
 
 def kv4_compact(kv: Kv4Layer, slots: Optional[torch.Tensor], idx: torch.Tensor, block_table: torch.Tensor, dst_table: torch.Tensor) -> None:
     """Copy token ``idx[i][h][j]`` of sequence ``slots[i]`` (kv head h, codes, maxima and mass as they are) to place j of the
-    pages ``dst_table[i]`` (int32 [S][>= ceil(keep / 16)]).  The destination pages must not be among the sources: pages that
-    other sequences share stay intact, and the caller swaps the tables afterwards.  Places whose ``idx`` is -1 stay as they
+    pages ``dst_table[i]`` (int32 [S][>= ceil(keep / 16)]).  The destination pages must not be among the sources, nor come twice:
+    pages that other sequences share stay intact, and the caller swaps the tables afterwards.  Places whose ``idx`` is -1 stay as they
     are."""
     data = kv.data
     P, Hkv, rec = data.shape

@@ -1,12 +1,20 @@
 """The engine over 4-bit KV pages: prompts in chunks, decode steps, verify blocks, and conversations cut by eviction."""
+import dataclasses
+
 import pytest
 import torch
 
 from grimoire_b200.config import EngineConfig
 from grimoire_b200.engine.engine import Engine, EngineLimits
-from grimoire_b200.models.config import tiny_dense
+from grimoire_b200.engine.generation import CopyDrafter, GenerationOptions, generate_tokens
+from grimoire_b200.models.config import FULL_ATTN, LINEAR_ATTN, ModelConfig, tiny_dense, tiny_gemma4, tiny_qwen4_exp
 from grimoire_b200.models.dense import DenseModel
-from grimoire_b200.models.synthetic import random_state_dict
+from grimoire_b200.models.gemma4 import Gemma4Model
+from grimoire_b200.models.hybrid import HybridModel, _DictSource
+from grimoire_b200.models.mtp import MtpDrafter, MtpHead
+from grimoire_b200.models.qwen4_exp import Qwen4ExpModel
+from grimoire_b200.models.synthetic import random_gemma4_state_dict, random_qwen4_exp_state_dict, random_state_dict
+from grimoire_b200.ops import kv4
 from grimoire_b200.ops.kv4 import Kv4Layer
 from grimoire_b200.sched.scheduler import Scheduler
 
@@ -188,3 +196,75 @@ def test_refusals():
         with pytest.raises(ValueError):
             EngineConfig(**kw).validate()
     EngineConfig(kv_bits=4, kv_keep=4096).validate()
+
+
+def _family(name, device):
+    if name == "hybrid":
+        cfg = ModelConfig(model_type="qwen3_5", hidden_size=512, num_hidden_layers=4, num_attention_heads=4, num_key_value_heads=2, head_dim=128,
+                          vocab_size=4096, intermediate_size=1024, partial_rotary_factor=0.5, attn_output_gate=True, qk_norm=True,
+                          norm_zero_centered=True, layer_types=[LINEAR_ATTN, LINEAR_ATTN, LINEAR_ATTN, FULL_ATTN], linear_num_key_heads=2,
+                          linear_num_value_heads=4, linear_key_head_dim=128, linear_value_head_dim=128, quant="int4")
+        return HybridModel.random(cfg, device, seed=2, max_slots=2, gen_device="cpu")
+    if name == "gemma4":
+        cfg = dataclasses.replace(tiny_gemma4(), hidden_size=512, head_dim=128, intermediate_size=1024, embed_scale=512 ** 0.5)
+        return Gemma4Model.from_state_dict(cfg, random_gemma4_state_dict(cfg, seed=2), device)
+    cfg = tiny_qwen4_exp(4)
+    return Qwen4ExpModel.from_checkpoint(_DictSource(cfg, random_qwen4_exp_state_dict(cfg, 2)), device)
+
+
+@pytest.mark.parametrize("name,device", [("hybrid", "cpu"), ("gemma4", "cpu"), ("qwen4_exp", "cpu"),
+                                         *(pytest.param(n, "cuda", marks=pytest.mark.gpu) for n in ("hybrid", "gemma4"))])
+def test_other_families_run_over_four_bit_pages(name, device):
+    """Gated, windowed and sparse attention layers: prompts in chunks, decode steps, a replayed step."""
+    lim = dict(max_slots=2, max_ctx=128, prefill_chunk=32, max_decode_rows=4)
+    got = []
+    for bits in (8, 4):
+        eng = Engine(_family(name, device), EngineLimits(kv_bits=bits, **lim))
+        s, V = eng.open(), eng.model.cfg.vocab_size
+        ids = [t % V for t in _prompt(56, 3)]
+        logits = [eng.prefill(s, ids[:50]).float().cpu()] + _feed(eng, s, ids[50:54])
+        if device == "cuda":
+            for t in ids[54:]:
+                _, lg = eng.decode_rows([t], [s], [s.length], use_graph=True, return_logits=True)
+                logits.append(lg[0].float().cpu().clone())
+                eng.commit_rows([s], [t], [s.length])
+        got.append(torch.stack(logits))
+        eng.release(s)
+    assert bool(torch.isfinite(got[1]).all()) and not torch.equal(got[0], got[1])
+    assert float((got[0] - got[1]).abs().max()) < 0.25 * float(got[0].abs().max())
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_draft_head_over_four_bit_pages_reproduces_greedy(device, monkeypatch):
+    """Speculative output equals plain output, and every call is planned for the lengths that it has."""
+    cfg = dataclasses.replace(tiny_dense(), tie_word_embeddings=False)
+    lim = EngineLimits(max_slots=2, max_ctx=160, prefill_chunk=16, max_decode_rows=8, extra_kv_layers=1, kv_bits=4)
+    p = _prompt(37, 3)
+    plain = Engine(DenseModel.random(cfg, device, seed=1, gen_device="cpu"), lim)
+    plain.enable_speculation()
+    want = plain.generate(p, 24, use_graph=False)
+    model = DenseModel.random(cfg, device, seed=1, gen_device="cpu")
+    eng = Engine(model, lim)
+    drafter = MtpDrafter(eng, MtpHead.random_from_target(model, seed=1, noise=0.01, gen_device="cpu"))
+    real, calls = kv4.kv4_attn, []
+
+    def watched(q, row_seq, row_pos, table, kv, geom, out, max_len, *a, **k):
+        calls.append((int(row_pos.max()) + 1, max_len))
+        return real(q, row_seq, row_pos, table, kv, geom, out, max_len, *a, **k)
+
+    monkeypatch.setattr(kv4, "kv4_attn", watched)
+    opts = GenerationOptions(max_new=24, draft_depth=3, drafter=drafter, use_graph=False)
+    toks, _ = generate_tokens(eng, p, opts)
+    assert toks == want and opts.stats.rounds > 0
+    assert calls and all(n <= bound for n, bound in calls)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("drafts", [False, True])
+def test_single_requests_stay_inside_the_budget(device, drafts):
+    """The path of a single request (with and without drafts from the conversation) cuts the cache as the scheduler does."""
+    eng = _engine(device, kv_keep=48, kv_recent=16, kv_slack=16, max_ctx=96)
+    opts = GenerationOptions(max_new=60, draft_depth=3 if drafts else 0, drafter=CopyDrafter() if drafts else None, use_graph=False)
+    s = eng.open()
+    toks, _ = generate_tokens(eng, _prompt(10, 5) * 5, opts, seq=s)
+    assert len(toks) == 60 and eng.counters["kv_evictions"] >= 2 and s.length + s.dropped >= 50 + 59 and s.length < 64 + 4

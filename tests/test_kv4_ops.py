@@ -560,6 +560,8 @@ def test_refusals(device):
         lambda: kv4.kv4_append(kv4.Kv4Layer(kv.data[:, :1]), x, x, i32(0, 1), i32(0, 0), table),
         lambda: kv4.kv4_append(kv4.Kv4Layer(kv.data, kv.mass[:2]), x, x, i32(0, 1), i32(0, 0), table),
         lambda: kv4.kv4_append(kv, x.t().contiguous().t(), x, i32(0, 1), i32(0, 0), table),
+        lambda: kv4.Kv4Layer(kv.data, torch.zeros(4 * Hkv * PAGE + 1, device=device)[1:].view(4, Hkv, PAGE)),
+        lambda: kv4.Kv4Layer(torch.zeros(18 * D + 8, dtype=torch.uint8, device=device)[8:].view(1, 1, 18 * D)),
         lambda: kv4.kv4_gather(kv, table, None, None, x[None].float(), x[None]),
         lambda: kv4.kv4_gather(kv, table, None, None, x, x),
         lambda: kv4.kv4_gather(kv, table, None, None, x[None].expand(2, 2, Hkv * D), x[None].expand(2, 2, Hkv * D)),
@@ -764,3 +766,86 @@ def test_block_with_tokens_of_far_larger_values(device):
         ref, size, _, top = c.expect([0] * block, pos, q, G, 0.1)
         scores_in_range(D, top)
         close(c.attend([0] * block, pos, q, G, 0.1, block=block), ref, size)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("window", [0, 20])
+def test_rows_at_the_largest_position_see_the_whole_table(device, window):
+    """Positions end where the table does: 2^31 - 1 is the last place of the last page, which need not be mapped."""
+    D, Hkv, G = 64, 1, 3
+    c = Cache([48], Hkv, D, device, seed=60)
+    q = torch.randn(2, Hkv * G * D, generator=torch.Generator().manual_seed(6)).bfloat16()
+    geom = AttnGeom(Hkv * G, Hkv, D, D, 0.2, window=window)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=device)
+    out = torch.zeros(2, Hkv * G * D, dtype=torch.bfloat16, device=device)
+    slot = int(c.slots[0])
+    kv4.kv4_attn(q.to(device), i32(slot, slot), i32(2 ** 31 - 1, -2 ** 31), c.table, c.kv, geom, out, 64, observe="set")
+    last = c.table.shape[1] * PAGE - 1                                                # 63: the last 16 places are not mapped
+    ref, size, weights, top = c.expect([0], [47], q[:1], G, 0.2, max(0, window - (last - 47)))
+    scores_in_range(D, top)
+    close(out[:1].cpu(), ref, size)
+    assert not bool(out[1].any())
+    assert float((c.mass_of(0).double() - weights[0]).abs().max()) < 2 ** -9 * G
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_one_row_for_all_heads_and_rows_of_the_queries(device):
+    """Broadcast rows (stride 0) are read like any others."""
+    D, Hkv, G = 128, 2, 4
+    c = Cache([100, 37], Hkv, D, device, seed=61)
+    q = torch.randn(1, Hkv * G * D, generator=torch.Generator().manual_seed(7)).bfloat16()
+    out = c.attend([0, 1, 0], [99, 36, 50], q.expand(3, -1), G, 0.1, gate=q.expand(3, -1))
+    ref, size, _, top = c.expect([0, 1, 0], [99, 36, 50], q.expand(3, -1), G, 0.1)
+    scores_in_range(D, top)
+    gate = torch.sigmoid(q.double())
+    close(out, ref * gate, size * gate)
+
+
+@pytest.mark.gpu
+def test_a_captured_cut_of_two_conversations_side_by_side():
+    """Write, observe, select, compact and read back as one graph per cache; two of them replayed on two streams at once give what
+    eager calls give."""
+    D, Hkv, G, n, keep = 128, 2, 4, 90, 33
+    geom = AttnGeom(Hkv * G, Hkv, D, D, 0.1)
+    x = [torch.randn(1, Hkv * D, device="cuda").bfloat16() for _ in range(2)]
+    q = torch.randn(1, Hkv * G * D, device="cuda").bfloat16()
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")
+
+    def job(c):
+        slot, pos, length, dst = c.slots[:1].cuda(), i32(n), i32(n + 1), c.fresh[:3][None].contiguous()
+        rows = torch.arange(1, dtype=torch.int32, device="cuda")
+        out, ok, ov = torch.zeros_like(q), *(torch.zeros(1, keep, Hkv * D, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+
+        def run():
+            kv4.kv4_append(c.kv, x[0], x[1], pos, slot, c.table)
+            kv4.kv4_attn(q, slot, pos, c.table, c.kv, geom, out, n + 1, observe="set")
+            idx = kv4.kv4_select(c.kv, slot, length, c.table, keep, 8, 2)
+            kv4.kv4_compact(c.kv, slot, idx, c.table, dst)
+            kv4.kv4_gather(c.kv, dst, rows * 0, None, ok, ov)
+            return idx
+        return run, (out, ok, ov)
+
+    caches = [Cache([n + 6], Hkv, D, "cuda", seed=70 + i) for i in range(2)]
+    wants = []
+    for c in caches:
+        run, outs = job(c)
+        idx = run()
+        wants.append([idx.clone()] + [t.clone() for t in outs] + [c.kv.data.clone(), c.kv.mass.clone()])
+    graphs, got = [], []
+    for c in caches:
+        run, outs = job(c)
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            idx = run()
+        graphs.append(gr)
+        got.append([idx, *outs, c.kv.data, c.kv.mass])
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(10):
+        for st, gr in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                gr.replay()
+    torch.cuda.synchronize()
+    for w, r in zip(wants, got):
+        for a, b in zip(w, r):
+            assert torch.equal(a.view(torch.uint8) if a.is_floating_point() else a, b.view(torch.uint8) if b.is_floating_point() else b)
