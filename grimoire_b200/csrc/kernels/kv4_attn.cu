@@ -172,11 +172,19 @@ __device__ __forceinline__ void nibbles(const Magic& mg, uint32_t x, uint32_t y,
 
 __device__ __forceinline__ float exp2_pos(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }   // 2^e, -127 < e < 128
 
+// The power of two that brings a query row whose largest magnitude has the bits ``mx`` to the top of fp16's range (exact: bf16 has
+// fewer bits).  ``f``: what a product with the codes' halves has to be multiplied by (and by the group's maximum) to give the score in
+// the log2 domain; positive, so that maxima stay maxima: a negative softmax scale goes into the operand.
+__device__ __forceinline__ float q_scale(const AttnParams& p, uint32_t mx, float& f) {
+  const int e = max((int)(mx >> 7), 14);                 // biased exponent
+  const float up = e == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)(268 - e) << 23);   // 2^14 / 2^(e - 127)
+  f = fmaxf(fabsf(p.scale_log2) * (2.f / 7.f / 16384.f) * exp2_pos(min(e - 127, 127)), 1e-37f);
+  return p.scale_log2 < 0.f ? -up : up;
+}
+
 // Lane (g, t)'s part of one query row as the column operand of K Q^T (the row is pair g's): q times a power of two that fills
-// fp16's range (exact: bf16 has fewer bits), k-step (group gi = 2 w + half, odd) made of the words w and w + NG / 2 of the
-// lane's NG words of codes, nibbles odd and odd + 2.  Returns what a product with the codes' halves has to be multiplied by
-// (and by the group's maximum) to give the score in the log2 domain; positive, so that maxima stay maxima: a negative softmax
-// scale goes into the operand.
+// fp16's range, k-step (group gi = 2 w + half, odd) made of the words w and w + NG / 2 of the lane's NG words of codes, nibbles
+// odd and odd + 2.  Returns q_scale()'s factor.
 template <int D>
 __device__ __forceinline__ float load_q(const AttnParams& p, int row, int head, bool live, int t, uint32_t (&qb)[D / 32][2][2]) {
   constexpr int NG = D / 32;
@@ -196,9 +204,8 @@ __device__ __forceinline__ float load_q(const AttnParams& p, int row, int head, 
     }
   mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
   mx = max(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-  const int e = max((int)(mx >> 7), 14);                 // biased exponent of the largest magnitude
-  float up = e == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float((uint32_t)(268 - e) << 23);   // 2^14 / 2^(e - 127)
-  up = p.scale_log2 < 0.f ? -up : up;
+  float f;
+  const float up = q_scale(p, mx, f);
 #pragma unroll
   for (int gi = 0; gi < NG; ++gi) {
     float a[4], b[4];
@@ -211,7 +218,7 @@ __device__ __forceinline__ float load_q(const AttnParams& p, int row, int head, 
 #pragma unroll
       for (int j = 0; j < 2; ++j) qb[gi][odd][j] = attn_mma::pack_f16x2(a[odd + 2 * j], b[odd + 2 * j]);
   }
-  return fmaxf(fabsf(p.scale_log2) * (2.f / 7.f / 16384.f) * exp2_pos(min(e - 127, 127)), 1e-37f);
+  return f;
 }
 
 // Rows of unit group u and the tokens they see.
@@ -673,6 +680,452 @@ __global__ void __launch_bounds__(kThreads, Ring<D>::kCtas) attn_kernel(const At
   }
 }
 
+// Attention of up to 128 (row, head) pairs of one kv head over one split of the pages, for blocks of many rows: a page is
+// unpacked once for 128 pairs (the kernel above: once for 16), and the products run on tcgen05.
+//
+//   * Four warps unpack 64 tokens (a page each) into fp16 operand tiles of 128-byte swizzled rows: (code - 8) / 2 times the
+//     group's maximum, which fp16 holds exactly (3 + 8 bits) once the maxima are scaled by a power of two, K by one of its own
+//     page, V by a running one of the CTA.  A word of codes becomes the 16 bytes of dims (0, 4, 1, 5, 2, 6, 3, 7): q is laid out
+//     and the output read in that order.
+//   * One thread issues S = Q K^T (64 columns of TMEM, two buffers) and O += P V (V as it lies, tokens by dims: the MN-major
+//     operand), so that S of the next tokens runs under the softmax of these.
+//   * Four warps do the softmax, a pair a thread: no shuffles, the reference follows the maximum when that is 2^kLag ahead.  P, rounded
+//     to fp16 (11 bits, against the output's 8), takes the place of S in TMEM.
+// A V group that is not finite would reach rows that do not see it as 0 * NaN: it is unpacked as zero, and the rows that see its
+// token remember the group.  Scores, statistics and outputs are fp32.
+template <int D>
+struct Tile {
+  static constexpr int kTok = 64, kRows = 128, kThreads = 288;
+  static constexpr int kQ = kRows * D * 2, kK = kTok * D * 2;
+  static constexpr int kBytes = kQ + 4 * kK + 1024;      // K and V twice
+  static constexpr int kCols = D == 256 ? 512 : 256;     // TMEM: S [0, 64) and [64, 128), P in the place of S, O behind them
+  static constexpr int kCtas = D == 256 ? 1 : 2;         // an SM
+};
+
+__device__ __forceinline__ void tmem_st_x32(uint32_t taddr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]),
+        "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]),
+        "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+      ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+// D[tmem] (+)= A[tmem] * B[smem]; A: a row a lane, two fp16 a column
+__device__ __forceinline__ void tc_mma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t desc_b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "r"(tmem_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_done() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void smem_to_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// What the unpacking warps tell the softmax about 64 tokens.
+struct alignas(16) TileNote {
+  float kf[4];               // K: what a product of the page has to be multiplied by
+  int e;                     // V: biased exponent of the largest maximum so far
+  uint8_t have[4], bad[4];   // a page is there; it holds a V group that is not finite
+  uint8_t groups[64];        // which ones, a bit each, by token
+};
+
+// rows_of(), by a warp.
+__device__ __forceinline__ Rows rows_of_warp(const AttnParams& p, int u) {
+  Rows r;
+  const int blk = u / p.groups, grp = u % p.groups, lane = threadIdx.x & 31;
+  r.row0 = blk * p.block + grp * p.rows;
+  r.nr = min(p.rows, p.block - grp * p.rows);
+  r.slot = p.row_seq[blk * p.block];
+  int len_hi = 0, len_lo = 0x7fffffff, first_lo = 0x7fffffff, first_hi = 0;
+  for (int i = lane; i < r.nr; i += 32) {
+    const int len = row_len(p, r.row0 + i), first = row_first(p, len);
+    len_lo = min(len_lo, len);
+    if (len > 0) {                                       // a row without keys widens nothing
+      len_hi = max(len_hi, len);
+      first_lo = min(first_lo, first); first_hi = max(first_hi, first);
+    }
+  }
+  r.len_hi = __reduce_max_sync(0xffffffffu, len_hi); r.len_lo = __reduce_min_sync(0xffffffffu, len_lo);
+  r.first_lo = __reduce_min_sync(0xffffffffu, first_lo); r.first_hi = __reduce_max_sync(0xffffffffu, first_hi);
+  r.page_lo = r.len_hi > 0 ? r.first_lo / kPage : 0;
+  r.pages = r.len_hi > 0 ? (r.len_hi + kPage - 1) / kPage - r.page_lo : 0;
+  return r;
+}
+
+// The 16 bytes that a word of codes becomes: dims 0, 4, 1, 5, 2, 6, 3, 7 times the maxima (of dims 0 - 3, of dims 4 - 7).
+__device__ __forceinline__ uint4 unpack_word(const Magic& mg, uint32_t x, uint32_t a) {
+  const uint32_t y = x >> 8;
+  return make_uint4(h2_mul(h2_fma(low_nibble(x, mg.one), mg.even, 0xe008e008u), a), h2_mul(h2_fma(high_nibble(x, mg.one), mg.odd, 0xd080d080u), a),
+                    h2_mul(h2_fma(low_nibble(y, mg.one), mg.even, 0xe008e008u), a), h2_mul(h2_fma(high_nibble(y, mg.one), mg.odd, 0xd080d080u), a));
+}
+// Largest exponent of the finite ones of two bf16 maxima.
+__device__ __forceinline__ int top_exponent(uint32_t w) {
+  const int lo = (int)(w >> 7) & 255, hi = (int)(w >> 23) & 255;
+  return max(lo < 255 ? lo : 0, hi < 255 ? hi : 0);
+}
+// B operand with the dims contiguous: 64 of them a 128-byte swizzled row, a token a row, eight rows 1024 bytes.  One instruction takes
+// 64 dims and 16 tokens, so that the only stride is the one between groups of eight tokens.
+__device__ __forceinline__ uint64_t tokens_by_dims_desc(uint32_t smem_addr) {
+  return (uint64_t)((smem_addr & 0x3FFFFu) >> 4) | (uint64_t)(1024 >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+
+template <int D>
+__global__ void __launch_bounds__(Tile<D>::kThreads, Tile<D>::kCtas) tile_kernel(const AttnParams p) {
+  using Gm = Geo<D>;
+  using T = Tile<D>;
+  constexpr int NG = Gm::kGroups, NW = NG / 2;           // words of a token's K (or V) maxima
+  constexpr int kUnits = D / 64;                         // 16-byte units of K (or V) codes a lane and page
+  constexpr int kBox = T::kTok * 128;                    // bytes of 64 dims of the tokens
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t b_q, b_p, b_k[2], b_v[2], b_s[2], b_o[2];
+  __shared__ TileNote notes[4];                          // of blocks j mod 4
+  __shared__ int v_top[2][4];
+  __shared__ uint32_t tmem_holder;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t *sQ = smem, *sK = sQ + T::kQ, *sV = sK + 2 * T::kK;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  grm_pdl_wait();
+  const int u = blockIdx.z, kvh = blockIdx.y;
+  const Rows rw = rows_of_warp(p, u);
+  const int np = rw.nr * p.G;
+  int per = (rw.pages + p.splits - 1) / p.splits;
+  per = (per + 3) / 4 * 4;
+  const int n0 = min((int)blockIdx.x * per, rw.pages), n1 = min(n0 + per, rw.pages);
+  const int pbeg = rw.page_lo + n0, pend = rw.page_lo + n1, nblk = (n1 - n0 + 3) / 4;
+  if (tid == 0) {
+    mbar_init(&b_q, 128); mbar_init(&b_p, 32 * ((np + 31) / 32));
+    for (int i = 0; i < 2; ++i) { mbar_init(&b_k[i], 128); mbar_init(&b_v[i], 128); mbar_init(&b_s[i], 1); mbar_init(&b_o[i], 1); }
+    mbar_fence_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(&tmem_holder, T::kCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_holder;
+  uint32_t limit = 4000000u;                             // a wait that runs out is on record in the status block: the next ones are short, the loops end as always
+
+  if (warp == 8) {
+    if (lane == 0 && nblk > 0) {
+      constexpr uint32_t idesc = make_idesc(128, 64, 0, 0), idesc_mn = idesc | (1u << 16);
+      auto issue_s = [&](int j) {
+        tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          tc_mma_f16(tmem + 64 * (j & 1), make_sw128_kmajor_desc(smem_u32(sQ) + (k >> 2) * (T::kRows * 128)) + (uint64_t)((k & 3) * 2),
+                     make_sw128_kmajor_desc(smem_u32(sK) + (j & 1) * T::kK + (k >> 2) * kBox) + (uint64_t)((k & 3) * 2), idesc, k != 0 ? 1u : 0u);
+        tc_commit(&b_s[j & 1]);
+      };
+      bool good = mbar_wait(&b_q, 0u, p.status, 0x4b563410u) && mbar_wait(&b_k[0], 0u, p.status, 0x4b563411u);
+      if (good) issue_s(0);
+      for (int j = 0; j < nblk && good; ++j) {
+        if (j + 1 < nblk) {                              // (its TMEM buffer holds P(j - 1), whose product was issued before)
+          good = mbar_wait(&b_k[(j + 1) & 1], (uint32_t)((j + 1) >> 1) & 1u, p.status, 0x4b563412u);
+          if (!good) break;
+          issue_s(j + 1);
+        }
+        good = mbar_wait(&b_p, (uint32_t)j & 1u, p.status, 0x4b563413u) && mbar_wait(&b_v[j & 1], (uint32_t)(j >> 1) & 1u, p.status, 0x4b563414u);
+        if (!good) break;
+        tc_fence_after();
+#pragma unroll
+        for (int x = 0; x < D / 64; ++x)
+#pragma unroll
+          for (int k = 0; k < T::kTok / 16; ++k)
+            tc_mma_f16_ts(tmem + 128 + 64 * x, tmem + 64 * (j & 1) + 8 * k,
+                          tokens_by_dims_desc(smem_u32(sV) + (j & 1) * T::kK + x * kBox + k * 2048), idesc_mn, (k != 0 || j != 0) ? 1u : 0u);
+        tc_commit(&b_o[j & 1]);
+      }
+    }
+  } else if (warp >= 4) {
+    // ---- unpack: a page a warp ----
+    const Magic mg;
+    const int w4 = warp - 4;
+    // the page of the next 64 tokens is on its way while these are unpacked, the id of the one after that too
+    uint4 ck[kUnits], cv[kUnits], ck_next[kUnits], cv_next[kUnits];
+    uint32_t am[kUnits][2 * NW], am_next[kUnits][2 * NW];          // maxima: K, then V
+    auto id_of = [&](int j) {
+      const int pg = pbeg + 4 * j + w4;
+      return pg < pend ? page_of(p.t, rw.slot, pg) : -1;
+    };
+    int id_next = id_of(0), id_after = id_of(1);
+    auto fetch = [&](int id) {                           // (a page that is not there: any other, for nothing)
+      const uint8_t* rec = p.data + ((size_t)max(id, 0) * p.Hkv + kvh) * Gm::kRecord;
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i) {
+        ck_next[i] = __ldg(reinterpret_cast<const uint4*>(rec) + lane + 32 * i);
+        cv_next[i] = __ldg(reinterpret_cast<const uint4*>(rec + Gm::kV) + lane + 32 * i);
+        load_words<2 * NW>(rec + Gm::kAmax + (lane + 32 * i) / (D / 32) * Gm::kAmaxTok, am_next[i]);
+      }
+    };
+    fetch(id_next);
+    int e_run = 14;
+    for (int j = 0; j < nblk; ++j) {
+      TileNote& note = notes[j & 3];
+      const bool have = id_next >= 0;
+      const int tok0 = (pbeg + 4 * j + w4) * kPage;
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i) {
+        ck[i] = ck_next[i]; cv[i] = cv_next[i];
+#pragma unroll
+        for (int n = 0; n < 2 * NW; ++n) am[i][n] = am_next[i][n];
+      }
+      if (!have || tok0 < rw.first_lo || tok0 + kPage > rw.len_hi) {       // a token that no row sees must not set a scale, nor be a NaN
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) {
+          const int at = tok0 + (lane + 32 * i) / (D / 32);
+          if (!have || at < rw.first_lo || at >= rw.len_hi)
+#pragma unroll
+            for (int n = 0; n < 2 * NW; ++n) am[i][n] = 0u;
+        }
+      }
+      id_next = id_after;
+      fetch(id_next);
+      id_after = id_of(j + 2);
+      uint32_t k2 = 0, v2 = 0;
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i)
+#pragma unroll
+        for (int n = 0; n < NW; ++n) { k2 = __vmaxu2(k2, am[i][n]); v2 = __vmaxu2(v2, am[i][NW + n]); }
+      int ek = (int)max(k2 & 0xffffu, k2 >> 16) >> 7, ev = (int)max(v2 & 0xffffu, v2 >> 16) >> 7;
+      const bool odd = __any_sync(0xffffffffu, max(ek, ev) >= 255);
+      bool bad = false;
+      if (odd) {                                         // the largest finite ones, and the V groups that are not
+        ek = ev = 0;
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) {
+          uint32_t groups = 0;
+#pragma unroll
+          for (int n = 0; n < NW; ++n) {
+            ek = max(ek, top_exponent(am[i][n]));
+            uint32_t& v = am[i][NW + n];
+            ev = max(ev, top_exponent(v));
+            if ((v & 0x7f80u) == 0x7f80u) { groups |= 1u << (2 * n); v &= 0xffff0000u; }
+            if ((v & 0x7f800000u) == 0x7f800000u) { groups |= 2u << (2 * n); v &= 0xffffu; }
+          }
+          const int x = lane + 32 * i;
+          bad = bad || groups;
+          if (x % (D / 32) == 0) note.groups[16 * w4 + x / (D / 32)] = (uint8_t)groups;
+        }
+        bad = __any_sync(0xffffffffu, bad);
+      }
+      ek = max(14, (int)__reduce_max_sync(0xffffffffu, (uint32_t)ek));
+      ev = max(14, (int)__reduce_max_sync(0xffffffffu, (uint32_t)ev));
+      if (lane == 0) {
+        note.kf[w4] = exp2_pos(ek - 140);
+        note.have[w4] = have; note.bad[w4] = bad;
+        v_top[j & 1][w4] = ev;
+      }
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+#pragma unroll
+      for (int w = 0; w < 4; ++w) e_run = max(e_run, v_top[j & 1][w]);
+      if (lane == 0 && w4 == 0) note.e = e_run;
+      auto store = [&](uint8_t* tile, const uint4 (&c)[kUnits], int first, int e) {
+        const float down = exp2_pos(140 - e);            // 2^13 / 2^(e - 127): a product with half a code stays below 2^16
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) {
+          const int x = lane + 32 * i, tok = 16 * w4 + x / (D / 32);
+          uint32_t a[NW];
+#pragma unroll
+          for (int n = 0; n < NW; ++n) a[n] = attn_mma::pack_f16x2(bf16lo_to_f(am[i][first + n]) * down, bf16hi_to_f(am[i][first + n]) * down);
+          const uint32_t c4[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int w = 4 * (x % (D / 32)) + k;
+            *reinterpret_cast<uint4*>(tile + (w >> 3) * kBox + tok * 128 + (((w & 7) ^ (tok & 7)) << 4)) = unpack_word(mg, c4[k], a[k % NW]);
+          }
+        }
+        smem_to_async();
+      };
+      if (j > 1 && !mbar_wait(&b_s[j & 1], (uint32_t)((j >> 1) - 1) & 1u, p.status, 0x4b563415u, limit)) limit = 16;
+      store(sK + (j & 1) * T::kK, ck, 0, ek);
+      mbar_arrive(&b_k[j & 1]);
+      if (j > 1 && !mbar_wait(&b_o[j & 1], (uint32_t)((j >> 1) - 1) & 1u, p.status, 0x4b563416u, limit)) limit = 16;
+      store(sV + (j & 1) * T::kK, cv, NW, e_run);
+      mbar_arrive(&b_v[j & 1]);
+    }
+  } else {
+    // ---- softmax: a pair a thread ----
+    constexpr float kLag = 1.f;
+    const bool live = tid < np;
+    const int row = rw.row0 + (live ? tid / p.G : 0), head = kvh * p.G + (live ? tid % p.G : 0);
+    const int hi = live ? row_len(p, row) : 0, lo = row_first(p, hi);
+    float f;
+    {
+      const unsigned short* src = reinterpret_cast<const unsigned short*>(p.q) + (size_t)row * p.ld_q + (size_t)head * D;
+      auto quad = [&](int i) -> uint2 {
+        if (!live) return make_uint2(0u, 0u);
+        if (p.vec) return __ldg(reinterpret_cast<const uint2*>(src) + i);
+        const unsigned short* at = src + 4 * i;
+        return make_uint2(at[0] | ((uint32_t)at[1] << 16), at[2] | ((uint32_t)at[3] << 16));
+      };
+      uint32_t mx = 0;
+#pragma unroll 8
+      for (int i = 0; i < D / 4; ++i) {
+        const uint2 v = quad(i);
+        const uint32_t mm = __vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu);
+        mx = max(mx, max(mm & 0xffffu, mm >> 16));
+      }
+      const float up = q_scale(p, mx, f);
+#pragma unroll 4
+      for (int w = 0; w < D / 8; ++w) {
+        const uint2 a = quad(2 * w), b = quad(2 * w + 1);
+        const uint4 v = make_uint4(attn_mma::pack_f16x2(bf16lo_to_f(a.x) * up, bf16lo_to_f(b.x) * up), attn_mma::pack_f16x2(bf16hi_to_f(a.x) * up, bf16hi_to_f(b.x) * up),
+                                   attn_mma::pack_f16x2(bf16lo_to_f(a.y) * up, bf16lo_to_f(b.y) * up), attn_mma::pack_f16x2(bf16hi_to_f(a.y) * up, bf16hi_to_f(b.y) * up));
+        *reinterpret_cast<uint4*>(sQ + (w >> 3) * (T::kRows * 128) + tid * 128 + (((w & 7) ^ (tid & 7)) << 4)) = v;
+      }
+      smem_to_async();
+      mbar_arrive(&b_q);
+    }
+    const uint32_t t_row = tmem + ((uint32_t)(warp * 32) << 16);
+    float m = -INFINITY, bar = -INFINITY, off = 14.f - kLag, l = 0.f;
+    int e_run = 14;
+    uint32_t poison = 0;                                 // V groups of a token that the row sees and that are not finite
+    const bool on = nblk > 0 && 32 * warp < np;
+    for (int j = 0; j < nblk && on; ++j) {
+      if (!mbar_wait(&b_s[j & 1], (uint32_t)(j >> 1) & 1u, p.status, 0x4b563417u, limit)) limit = 16;
+      __syncwarp();
+      tc_fence_after();
+      const TileNote& note = notes[j & 3];
+      const int tok0 = (pbeg + 4 * j) * kPage;
+      const uint32_t haves = *reinterpret_cast<const uint32_t*>(note.have), bads = *reinterpret_cast<const uint32_t*>(note.bad);
+      const float4 k4 = *reinterpret_cast<const float4*>(note.kf);
+      const float kf[4] = {fmaxf(f * k4.x, 1e-37f), fmaxf(f * k4.y, 1e-37f), fmaxf(f * k4.z, 1e-37f), fmaxf(f * k4.w, 1e-37f)};      // (0 * -inf)
+      const bool edge = haves != 0x01010101u || tok0 + T::kTok > rw.len_lo || tok0 < rw.first_hi;
+      const uint32_t ts = t_row + 64 * (j & 1);
+      const int e_new = note.e;
+      auto hide = [&](uint32_t (&r)[32], int half) {
+#pragma unroll
+        for (int pg = 0; pg < 2; ++pg) {
+          const int at = tok0 + 32 * half + 16 * pg, a = lo - at, b = (haves >> (8 * (2 * half + pg)) & 255u) ? hi - at : 0;
+#pragma unroll
+          for (int i = 0; i < 16; ++i)
+            if (i < a || i >= b) r[16 * pg + i] = 0xff800000u;
+        }
+      };
+      float mx = -INFINITY;
+      uint32_t r[32];
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        tmem_ld_32x32b_x32(ts + 32 * half, r);
+        tmem_ld_wait();
+        if (edge) hide(r, half);
+#pragma unroll
+        for (int pg = 0; pg < 2; ++pg) {
+          float a = __uint_as_float(r[16 * pg]), b = __uint_as_float(r[16 * pg + 1]);
+#pragma unroll
+          for (int i = 2; i < 16; i += 2) { a = fmaxf(a, __uint_as_float(r[16 * pg + i])); b = fmaxf(b, __uint_as_float(r[16 * pg + i + 1])); }
+          mx = fmaxf(mx, fmaxf(a, b) * kf[2 * half + pg]);
+        }
+      }
+      float alpha = 1.f;
+      if (mx > bar) {
+        alpha = m == -INFINITY ? 0.f : exp2_fast(m - mx);
+        m = mx;
+        bar = mx + kLag;
+        off = 14.f - kLag - mx;
+        l *= alpha;
+      }
+      if (e_new != e_run) {                              // the values' power of two has moved: the sums follow, P does not
+        alpha *= e_new - e_run < 127 ? exp2_pos(e_run - e_new) : 0.f;
+        e_run = e_new;
+      }
+      if (bads)
+        for (int i = 0; i < T::kTok; ++i) poison |= (note.bad[i >> 4] && tok0 + i >= lo && tok0 + i < hi) ? note.groups[i] : 0u;
+      if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {       // O(j - 1) has to be there
+        if (!mbar_wait(&b_o[(j - 1) & 1], (uint32_t)((j - 1) >> 1) & 1u, p.status, 0x4b563418u, limit)) limit = 16;
+        __syncwarp();
+        tc_fence_after();
+#pragma unroll 1
+        for (int c = 0; c < D / 32; ++c) {
+          tmem_ld_32x32b_x32(t_row + 128 + 32 * c, r);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
+          tmem_st_x32(t_row + 128 + 32 * c, r);
+        }
+      }
+      float sum[2] = {0.f, 0.f};
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        tmem_ld_32x32b_x32(ts + 32 * half, r);
+        tmem_ld_wait();
+        if (edge) hide(r, half);
+        uint32_t o[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const float k = kf[2 * half + (i >> 3)];
+          const float x = exp2_fast(fmaf(__uint_as_float(r[2 * i]), k, off)), y = exp2_fast(fmaf(__uint_as_float(r[2 * i + 1]), k, off));
+          sum[0] += x; sum[1] += y;
+          o[i] = attn_mma::pack_f16x2(x, y);
+        }
+        tmem_st_x16(ts + 16 * half, o);
+      }
+      l += sum[0] + sum[1];
+      tmem_st_done();
+      tc_fence_before();
+      mbar_arrive(&b_p);
+    }
+    if (on) {
+      mbar_wait(&b_o[(nblk - 1) & 1], (uint32_t)((nblk - 1) >> 1) & 1u, p.status, 0x4b563419u, limit);
+      tc_fence_after();
+    }
+    // (a CTA without pages has nothing in TMEM: its sums are zero)
+    const float ls = l * (1.f / 8192.f), fo = exp2_pos(e_run - 140);
+    const size_t pi = ((size_t)(u * p.uheads + kvh) * p.splits + blockIdx.x) * T::kRows + tid;
+    if (32 * warp < np) {
+#pragma unroll 1
+      for (int c = 0; c < D / 32; ++c) {
+        uint32_t r[32];
+        __syncwarp();
+        if (on) {
+          tmem_ld_32x32b_x32(t_row + 128 + 32 * c, r);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) r[i] = 0u;
+        }
+        if (live && (on || p.splits == 1)) {
+#pragma unroll
+          for (int w = 0; w < 4; ++w) {
+            float o[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const int g = (8 * c + 2 * w + (i & 1)) % NG;           // the group of dims i >> 1 (+ 4)
+              o[(i >> 1) + 4 * (i & 1)] = (poison >> g & 1u) ? __uint_as_float(0x7fc00000u) : __uint_as_float(r[8 * w + i]) * (2.f / 7.f / 8192.f) * fo;
+            }
+            const int d = 32 * c + 8 * w;
+            if (p.splits == 1) {
+#pragma unroll
+              for (int i = 0; i < 8; i += 2) finish(p, row, head, d + i, D, o[i], o[i + 1], m, ls);
+            } else {
+              float4* dst = reinterpret_cast<float4*>(p.part_o + pi * D + d);
+              dst[0] = make_float4(o[0], o[1], o[2], o[3]);
+              dst[1] = make_float4(o[4], o[5], o[6], o[7]);
+            }
+          }
+        }
+      }
+      if (live && p.splits != 1) { p.part_ml[2 * pi] = m; p.part_ml[2 * pi + 1] = ls; }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 0) tmem_dealloc(tmem, T::kCols);
+}
+
 // Joins the parts of a unit: one CTA per (query head, row).  Groups of D / 2 threads (two dims each) take every n-th part and are
 // joined in order: the result does not depend on timing.  Bound by the latency of its dependent loads: the parts' statistics are
 // read once, and a group keeps eight parts in flight.
@@ -937,6 +1390,7 @@ __global__ void __launch_bounds__(kThreads) mass_kernel(const AttnParams p, int 
 // How a call is cut into CTAs, and what it needs as scratch.
 struct Plan {
   int heads, subs, rows, groups, units, uheads, pairs, splits, ctas, sms;
+  bool tile;                // 128 pairs a CTA
   long slots;               // parts that are stored
   long floats(long M, long Hq, long D, long observe) const {
     return (splits == 1 ? 0 : slots * pairs * (D + 2)) + (splits == 0 ? 2L * (units + 2) : 0) + (observe ? 2 * M * Hq : 0);
@@ -959,19 +1413,26 @@ int plan(Plan& pl, long M, long Hq, long Hkv, long D, long block, long max_len, 
   if (!sms) return -2;
   // (row, head) pairs of a CTA: one MMA column tile holds 8.  Two tiles where more pairs than that share the keys, except at
   // head_dim 256, whose accumulators fill the registers with one.
-  const int most = D == 256 ? 8 : 16;
+  // Tiles of 128 pairs pay where a block has many and the keys are long enough to carry the wider kernel's start (10 us).  Measured,
+  // us without / with tiles, observed weight included: 160 pairs, 4 x 16384 tokens x 8 kv heads 375 / 269; 512 pairs at head_dim 64,
+  // 2 x 8192 x 4 138 / 109; 96 pairs at head_dim 256, 2 x 8192 x 4 152 / 123; 40 pairs, 4 x 8192 x 8 109 / 106; but 20 pairs of
+  // those 94 / 102, 40 pairs, 8192 x 8 56 / 61, 80 pairs, 2001 x 8 44 / 50.
+  const long key_pages = (max_len + kPage - 1) / kPage;
+  pl.tile = block * G >= 40 && M * Hq * key_pages >= 256L * 1024;
+  const int most = pl.tile ? 128 : (D == 256 ? 8 : 16);
   pl.heads = G < most ? G : most;
   pl.subs = (G + pl.heads - 1) / pl.heads;
   pl.rows = pl.subs > 1 ? 1 : most / G;
   if (pl.rows > block) pl.rows = (int)block;
   pl.groups = (int)((block + pl.rows - 1) / pl.rows);
-  pl.pairs = pl.rows * pl.heads <= 8 ? 8 : 16;
+  if (pl.tile) pl.rows = (int)((block + pl.groups - 1) / pl.groups);       // tiles of like size
+  pl.pairs = pl.tile ? 128 : (pl.rows * pl.heads <= 8 ? 8 : 16);
   const long units = M / block * pl.groups;
   if (units > 65535 || Hkv * pl.subs > 65535) return -2;
   pl.units = (int)units;
   pl.uheads = (int)Hkv * pl.subs;
   pl.sms = sms;
-  pl.ctas = sms * (D == 256 ? Ring<256>::kCtas : Ring<128>::kCtas);
+  pl.ctas = sms * (pl.tile ? (D == 256 ? Tile<256>::kCtas : Tile<128>::kCtas) : (D == 256 ? Ring<256>::kCtas : Ring<128>::kCtas));
   // alone: the keys of a block are cut as in a call of that block only, so that its rows get the same bits in both
   const long cells = (alone ? pl.groups : units) * pl.uheads, pages = (max_len + kPage - 1) / kPage;
   // Streamed: every CTA gets the same number of pages of the flat list, whatever the rows' lengths, at the price of a scan over
@@ -980,7 +1441,7 @@ int plan(Plan& pl, long M, long Hq, long Hkv, long D, long block, long max_len, 
   // up to 8191 at head_dim 256 (110 pages) 51.0 / 54.1, one row of 131072 (147 pages) 47.9 / 52.7, 32 rows of up to 32768 (900
   // pages) 320 / 231.
   pl.splits = 0;
-  if (alone || units > kMaxUnits || cells * pages < 256L * pl.ctas) {
+  if (pl.tile || alone || units > kMaxUnits || cells * pages < 256L * pl.ctas) {
     long s = pages / 8 < pl.ctas / cells ? pages / 8 : pl.ctas / cells;
     pl.splits = (int)(s < 1 ? 1 : s);
   }
@@ -1009,9 +1470,18 @@ int launch_attn(const AttnParams& p, cudaStream_t st) {
 }
 
 template <int D>
+int launch_tile(const AttnParams& p, cudaStream_t st) {
+  static unsigned long long ready = 0;
+  const cudaError_t e = allow_smem(ready, (const void*)tile_kernel<D>, Tile<D>::kBytes);
+  if (e != cudaSuccess) return (int)e;
+  return (int)grm_launch_pdl(GRM_PDL_ATTN, tile_kernel<D>, dim3(p.splits, p.uheads, p.units), dim3(Tile<D>::kThreads), Tile<D>::kBytes, st, p);
+}
+
+template <int D>
 int launch(const AttnParams& p, int nblocks, int mass_pages, cudaStream_t st) {
   int rc;
-  if constexpr (D == 256) rc = launch_attn<D, 1>(p, st);
+  if (p.pairs == 128) rc = launch_tile<D>(p, st);
+  else if constexpr (D == 256) rc = launch_attn<D, 1>(p, st);
   else rc = p.pairs == 8 ? launch_attn<D, 1>(p, st) : launch_attn<D, 2>(p, st);
   if (rc) return rc;
   if (p.splits != 1) {
@@ -1051,7 +1521,7 @@ GRM_API long grm_kv4_attn_scratch(int M, int Hq, int Hkv, int D, int block, int 
 
 // One record of 64-bit words (kv4::Args):
 //   data, mass (or 0), table, slots, width, stride, pages, q, ld_q, row_seq, row_pos, gate (or 0), ld_gate, out, ld_o, scratch
-//   (8-byte aligned, or 0: the call returns -3 where it needs some), M, Hq, Hkv, D, window, scale, block, observe (0 nothing, 1 set, 2 add), max_len,
+//   (16-byte aligned, or 0: the call returns -3 where it needs some), M, Hq, Hkv, D, window, scale, block, observe (0 nothing, 1 set, 2 add), max_len,
 //   alone
 // max_len bounds the positions of the call's rows for the observed weight and sets how the keys are cut.
 GRM_API int grm_kv4_attn(const void* words, void* stream) {

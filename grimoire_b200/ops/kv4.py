@@ -219,7 +219,8 @@ def kv4_attn(q: torch.Tensor, row_seq: torch.Tensor, row_pos: torch.Tensor, bloc
     """Attention of M rows over the 4-bit pages: row m (bf16 [Hq * D], after norm and RoPE) of sequence slot ``row_seq[m]`` sees
     the cached positions 0 .. ``row_pos[m]``, the last ``geom.window`` of them with a window, and leaves its output (bf16,
     times sigmoid(``gate[m]``) with a gate) in ``out[m]`` (which must not overlap ``q``).  A row that sees no key (a negative position, no mapped page)
-    gives zeros.  ``max_len`` is the longest row's ``row_pos + 1`` as the host knows it: it sets how the keys are split, and
+    gives zeros.  Within a block, values below 2^-24 of the largest one that any of its rows sees are rounded to fewer bits (2^-36 of
+    that one at worst).  ``max_len`` is the longest row's ``row_pos + 1`` as the host knows it: it sets how the keys are split, and
     bounds the tokens that ``observe`` covers.
 
     ``block`` > 1: every ``block`` consecutive rows belong to one sequence (the last rows of a prompt, a verify block).

@@ -849,3 +849,134 @@ def test_a_captured_cut_of_two_conversations_side_by_side():
     for w, r in zip(wants, got):
         for a, b in zip(w, r):
             assert torch.equal(a.view(torch.uint8) if a.is_floating_point() else a, b.view(torch.uint8) if b.is_floating_point() else b)
+
+
+# ---------------------------------------------------------------------------------------------
+# blocks of many rows over keys that the caller announces as long: 128 pairs a tile
+# ---------------------------------------------------------------------------------------------
+LONG = 1 << 20
+
+
+def attend_long(c, seqs, pos, q, G, scale, window=0, gate=None, table=None, **kw):
+    geom = AttnGeom(c.Hkv * G, c.Hkv, c.D, c.D, scale, window=window)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=c.device)
+    out = torch.full((len(seqs), c.Hkv * G * c.D), 9.0, dtype=torch.bfloat16, device=c.device)
+    kv4.kv4_attn(q.to(c.device), i32([int(c.slots[s]) for s in seqs]), i32(list(pos)), c.table if table is None else table, c.kv, geom, out, LONG,
+                 gate=None if gate is None else gate.to(c.device), **kw)
+    return out.cpu()
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("D,G,block,window", [(64, 16, 9, 0), (64, 1, 40, 33), (128, 5, 32, 0), (128, 16, 5, 70), (256, 12, 4, 0), (256, 3, 20, 0),
+                                              (256, 16, 3, 25), (128, 1, 150, 0), (64, 7, 19, 64), (128, 3, 43, 1)])
+def test_tiles_of_many_rows(device, D, G, block, window):
+    lens, Hkv = [300, 165, 1700], 2
+    c = Cache(lens, Hkv, D, device, seed=D + G)
+    seqs = [s for s in range(3) for _ in range(block)]
+    pos = [lens[s] - block + r for s in range(3) for r in range(block)]
+    pos[0] = -1
+    q = torch.randn(len(seqs), Hkv * G * D + 3, generator=torch.Generator().manual_seed(G)).bfloat16()[:, : Hkv * G * D]
+    gate = torch.randn(len(seqs), Hkv * G * D, generator=torch.Generator().manual_seed(G + 1)).bfloat16()
+    scale = -1 / math.sqrt(D) if window else 1 / math.sqrt(D)
+    ref, size, weights, top = c.expect(seqs, pos, q, G, scale, window)
+    scores_in_range(D, c.expect(seqs, pos, q, G, abs(scale), window)[3])
+    sg = torch.sigmoid(gate.double())
+    for kw in (dict(), dict(observe="set"), dict(observe="add", alone=True)):
+        close(attend_long(c, seqs, pos, q, G, scale, window, gate=gate, block=block, **kw), ref * sg, size * sg)
+    for s in range(3):
+        want = sum(torch.nn.functional.pad(weights[m], (0, lens[s] - weights[m].shape[1])) for m in range(len(seqs)) if seqs[m] == s)
+        err = (c.mass_of(s).double() - 2 * want).abs()
+        assert float((err - 2 ** -8 * 2 * want).max()) < 2 ** -16 * block * G
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_tiles_keep_nan_and_unmapped_pages_from_rows_and_channels(device, D):
+    """Tokens with a NaN or infinite group in V reach only the rows that see them, and only that group's channels; a NaN in K only
+    the rows that see it; pages that are not mapped hold nothing."""
+    n, Hkv, G, block = 230, 1, 5, 40
+    c = Cache([n], Hkv, D, device, seed=90)
+    slot = int(c.slots[0])
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=device)
+    rows = torch.cat([c.kx[0][200:201], c.kx[0][215:216], c.kx[0][225:226]]), torch.cat([c.vx[0][200:201], c.vx[0][215:216], c.vx[0][225:226]])
+    rows[1][0, 3] = float("nan")                                                       # token 200: quad 0, group 0
+    rows[1][1, 4 * (D // 32 - 1)] = float("inf")                                       # token 215: the last group
+    rows[0][2, 9] = float("nan")                                                       # token 225: K
+    kv4.kv4_append(c.kv, rows[0].to(device), rows[1].to(device), i32(200, 215, 225), i32(slot, slot, slot), c.table)
+    hole = c.table.clone()
+    hole[slot, 5] = -1
+    hole[slot, 6] = 2 ** 30
+    q = torch.randn(block, G * D, generator=torch.Generator().manual_seed(3)).bfloat16()
+    pos = list(range(190, 230))
+    scale = 1 / math.sqrt(D)
+    got = attend_long(c, [0] * block, pos, q, G, scale, block=block, table=hole).reshape(block, G, D)
+    group = (torch.arange(D) // 4) % (D // 32)
+    keep = torch.tensor([t for t in range(n) if not 80 <= t < 112])
+    for m, p in enumerate(pos):
+        bad = torch.zeros(D, dtype=torch.bool)
+        if p >= 200:
+            bad |= group == 0
+        if p >= 215:
+            bad |= group == D // 32 - 1
+        if p >= 225:
+            bad[:] = True
+        assert bool(torch.isnan(got[m][:, bad]).all()) and not bool(torch.isnan(got[m][:, ~bad]).any())
+        at = keep[keep <= p]
+        if not bool(bad.all()):
+            v = c.v[0][at, 0].clone()
+            v[:, bad] = 0
+            o, size, _, top = attend64(q[m].reshape(G, D), c.k[0][at, 0], v, len(at) - 1, scale, 0)
+            scores_in_range(D, top)
+            close(got[m][:, ~bad], o[:, ~bad], size[:, ~bad])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("amp", [2.0 ** -60, 1e-4, 300.0, 2.0 ** 50])
+def test_tiles_over_small_and_large_values(device, amp):
+    D, Hkv, G, block = 128, 2, 4, 24
+    c = Cache([333, 90], Hkv, D, device, seed=91, amp=amp)
+    seqs, pos = [0] * block + [1] * block, list(range(333 - block, 333)) + list(range(90 - block, 90))
+    q = torch.randn(2 * block, Hkv * G * D, generator=torch.Generator().manual_seed(8)).bfloat16()
+    scale = 1 / (amp * math.sqrt(D))
+    ref, size, _, top = c.expect(seqs, pos, q, G, scale)
+    scores_in_range(D, top)
+    close(attend_long(c, seqs, pos, q, G, scale, block=block), ref, size)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("far", [2.0 ** 24, 2.0 ** 100])
+def test_tiles_with_tokens_of_far_larger_values(device, far):
+    """The last token holds values ``far`` times the others', which its own row alone sees: the other rows must not lose theirs
+    while those are within 2^-24 of the largest.  Beyond that a value is rounded where the operand's fp16 ends: the largest maximum
+    stands at 2^13 or above and subnormals are 2^-24 apart, so half a code times a maximum is off by 2^-25 at most, 2^-38 of the
+    largest maximum, a value by twice that; the softmax (at 2^13, weights of 2^-38 lost) adds as much: 2^-36 of the largest value."""
+    D, Hkv, G, n, block = 128, 1, 5, 200, 24
+    c = Cache([n], Hkv, D, device, seed=92)
+    big = (far * torch.randn(1, D, generator=torch.Generator().manual_seed(1))).bfloat16()
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=device)
+    kv4.kv4_append(c.kv, c.kx[0][n - 1:].to(device), big.to(device), i32(n - 1), i32(int(c.slots[0])), c.table)
+    c.v[0][n - 1] = quantised(big.reshape(Hkv, D))
+    q = torch.randn(block, G * D, generator=torch.Generator().manual_seed(2)).bfloat16()
+    pos = list(range(n - block, n))
+    ref, size, _, top = c.expect([0] * block, pos, q, G, 0.1)
+    scores_in_range(D, top)
+    got = attend_long(c, [0] * block, pos, q, G, 0.1, block=block)
+    if far <= 2.0 ** 24:
+        close(got, ref, size)
+    else:
+        size = size + 2 ** 9 * 2 ** -36 * float(big.abs().max())                       # close() allows 2^-9 of it
+        close(got[-1:], ref[-1:], size[-1:])
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_tiles_of_more_units_than_the_gpu_holds(device):
+    """No cut of the keys: the rows are finished where they are computed; sequences of one block up to several."""
+    D, Hkv, G, block, S = 64, 8, 4, 11, 40
+    lens = [11 + 7 * i for i in range(S)]
+    c = Cache(lens, Hkv, D, device, seed=93)
+    seqs = [s for s in range(S) for _ in range(block)]
+    pos = [lens[s] - block + r for s in range(S) for r in range(block)]
+    q = torch.randn(len(seqs), Hkv * G * D, generator=torch.Generator().manual_seed(4)).bfloat16()
+    ref, size, _, top = c.expect(seqs, pos, q, G, 0.125)
+    scores_in_range(D, top)
+    close(attend_long(c, seqs, pos, q, G, 0.125, block=block), ref, size)
