@@ -184,7 +184,7 @@ __device__ __forceinline__ uint32_t order_key(float f) {
 }
 
 constexpr int kSelThreads = 1024, kSelBins = 2048;
-constexpr int kSelKeys = 16384;          // keys that a CTA keeps in shared memory
+constexpr int kSelKeys = 32768;          // keys that a CTA keeps in shared memory
 
 __device__ __forceinline__ void cluster_sync_() {
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -458,18 +458,20 @@ GRM_API int grm_kv4_select(const void* words, void* stream) {
   if (!fits(S, 1, 65535) || !fits(Hkv, 1, 0x7fffffff) || !fits(keep, 1, 0x7fffffff) || !fits(recent, 0, keep) || !fits(sink, 0, keep - recent)) return -2;
   p.Hkv = (int)Hkv; p.keep = (int)keep; p.recent = (int)recent; p.sink = (int)sink;
   // CTAs a (kv head, sequence): a stretch of up to 4096 tokens is quickest in one (no sums across CTAs); longer ones are shared by up
-  // to eight, as many as leave every CTA a place on the GPU at once
-  int dev = 0, sms = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  if (e != cudaSuccess) return (int)e;
+  // to eight, as many as run at once with a CTA an SM (its registers allow no more), or as it takes to keep the keys.  Measured, us
+  // with one CTA to two an SM / as it is: 4 sequences of 16384 tokens x 8 kv heads 81 / 18, 8 of 8192 33 / 14; with 16384 keys a
+  // CTA / 32768: 8 of 32768 43 / 27
+  const int sms = sm_count();
+  if (!sms) return -2;
   int n = 1;
-  while (n < 8 && (long)p.t.width * kPage > 4096L * n && (S * Hkv * n < sms || (long)p.t.width * kPage > (long)kSelKeys * n)) n *= 2;
+  while (n < 8 && (long)p.t.width * kPage > 4096L * n && (S * Hkv * 2 * n <= sms || (long)p.t.width * kPage > (long)kSelKeys * n)) n *= 2;
   if (Hkv * n > 0x7fffffffL) return -2;
-  e = cudaFuncSetAttribute(select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelKeys * 4);
+  static unsigned long long ready = 0;
+  const cudaError_t e = allow_smem(ready, (const void*)select_kernel, kSelKeys * 4);
   if (e != cudaSuccess) return (int)e;
+  const long most = (p.t.width + n - 1L) / n * kPage;           // tokens of a CTA
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(Hkv * n), (unsigned)S); cfg.blockDim = dim3(kSelThreads); cfg.dynamicSmemBytes = kSelKeys * 4; cfg.stream = (cudaStream_t)stream;
+  cfg.gridDim = dim3((unsigned)(Hkv * n), (unsigned)S); cfg.blockDim = dim3(kSelThreads); cfg.dynamicSmemBytes = 4 * (size_t)(most < kSelKeys ? most : kSelKeys); cfg.stream = (cudaStream_t)stream;
   cudaLaunchAttribute at[2];
   at[0].id = cudaLaunchAttributeClusterDimension;
   at[0].val.clusterDim.x = (unsigned)n; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;

@@ -66,4 +66,23 @@ inline bool read_table(Args& a, Table& t) {
   return true;
 }
 
+// The multiprocessors of the current device (0 where that fails).
+inline int sm_count() {
+  static int known[64] = {0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  if (!known[dev] && cudaDeviceGetAttribute(&known[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
+  return known[dev];
+}
+
+// Opts a kernel in to its dynamic shared memory, once per device (bit of ``ready``; setting it twice does no harm).
+inline cudaError_t allow_smem(unsigned long long& ready, const void* kernel, int bytes) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (ready >> (dev & 63) & 1)) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) ready |= 1ull << (dev & 63);
+  return e;
+}
+
 }  // namespace kv4

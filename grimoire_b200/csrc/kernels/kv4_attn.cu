@@ -1397,15 +1397,6 @@ struct Plan {
   }
 };
 
-// The multiprocessors of the current device (0 where that fails).
-int sm_count() {
-  static int known[64] = {0};
-  int dev = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
-  if (!known[dev] && cudaDeviceGetAttribute(&known[dev], cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 0;
-  return known[dev];
-}
-
 int plan(Plan& pl, long M, long Hq, long Hkv, long D, long block, long max_len, long alone) {
   if (!fits(M, 1, 65535) || !fits(Hkv, 1, 65535) || !fits(Hq, 1, 16 * Hkv) || Hq % Hkv || !fits(block, 1, M) || M % block || !fits(max_len, 1, 0x7fffffff)) return -2;
   if (D != 64 && D != 128 && D != 256) return -2;
@@ -1447,16 +1438,6 @@ int plan(Plan& pl, long M, long Hq, long Hkv, long D, long block, long max_len, 
   }
   pl.slots = pl.splits == 0 ? pl.ctas + cells : units * pl.uheads * pl.splits;
   return 0;
-}
-
-// Opts a kernel in to its dynamic shared memory, once per device (bit of ``ready``; setting it twice does no harm).
-cudaError_t allow_smem(unsigned long long& ready, const void* kernel, int bytes) {
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess || (ready >> (dev & 63) & 1)) return e;
-  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-  if (e == cudaSuccess) ready |= 1ull << (dev & 63);
-  return e;
 }
 
 template <int D, int HH>

@@ -980,3 +980,19 @@ def test_tiles_of_more_units_than_the_gpu_holds(device):
     ref, size, _, top = c.expect(seqs, pos, q, G, 0.125)
     scores_in_range(D, top)
     close(attend_long(c, seqs, pos, q, G, 0.125, block=block), ref, size)
+
+
+@pytest.mark.gpu
+def test_selection_of_a_sequence_whose_keys_no_cluster_holds():
+    n, keep = 300001, 5000
+    pages = (n + PAGE - 1) // PAGE
+    kv = kv4.Kv4Layer.alloc(pages, 1, 64, "cuda", mass=True)
+    mass = torch.exp(3 * torch.randn(pages, 1, PAGE, generator=torch.Generator().manual_seed(9)))
+    mass[::3] = 0
+    kv.mass.copy_(mass)
+    table = torch.randperm(pages, generator=torch.Generator().manual_seed(10)).to(torch.int32)[None]
+    got = kv4.kv4_select(kv, None, torch.tensor([n], dtype=torch.int32, device="cuda"), table.cuda(), keep, 100, 4)[0, 0].cpu().long()
+    m = mass[table[0].long()].reshape(-1)[:n]
+    rest = torch.sort(m[4: n - 100], descending=True, stable=True).indices[: keep - 104] + 4
+    want = torch.cat([torch.arange(4), rest.sort().values, torch.arange(n - 100, n)])
+    assert torch.equal(got, want)
