@@ -295,7 +295,7 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectParams 
   }
   if (cached) __syncthreads();                           // (no pass has run where nothing is wanted)
   // prefix: the key of the last kept token; need: how many tokens with that key stay
-  auto judge = [&](int t, bool& gt, bool& eq) {
+  auto rank_of = [&](int t, bool& gt, bool& eq) {
     const bool cand = t >= lo && t < hi;
     const uint32_t k = (cand && want > 0) ? key(t) : 0u;
     gt = !cand || (want > 0 && k > prefix);
@@ -305,7 +305,7 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectParams 
   int n_gt = 0, n_eq = 0;
   for (int t = wbeg + lane; t < wend; t += 32) {
     bool gt, eq;
-    judge(t, gt, eq);
+    rank_of(t, gt, eq);
     n_gt += gt; n_eq += eq;
   }
   n_gt = __reduce_add_sync(0xffffffffu, n_gt);
@@ -324,7 +324,7 @@ __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectParams 
   for (int t0 = wbeg; t0 < wend; t0 += 32) {
     const int t = t0 + lane;
     bool gt = false, eq = false;
-    if (t < wend) judge(t, gt, eq);
+    if (t < wend) rank_of(t, gt, eq);
     const uint32_t gts = __ballot_sync(0xffffffffu, gt), eqs = __ballot_sync(0xffffffffu, eq), under = (1u << lane) - 1u;
     const int eq_here = eq_before + __popc(eqs & under);
     const int to = gt_before + __popc(gts & under) + min(eq_here, need);
