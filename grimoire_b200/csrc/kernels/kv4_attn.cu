@@ -694,7 +694,9 @@ __global__ void __launch_bounds__(kThreads, Ring<D>::kCtas) attn_kernel(const At
 //   * One thread issues S = Q K^T (64 columns of TMEM, two buffers) and O += P V (V as it lies, tokens by dims: the MN-major
 //     operand), so that S of the next tokens runs under the softmax of these.
 //   * Four warps do the softmax, a pair a thread: no shuffles, the reference follows the maximum when that is 2^kLag ahead.  P, rounded
-//     to fp16 (11 bits, against the output's 8), takes the place of S in TMEM.
+//     to fp16 (11 bits, against the output's 8), takes the place of S in TMEM.  S(j + 1) is on its way before P(j) is complete, so a
+//     warp may be a block ahead of a slower one: P has a barrier for even and one for odd blocks, and an arrival for P(j + 1) never
+//     counts for P(j).  Two blocks ahead it cannot be: S(j + 2) is issued after P V(j), which waits for every warp's P(j).
 // A V group that is not finite would reach rows that do not see it as 0 * NaN: it is unpacked as zero, and the rows that see its
 // token remember the group.  Scores, statistics and outputs are fp32.
 //
@@ -795,7 +797,7 @@ __global__ void __launch_bounds__(Tile<D>::kThreads, Tile<D>::kCtas) tile_kernel
   constexpr int kUnits = D / 64;                         // 16-byte units of K (or V) codes a lane and page
   constexpr int kBox = T::kTok * 128;                    // bytes of 64 dims of the tokens
   extern __shared__ uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t b_q, b_p, b_k[2], b_v[2], b_s[2], b_o[2];
+  __shared__ __align__(8) uint64_t b_q, b_p[2], b_k[2], b_v[2], b_s[2], b_o[2];
   __shared__ TileNote notes[4];                          // of blocks j mod 4
   __shared__ int v_top[2][4];
   __shared__ uint32_t tmem_holder;
@@ -811,8 +813,8 @@ __global__ void __launch_bounds__(Tile<D>::kThreads, Tile<D>::kCtas) tile_kernel
   const int n0 = min((int)blockIdx.x * per, rw.pages), n1 = min(n0 + per, rw.pages);
   const int pbeg = rw.page_lo + n0, pend = rw.page_lo + n1, nblk = (n1 - n0 + 3) / 4;
   if (tid == 0) {
-    mbar_init(&b_q, 128); mbar_init(&b_p, 32 * ((np + 31) / 32));
-    for (int i = 0; i < 2; ++i) { mbar_init(&b_k[i], 128); mbar_init(&b_v[i], 128); mbar_init(&b_s[i], 1); mbar_init(&b_o[i], 1); }
+    mbar_init(&b_q, 128);
+    for (int i = 0; i < 2; ++i) { mbar_init(&b_p[i], 32 * ((np + 31) / 32)); mbar_init(&b_k[i], 128); mbar_init(&b_v[i], 128); mbar_init(&b_s[i], 1); mbar_init(&b_o[i], 1); }
     mbar_fence_init();
   }
   if (warp == 0) {
@@ -844,7 +846,7 @@ __global__ void __launch_bounds__(Tile<D>::kThreads, Tile<D>::kCtas) tile_kernel
           if (!good) break;
           issue_s(j + 1);
         }
-        good = mbar_wait(&b_p, (uint32_t)j & 1u, p.status, 0x4b563413u) && mbar_wait(&b_v[j & 1], (uint32_t)(j >> 1) & 1u, p.status, 0x4b563414u);
+        good = mbar_wait(&b_p[j & 1], (uint32_t)(j >> 1) & 1u, p.status, 0x4b563413u) && mbar_wait(&b_v[j & 1], (uint32_t)(j >> 1) & 1u, p.status, 0x4b563414u);
         if (!good) break;
         tc_fence_after();
 #pragma unroll
@@ -1083,7 +1085,7 @@ __global__ void __launch_bounds__(Tile<D>::kThreads, Tile<D>::kCtas) tile_kernel
       l += sum[0] + sum[1];
       tmem_st_done();
       tc_fence_before();
-      mbar_arrive(&b_p);
+      mbar_arrive(&b_p[j & 1]);
     }
     if (on) {
       mbar_wait(&b_o[(nblk - 1) & 1], (uint32_t)((nblk - 1) >> 1) & 1u, p.status, 0x4b563419u, limit);

@@ -1,0 +1,100 @@
+"""Blocks of many rows over long 4-bit caches: tiles of 128 (row, head) pairs whose CTAs walk through 30 and more blocks of 64
+tokens, against the definition in 64 bits and against themselves."""
+import math
+
+import pytest
+import torch
+
+from grimoire_b200.ops import kv4, ref
+from grimoire_b200.ops.core import AttnGeom
+
+from .test_kv4_ops import close, scores_in_range
+
+PAGE = 16
+
+
+class LongCache:
+    """Sequences of ``lens`` tokens, each on pages of its own, filled on the device.  Keys carry a component along a fixed pattern of
+    signs that grows from 0 to 3 over the sequence: rows with a share of it in their query see maxima that rise to the end."""
+
+    def __init__(self, lens, Hkv, D, seed):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        per = [(n + PAGE - 1) // PAGE for n in lens]
+        order = torch.randperm(sum(per), generator=g, device="cuda").to(torch.int32)
+        self.table = torch.full((len(lens), max(per)), -1, dtype=torch.int32, device="cuda")
+        at = 0
+        for s, n in enumerate(per):
+            self.table[s, :n] = order[at: at + n]
+            at += n
+        self.lens, self.Hkv, self.D = lens, Hkv, D
+        self.sign = torch.randint(0, 2, (D,), generator=g, device="cuda").float() * 2 - 1
+        self.kv = kv4.Kv4Layer.alloc(sum(per), Hkv, D, "cuda", mass=True)
+        for s, n in enumerate(lens):
+            pos = torch.arange(n, dtype=torch.int32, device="cuda")
+            k, v = (torch.randn(n, Hkv, D, generator=g, device="cuda") for _ in range(2))
+            k += (3 * pos / n)[:, None, None] * self.sign
+            kv4.kv4_append(self.kv, k.bfloat16().flatten(1), v.bfloat16().flatten(1), pos, torch.full_like(pos, s), self.table)
+
+    def values(self, s):
+        """K, V of sequence ``s`` in 64 bits: [Hkv][n][D]."""
+        codes, amax = ref.kv4_views(self.kv.data[self.table[s, : (self.lens[s] + PAGE - 1) // PAGE].long()])
+        q = torch.stack((codes & 15, codes >> 4), dim=-1).flatten(-2).double() - 8                       # [pages][Hkv][K, V][16][D]
+        x = (q.unflatten(-1, (8, self.D // 32, 4)) * amax.transpose(2, 3).double()[..., None, :, None] / 7).flatten(-3)
+        return (x[:, :, i].transpose(0, 1).flatten(1, 2)[:, : self.lens[s]] for i in (0, 1))
+
+    def mass_of(self, s):
+        t = torch.arange(self.lens[s], device="cuda")
+        return self.kv.mass[self.table[s, t // PAGE].long(), :, t % PAGE].t()
+
+
+def deep_case(D, G, block, seqs, seed):
+    """(cache, query rows [seqs * block][Hkv * G * D], positions) with late maxima for every other 32 pairs of a block."""
+    Hkv = 4
+    c = LongCache([2000 - 2 * (s % 37) for s in range(seqs)], Hkv, D, seed)
+    g = torch.Generator(device="cuda").manual_seed(seed + 1)
+    pair = torch.arange(block * G, device="cuda").reshape(block, 1, G, 1)
+    late = (pair // 32 % 2 == 1).float() * (20 / (3 * math.sqrt(D)))             # scores that rise by 20 (29 binades)
+    q = torch.randn(seqs, block, Hkv, G, D, generator=g, device="cuda") + late * c.sign
+    pos = torch.tensor([n - block + r for n in c.lens for r in range(block)], dtype=torch.int32, device="cuda")
+    return c, q.bfloat16().reshape(seqs * block, -1), pos
+
+
+def against_definition(c, q, pos, out, G, block, scale):
+    D, Hkv = c.D, c.Hkv
+    for s, n in enumerate(c.lens):
+        k, v = c.values(s)
+        rows = slice(s * block, (s + 1) * block)
+        qq = q[rows].double().reshape(block, Hkv, G, D)
+        size = float(torch.einsum("rhgd,htd->rhgt", qq.abs(), k.abs()).max()) * abs(scale)
+        scores_in_range(D, size)
+        w = torch.einsum("rhgd,htd->rhgt", qq, k) * scale
+        hidden = torch.arange(n, device="cuda") > pos[rows, None]
+        w = torch.softmax(w.masked_fill(hidden[:, None, None], -math.inf), dim=-1)
+        o, a = (torch.einsum("rhgt,htd->rhgd", w, x).reshape(block, -1).cpu() for x in (v, v.abs()))
+        close(out[rows].cpu(), o, a)
+        # A weight: twice the error of a score and of the maximum, as for short blocks, and 2^-19.  The sum over a row's tokens: a thread
+        # adds 32 + 2 numbers a block of 64 tokens and one number a block in turn (2^-24 each), and scales the sum once a block at worst, by an
+        # exponential of 2^-22 + 2^-24; the row's parts, a few, add 2^-24 each.  The sum over a token's pairs: 2^-24 each.
+        blocks = (n + 63) // 64
+        eps = 2 * (D + 16) * 2 ** -24 * size + 2 ** -19 + (34 + blocks + 8) * 2 ** -24 + blocks * (2 ** -22 + 2 ** -24) + block * G * 2 ** -24
+        want = w.sum((0, 2))
+        assert bool(((c.mass_of(s).double() - want).abs() <= eps * want + 1e-35).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,seqs", [(64, 38), (128, 38), (256, 19)])
+@pytest.mark.parametrize("G,block", [(5, 8), (5, 16)])
+def test_deep_tiles_are_the_definition_and_repeat_to_the_bit(D, seqs, G, block):
+    """As many units as fill the GPU, so that a CTA walks through a whole sequence (31 blocks and more): every call gives the same bits,
+    with warps that rescale at nearly every block beside warps that hardly ever do."""
+    c, q, pos = deep_case(D, G, block, seqs, seed=D + G + block)
+    geom = AttnGeom(c.Hkv * G, c.Hkv, D, D, 1 / math.sqrt(D))
+    seq = torch.arange(seqs, dtype=torch.int32, device="cuda").repeat_interleave(block)
+    out = torch.empty_like(q)
+    kv4.kv4_attn(q, seq, pos, c.table, c.kv, geom, out, max(c.lens), block=block, observe="set")
+    against_definition(c, q, pos, out, G, block, geom.scale)
+    first, mass = out.clone(), c.kv.mass.clone()
+    for _ in range(200):
+        out.fill_(9)
+        kv4.kv4_attn(q, seq, pos, c.table, c.kv, geom, out, max(c.lens), block=block, observe="set")
+        assert torch.equal(out, first) and torch.equal(c.kv.mass, mass)
