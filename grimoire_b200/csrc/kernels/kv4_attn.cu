@@ -841,8 +841,11 @@ __global__ void __launch_bounds__(Tile<D>::kThreads, Tile<D>::kCtas) tile_kernel
       bool good = mbar_wait(&b_q, 0u, p.status, 0x4b563410u) && mbar_wait(&b_k[0], 0u, p.status, 0x4b563411u);
       if (good) issue_s(0);
       for (int j = 0; j < nblk && good; ++j) {
-        if (j + 1 < nblk) {                              // (its TMEM buffer holds P(j - 1), whose product was issued before)
+        if (j + 1 < nblk) {
           good = mbar_wait(&b_k[(j + 1) & 1], (uint32_t)((j + 1) >> 1) & 1u, p.status, 0x4b563412u);
+          // its TMEM buffer holds P(j - 1): products with different accumulators are not ordered by their issue, so P V(j - 1) has to be
+          // through with it (it runs beside the softmax of block j, which takes longer)
+          if (j > 0) good = good && mbar_wait(&b_o[(j - 1) & 1], (uint32_t)((j - 1) >> 1) & 1u, p.status, 0x4b56341au);
           if (!good) break;
           issue_s(j + 1);
         }

@@ -83,7 +83,7 @@ def against_definition(c, q, pos, out, G, block, scale):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("D,seqs", [(64, 38), (128, 38), (256, 19)])
-@pytest.mark.parametrize("G,block", [(5, 8), (5, 16)])
+@pytest.mark.parametrize("G,block", [(5, 8), (5, 16), (8, 16)])
 def test_deep_tiles_are_the_definition_and_repeat_to_the_bit(D, seqs, G, block):
     """As many units as fill the GPU, so that a CTA walks through a whole sequence (31 blocks and more): every call gives the same bits,
     with warps that rescale at nearly every block beside warps that hardly ever do."""
