@@ -1422,7 +1422,8 @@ int plan(Plan& pl, long M, long Hq, long Hkv, long D, long block, long max_len, 
   // 2 x 8192 x 4 138 / 109; 96 pairs at head_dim 256, 2 x 8192 x 4 152 / 123; 40 pairs, 4 x 8192 x 8 109 / 106; but 20 pairs of
   // those 94 / 102, 40 pairs, 8192 x 8 56 / 61, 80 pairs, 2001 x 8 44 / 50.
   const long key_pages = (max_len + kPage - 1) / kPage;
-  pl.tile = block * G >= 40 && M * Hq * key_pages >= 256L * 1024;
+  // alone: as in a call of one block, in this as in the cut of the keys below
+  pl.tile = block * G >= 40 && (alone ? block : M) * Hq * key_pages >= 256L * 1024;
   const int most = pl.tile ? 128 : (D == 256 ? 8 : 16);
   pl.heads = G < most ? G : most;
   pl.subs = (G + pl.heads - 1) / pl.heads;

@@ -98,3 +98,26 @@ def test_deep_tiles_are_the_definition_and_repeat_to_the_bit(D, seqs, G, block):
         out.fill_(9)
         kv4.kv4_attn(q, seq, pos, c.table, c.kv, geom, out, max(c.lens), block=block, observe="set")
         assert torch.equal(out, first) and torch.equal(c.kv.mass, mass)
+
+
+def call(c, rows, q, pos, G, max_len, block, **kw):
+    """Outputs of blocks of sequences ``rows`` (a sequence per block)."""
+    seq = torch.tensor(rows, dtype=torch.int32, device="cuda").repeat_interleave(block)
+    out = torch.empty_like(q)
+    kv4.kv4_attn(q, seq, torch.tensor(pos, dtype=torch.int32, device="cuda"), c.table, c.kv, AttnGeom(c.Hkv * G, c.Hkv, c.D, c.D, 0.1), out, max_len,
+                 block=block, **kw)
+    return out
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,Hkv,G,block,max_len", [(128, 8, 5, 16, 4096), (128, 8, 5, 16, 8192), (64, 4, 8, 5, 16384), (256, 4, 6, 7, 12000), (128, 8, 5, 1, 4096)])
+def test_alone_means_the_bits_of_a_call_of_one_block(D, Hkv, G, block, max_len):
+    """Below and above the number of pairs and keys from which one block, or only several of them, would run in tiles."""
+    c = LongCache([3000, 2100, 2900], Hkv, D, seed=D + block)
+    q = torch.randn(3 * block, Hkv * G * D, device="cuda", generator=torch.Generator(device="cuda").manual_seed(block)).bfloat16()
+    pos = [n - block + r for n in c.lens for r in range(block)]
+    together = call(c, [0, 1, 2], q, pos, G, max_len, block, alone=True)
+    for s in range(3):
+        rows = slice(s * block, (s + 1) * block)
+        for kw in (dict(), dict(alone=True)):
+            assert torch.equal(call(c, [s], q[rows], pos[rows], G, max_len, block, **kw), together[rows])
