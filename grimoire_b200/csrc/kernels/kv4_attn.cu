@@ -1443,10 +1443,11 @@ int plan(Plan& pl, long M, long Hq, long Hkv, long D, long block, long max_len, 
   // Streamed: every CTA gets the same number of pages of the flat list, whatever the rows' lengths, at the price of a scan over
   // the rows and of parts that begin anywhere.  Split: a fixed number of CTAs a unit, at least eight pages (a step of the four
   // warps) each.  Measured, us split / streamed: 8 rows of up to 4999 tokens x 8 heads (45 pages a CTA) 20.7 / 24.5, 16 rows of
-  // up to 8191 at head_dim 256 (110 pages) 51.0 / 54.1, one row of 131072 (147 pages) 47.9 / 52.7, 32 rows of up to 32768 (900
-  // pages) 320 / 231.
+  // up to 8191 at head_dim 256 (110 pages) 51.0 / 54.1, 32 rows of up to 32768 (900 pages) 320 / 231.  A single block has nothing to
+  // even out and is always split, at whatever length, so that its rows and those of `alone` calls are cut alike: one row of 200000
+  // tokens x 8 heads 69.7 / 77.8, of 524288 152 / 156, of 262144 x 4 heads of 256 90 / 90.
   pl.splits = 0;
-  if (pl.tile || alone || units > kMaxUnits || cells * pages < 256L * pl.ctas) {
+  if (pl.tile || alone || M == block || units > kMaxUnits || cells * pages < 256L * pl.ctas) {
     long s = pages / 8 < pl.ctas / cells ? pages / 8 : pl.ctas / cells;
     pl.splits = (int)(s < 1 ? 1 : s);
   }

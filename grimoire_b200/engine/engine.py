@@ -348,7 +348,7 @@ class Engine:
         distinct = len({s.slot for s in seqs}) == M      # no verify block: the attention kernel may append K / V itself
         shape = ()
         if not distinct and self.kv.bits == 4:
-            splits = -self._splits_for(1, max_len)       # verify blocks over 4-bit pages: every row as in a step of its own
+            splits = -self._splits_for(1, max_len)       # verify blocks over 4-bit pages: every row as in a step of its own with this bound
         elif not distinct and max_len < K.VERIFY_ATTN_MIN_CTX:
             # Short contexts: every row of a verify block is scored exactly as a single-row step at its position would be
             # (the per-row kernel with the single-row split factor, whose page partition depends on the row's own length

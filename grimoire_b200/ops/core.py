@@ -244,9 +244,9 @@ def paged_decode_attn(q: torch.Tensor, row_seq: torch.Tensor, row_pos: torch.Ten
                       gate: Optional[torch.Tensor] = None, observe: Optional[str] = None) -> torch.Tensor:
     """Attention of M (sequence, position) rows over the paged int8 cache; see attn_decode.cu.
 
-    Over 4-bit pages (``ops.kv4``) ``splits`` is the bound on the rows' lengths that the step was planned with, negative where a
-    row's result must not depend on the step's other rows (verify blocks), and ``observe`` may keep the weight that every
-    cached token draws."""
+    Over 4-bit pages (``ops.kv4``) ``splits`` is the bound on the rows' lengths that the step was planned with, negative where every
+    row is to give what a step of that row alone, planned with the same bound, gives (verify blocks), and ``observe`` may keep
+    the weight that every cached token draws."""
     if _four_bit(kv):
         from . import kv4
 

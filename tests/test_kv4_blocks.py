@@ -121,3 +121,17 @@ def test_alone_means_the_bits_of_a_call_of_one_block(D, Hkv, G, block, max_len):
         rows = slice(s * block, (s + 1) * block)
         for kw in (dict(), dict(alone=True)):
             assert torch.equal(call(c, [s], q[rows], pos[rows], G, max_len, block, **kw), together[rows])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D,Hkv,G", [(128, 8, 5), (64, 16, 2), (256, 4, 6)])
+@pytest.mark.parametrize("max_len", [1 << 16, 1 << 17, 1 << 18, 1 << 20])
+def test_rows_of_a_verify_block_equal_single_steps_at_announced_lengths(D, Hkv, G, max_len):
+    """One row by itself, and the same row among others with alone=True, below and above the lengths from which a batch's pages are dealt
+    out over all CTAs."""
+    c = LongCache([2500], Hkv, D, seed=G)
+    q = torch.randn(5, Hkv * G * D, device="cuda", generator=torch.Generator(device="cuda").manual_seed(G)).bfloat16()
+    pos = list(range(2495, 2500))
+    block = call(c, [0] * 5, q, pos, G, max_len, 1, alone=True)
+    for i in range(5):
+        assert torch.equal(call(c, [0], q[i: i + 1], pos[i: i + 1], G, max_len, 1), block[i: i + 1])
