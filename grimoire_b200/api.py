@@ -242,7 +242,7 @@ class Grimoire:
                 raise UnsupportedModel("the head / sequence exchange (multi UP) runs over whole replicas of the dense decoder family")
             UlyssesParallel(up_group, dev).attach(model)
         # draft head: on a single-stage, single-rank dense model or dense-FFN hybrid (the reference drafts on the last stage)
-        want_mtp = mtp_src is not None and ec.tp_world == 1 and ec.pp_world == 1
+        want_mtp = mtp_src is not None and ec.tp_world == 1 and ec.pp_world == 1 and not ec.kv_keep      # (eviction: nothing is drafted)
         lim = EngineLimits(max_slots=ec.seq_slots, max_ctx=ec.ctx, prefill_chunk=ec.prefill_chunk, max_decode_rows=64,
                            kv_pages=ec.kv_pages, extra_kv_layers=1 if want_mtp else 0, kv_bits=ec.kv_bits, kv_keep=ec.kv_keep, kv_recent=ec.kv_recent)
         eng = Engine(model, lim)
@@ -255,8 +255,8 @@ class Grimoire:
             g.drafter = MtpDrafter(eng, MtpHead.from_checkpoint(model, mtp_src, draft_vocab=ec.mtp_draft_vocab))
         elif ec.dflash_model:
             # --dflash-model: a block drafter over the target's residual taps (dense family, one GPU)
-            if hybrid or ec.tp_world > 1 or ec.pp_world > 1:
-                raise UnsupportedModel("the block drafter (--dflash-model) runs beside a single-GPU dense target")
+            if hybrid or ec.tp_world > 1 or ec.pp_world > 1 or ec.kv_keep:
+                raise UnsupportedModel("the block drafter (--dflash-model) runs beside a single-GPU dense target whose cache is not cut (--kv-keep)")
             from .models.dflash_drafter import load_dflash
 
             g.drafter = load_dflash(ec.dflash_model, eng)
@@ -276,7 +276,8 @@ class Grimoire:
             f"  kv cache   : {'int8' if self.engine.kv.bits == 8 else '4-bit'} paged, {self.engine.kv.num_pages} pages x 16 tokens, {self.engine.kv.bytes_per_token()} B/token"
             + (f", cut to {ec.kv_keep} tokens a conversation" if ec.kv_keep else ""),
             f"  batching   : width {ec.width()}, prefill chunk {ec.prefill_chunk}, interleave chunk {ec.interleave_chunk}",
-            f"  speculation: copy drafts={'on' if ec.copy_drafts else 'off'} depth table {ec.spec_depth_table()}",
+            f"  speculation: copy drafts={'on' if ec.copy_drafts else 'off'} depth table {ec.spec_depth_table()}" if getattr(self.engine, "takes_drafts", True)
+            else "  speculation: off (the cache is cut by attention weight)",
             f"  prefix     : {'on' if self.engine.prefix_cache is not None else 'off'}",
             f"  norms      : {'zero-centred (1+w)' if m.cfg.norm_zero_centered else 'plain w'}",
         ]
@@ -315,7 +316,7 @@ class Grimoire:
             from .sched.scheduler import Scheduler
 
             ec = self.config
-            spec = self.drafter is not None or (ec.copy_drafts and getattr(self.model, "supports_verify_rows", True))
+            spec = getattr(self.engine, "takes_drafts", True) and (self.drafter is not None or (ec.copy_drafts and getattr(self.model, "supports_verify_rows", True)))
             self._sched = Scheduler(self.engine, width=ec.width(), interleave_chunk=ec.interleave_chunk,
                                     prefill_chunk=ec.prefill_chunk, hold_ms=ec.admit_hold_ms, hold_long_ms=ec.admit_hold_long_ms,
                                     depths=ec.spec_depth_table() if spec else (0,), spec_rows=ec.spec_rows,

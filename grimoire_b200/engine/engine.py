@@ -31,7 +31,8 @@ class EngineLimits:
     extra_kv_layers: int = 0         # KV layers beyond the model's own (1 for an MTP draft head)
     kv_bits: int = 8                 # bits of a cached K / V element: 8 (a scale per token and head) or 4 (a maximum per 32)
     # eviction over 4-bit pages: a conversation that has grown to kv_keep + kv_slack cached tokens is cut to kv_keep -- the first
-    # kv_sink, the last kv_recent and those that drew the most attention weight; 0 keeps everything
+    # kv_sink, the last kv_recent and those that drew the most attention weight; 0 keeps everything.  Nothing is drafted then: the
+    # weight counts the conversation's own rows only
     kv_keep: int = 0
     kv_recent: int = 0               # 0 = half of kv_keep
     kv_sink: int = 4
@@ -107,6 +108,12 @@ class Engine:
             if not seq.dropped:          # (what is left of a cut conversation is nobody's prefix)
                 self.prefix_cache.store(seq, head_logits, extra)
         self.kv.release(seq)
+
+    @property
+    def takes_drafts(self) -> bool:
+        """Whether drafted tokens may be scored as rows of a step.  With eviction they may not: every row adds to the weight that
+        the cached tokens have drawn, rejected ones too."""
+        return not self.limits.kv_keep
 
     def _kv_recent(self) -> int:
         return self.limits.kv_recent or self.limits.kv_keep // 2
@@ -304,6 +311,9 @@ class Engine:
             return []
         if M > self.limits.max_decode_rows:
             raise ValueError("too many rows for one step")
+        if not self.takes_drafts and len({s.slot for s in seqs}) != M:
+            # a rejected row's attention weight could not be taken back: what is evicted would depend on wrong guesses
+            raise NotImplementedError("with eviction from the KV cache a step scores one row of a conversation")
         if not getattr(self.model, "supports_verify_rows", True) and len({s.slot for s in seqs}) != M:
             # recurrent layers advance one token per conversation per step: no multi-row verify blocks
             raise NotImplementedError("this model cannot score several rows of one conversation in one step")

@@ -5,7 +5,7 @@ Same contract as the reference's ``generate_tokens<Engine>`` template (include/b
 82-432), which is written against an engine *concept* so host tests can drive it with fake engines
 (tests/test_generation.cpp).  Here the concept is the ``EngineLike`` protocol: anything that offers
 ``open / release / prefill / decode_rows / commit_rows`` (and optionally ``draft`` / ``rollback`` /
-``prefix_reuse`` / ``trim``) can be driven -- the real ``Engine`` or the fakes of tests/test_generation.py.
+``prefix_reuse`` / ``trim`` / ``takes_drafts``) can be driven -- the real ``Engine`` or the fakes of tests/test_generation.py.
 
 Speculation: K draft tokens come from a drafter (MTP chain, copy / prompt-lookup, or none); ONE
 verify pass scores the candidate block as K+1 rows of the same conversation; the longest prefix
@@ -153,7 +153,8 @@ def generate_tokens(engine: EngineLike, prompt: Sequence[int], opts: GenerationO
     """Run one request to completion.  ``on_token(tok)`` returning False cancels at that token
     (client disconnect / stop signal).  Returns (tokens, finish_reason)."""
     own = seq is None
-    if opts.draft_depth > 0 and opts.drafter is not None and hasattr(engine, "enable_speculation"):
+    drafter = opts.drafter if getattr(engine, "takes_drafts", True) else None
+    if opts.draft_depth > 0 and drafter is not None and hasattr(engine, "enable_speculation"):
         engine.enable_speculation()            # verify blocks and single rows on the same arithmetic from here on
     if own:
         seq = engine.open()
@@ -181,16 +182,16 @@ def generate_tokens(engine: EngineLike, prompt: Sequence[int], opts: GenerationO
                 engine.trim(seq)                       # KV eviction, where the engine is set up for it
             pos = seq.length
             drafts: list[int] = []
-            if opts.draft_depth > 0 and opts.drafter is not None:
+            if opts.draft_depth > 0 and drafter is not None:
                 room = opts.max_new - len(out) - 1
                 depth = max(0, min(opts.draft_depth, room))
                 if depth:
-                    drafts = list(opts.drafter.propose(engine, seq, tok, depth))[:depth]
+                    drafts = list(drafter.propose(engine, seq, tok, depth))[:depth]
             if not drafts:
                 nxt = engine.decode_rows([tok], [seq], [pos], use_graph=opts.use_graph)
                 engine.commit_rows([seq], [tok], [pos])
-                if opts.drafter is not None:
-                    opts.drafter.observe(engine, seq, [tok])      # a model drafter tracks the newest hidden state
+                if drafter is not None:
+                    drafter.observe(engine, seq, [tok])      # a model drafter tracks the newest hidden state
                 tok = int(nxt[0])
                 continue
             # ---- verify: block [tok, d1..dK] as K+1 rows of this conversation ----
@@ -216,7 +217,7 @@ def generate_tokens(engine: EngineLike, prompt: Sequence[int], opts: GenerationO
             engine.commit_rows([seq] * len(keep), keep, list(range(pos, pos + len(keep))))
             if hasattr(engine, "rollback"):
                 engine.rollback(seq, pos + len(keep))
-            opts.drafter.observe(engine, seq, keep)
+            drafter.observe(engine, seq, keep)
             stop = False
             for d in drafts[:accepted]:
                 out.append(d)

@@ -71,6 +71,10 @@ class ControlledEngine:
         self.limits, self.device, self.cfg, self.kv, self.model = engine.limits, engine.device, engine.cfg, engine.kv, engine.model
 
     @property
+    def takes_drafts(self) -> bool:
+        return self.engine.takes_drafts
+
+    @property
     def prefix_cache(self):
         return self.engine.prefix_cache
 
