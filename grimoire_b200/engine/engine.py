@@ -37,7 +37,7 @@ class EngineLimits:
     kv_recent: int = 0               # 0 = half of kv_keep
     kv_sink: int = 4
     kv_slack: int = 256
-    kv_observe: int = 32             # last rows of a prompt whose attention weight is kept
+    kv_observe: int = 32             # last rows of a prompt whose attention weight is kept (at most prefill_chunk)
 
 
 class Engine:
@@ -166,9 +166,11 @@ class Engine:
             self.prefill_buf = self.model.make_buffers(self._prefill_rows, self._prefill_logit_rows,
                                                        dense_kv_tokens=max(self.limits.max_ctx, self._prefill_rows))
 
-    def prefill(self, seq: SeqSlot, tokens: Sequence[int] | torch.Tensor, want_logits: bool = True) -> Optional[torch.Tensor]:
+    def prefill(self, seq: SeqSlot, tokens: Sequence[int] | torch.Tensor, want_logits: bool = True, last: bool = True) -> Optional[torch.Tensor]:
         """Append ``tokens`` to the sequence in chunks of ``prefill_chunk`` rows; returns the fp32
-        logits of the last token (device tensor [V]) when ``want_logits``."""
+        logits of the last token (device tensor [V]) when ``want_logits``.  ``last``: the prompt ends with these tokens.  With
+        eviction the attention weight of its last ``kv_observe`` rows is kept, once a prompt: one that comes in slices
+        should end with a slice of at least that many tokens (``ends_prompt``)."""
         self._ensure_prefill_buf()
         if not torch.is_tensor(tokens):
             tokens = torch.tensor(list(tokens), dtype=torch.int32)
@@ -186,6 +188,7 @@ class Engine:
         tok_dev = tokens.to(self.device, non_blocking=True)
         logits = None
         done = 0
+        held: list = []                  # observed rows that fall into the chunk before the last one: their queries, a tensor a layer
         while done < n:
             m = min(self._prefill_rows, n - done)
             pos0 = seq.length
@@ -196,8 +199,11 @@ class Engine:
             if self.limits.kv_keep:
                 if seq.dropped:
                     rb.row_rope = rows + seq.dropped
-                if done + m == n:
-                    rb.observe_rows, rb.observe = min(m, self.limits.kv_observe), "add" if seq.tokens else "set"
+                left, w = n - done - m, self._observed_rows()
+                if last and left == 0:
+                    rb.observe_rows, rb.observe, rb.observe_before = min(m, w), "add" if seq.tokens else "set", held
+                elif last and left < w:
+                    rb.hold_rows, rb.held = min(m, w - left), held
             out = self.model.forward(rb, self.prefill_buf, self.kv.layers, self.kv.table)
             if self.mtp is not None:
                 self.mtp.warm_chunk(seq, tok_dev, done, m, pos0, self.prefill_buf, last=(done + m == n))
@@ -215,6 +221,13 @@ class Engine:
             row = logits[0] if logits is not None else torch.empty(self.cfg.vocab_size, dtype=torch.float32, device=self.device)
             logits = pp.broadcast_from_last(row)[None]
         return logits[0] if want_logits else None
+
+    def _observed_rows(self) -> int:
+        return min(self.limits.kv_observe, self._prefill_rows)
+
+    def ends_prompt(self, left: int) -> bool:
+        """Whether a slice of a prompt that would leave ``left`` tokens has to take them too (see ``prefill``)."""
+        return left == 0 or (self.limits.kv_keep > 0 and left < self._observed_rows())
 
     def can_prefill_batch(self) -> bool:
         """Several fresh prompts in one M-row pass: dense models without a draft head or pipeline stages."""

@@ -14,7 +14,7 @@ all-reduce (parallel/tp.py) instead of accumulating into ``h`` directly.
 from __future__ import annotations
 
 from dataclasses import dataclass
-from typing import Optional
+from typing import Optional, Sequence
 
 import torch
 
@@ -77,6 +77,11 @@ class RowBatch:
     row_rope: Optional[torch.Tensor] = None
     observe: Optional[str] = None
     observe_rows: int = 0
+    # observed rows of the chunk before: their queries, a tensor a layer; a chunk that is followed by a short last one appends
+    # those of its own last ``hold_rows`` rows to ``held``
+    observe_before: Sequence[torch.Tensor] = ()
+    hold_rows: int = 0
+    held: Optional[list] = None
 
 
 class Buffers:
@@ -634,11 +639,16 @@ class DenseModel:
                 K.rope_kvwrite(qkv, rope_pos, rb.row_seq, block_table, self.inv_freq, geom, q, kvl, L.q_norm, L.k_norm,
                                gate, buf.dense_k[rb.q_pos0: T], buf.dense_v[rb.q_pos0: T], row_cache=row_cache)
                 K.flash_prefill(q, buf.dense_k, buf.dense_v, geom, attn, rb.q_pos0, gate)
+                if rb.hold_rows:
+                    rb.held.append(q[M - rb.hold_rows: M].clone())
                 if rb.observe_rows:
-                    # what the chunk's last rows look at: the weight that a later eviction goes by (their output is not needed)
-                    w = rb.observe_rows
-                    kv4.kv4_attn(q[M - w: M], rb.row_seq[M - w: M], rb.row_pos[M - w: M], block_table, kvl, geom,
-                                 torch.empty(w, q.shape[1], dtype=q.dtype, device=q.device), T, block=w, observe=rb.observe)
+                    # what the prompt's last rows look at: the weight that a later eviction goes by (their output is not needed)
+                    qw = q[M - rb.observe_rows: M]
+                    if rb.observe_before:
+                        qw = torch.cat((rb.observe_before[li], qw))
+                    w = qw.shape[0]
+                    kv4.kv4_attn(qw, rb.row_seq[:1].expand(w).contiguous(), torch.arange(T - w, T, dtype=torch.int32, device=q.device), block_table,
+                                 kvl, geom, torch.empty_like(qw), T, block=w, observe=rb.observe)
             elif not ((M == 1 or rb.distinct) and gate is None and K.paged_decode_attn_fused(qkv, self.inv_freq, L.q_norm, L.k_norm, rb.row_seq, rb.row_pos,
                                                                           block_table, kvl, geom, attn, rb.splits, self.ws, prefetch=True)):
                 K.rope_kvwrite(qkv, rope_pos, rb.row_seq, block_table, self.inv_freq, geom, q, kvl, L.q_norm, L.k_norm, gate, row_cache=row_cache)

@@ -294,7 +294,13 @@ class Scheduler:
                 if lo >= hi:
                     hi = min(len(job.prompt), max(hi, lo))
             lo = max(lo, job.seq.length)
-            logits = eng.prefill(job.seq, job.prompt[lo:hi]) if hi > lo or lo >= len(job.prompt) else None
+            kw = {}
+            if getattr(eng.limits, "kv_keep", 0):
+                # the last rows of a prompt are observed, in one piece and once
+                if eng.ends_prompt(len(job.prompt) - hi):
+                    hi = len(job.prompt)
+                kw = {"last": hi == len(job.prompt)}
+            logits = eng.prefill(job.seq, job.prompt[lo:hi], **kw) if hi > lo or lo >= len(job.prompt) else None
             self.metrics["admit_rows"] += max(0, hi - lo)
             state = self.lib.grm_sched_on_prefilled(self.h, ctypes.c_int64(job.id), hi)
             if state == 2 and logits is not None:

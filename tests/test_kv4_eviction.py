@@ -1,4 +1,6 @@
 """Conversations cut by attention weight: what the weight counts, when a cut happens, and what must not depend on it."""
+import threading
+
 import pytest
 import torch
 
@@ -53,3 +55,53 @@ def test_scheduler_drafts_nothing_over_a_cut_cache():
         finally:
             s.shutdown()
     assert outs[0] == outs[1] and len(outs[0][0]) == 30
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("n", [20, 100, 131])
+def test_a_prompt_is_observed_once_however_it_is_read(device, n):
+    """Whole, in chunks whose last one would be short, in slices: the last 32 rows (all, of a shorter prompt) and nothing else."""
+    p, got = _prompt(n), []
+    for chunk, step in ((256, n), (33, n), (64, n), (256, 25), (64, 40), (128, 7)):
+        eng = _engine(device, kv_keep=48, kv_recent=16, prefill_chunk=chunk, kv_slack=200)
+        s = eng.open()
+        lo = 0
+        while lo < n:
+            hi = min(n, lo + step)
+            hi = n if eng.ends_prompt(n - hi) else hi
+            eng.prefill(s, p[lo:hi], last=hi == n)
+            lo = hi
+        m = _mass(eng, s)
+        rows = min(n, 32) * (eng.model.geom.Hq // eng.model.geom.Hkv)
+        # every row and query head gives a weight of one in all, summed in fp32 from weights that are off by 2^-9 at most
+        assert float((m.sum(1) - rows).abs().max()) < 2 ** -9 * rows
+        got.append(m[0])
+    # the first layer's rows and keys are the same up to the rounding of a projection (q is bf16): a few percent of a weight
+    for m in got[1:]:
+        assert float((m - got[0]).abs().sum(0).max()) < 0.05 * rows
+
+
+def test_scheduler_observes_a_sliced_prompt_once():
+    """A long prompt beside a conversation that decodes is read in slices; one observation of its last rows is made of it."""
+    eng = _engine("cpu", kv_keep=200, kv_recent=16, kv_slack=40, max_ctx=256)
+    seen, real = [], eng.model.forward
+
+    def forward(rb, *a):
+        if rb.mode == "prefill":
+            seen.append((rb.tokens.shape[0], rb.observe_rows, rb.observe))
+        return real(rb, *a)
+
+    eng.model.forward = forward
+    s = Scheduler(eng, width=2, hold_ms=0, hold_long_ms=0, interleave_chunk=24)
+    try:
+        started = threading.Event()
+        t = threading.Thread(target=lambda: s.generate(_prompt(8), 120, on_token=lambda _: started.set() or True))
+        t.start()
+        assert started.wait(60)
+        s.generate(_prompt(100, 2), 2)
+        t.join()
+    finally:
+        s.shutdown()
+    slices = seen[1:]
+    assert seen[0] == (8, 8, "set") and len(slices) > 1 and sum(x[0] for x in slices) == 100
+    assert [x[1] for x in slices] == [0] * (len(slices) - 1) + [32]
