@@ -60,7 +60,13 @@ class Engine:
             if lim.kv_keep < 1 or lim.kv_slack < 1 or lim.kv_observe < 1 or lim.kv_sink < 0 or self._kv_recent() + lim.kv_sink > lim.kv_keep or \
                     self._kv_recent() < 1:
                 raise ValueError("eviction: kv_keep tokens hold kv_sink first and kv_recent last ones, and at least one of the latter")
-        self.kv = KvPool(n_attn, model.geom.Hkv, model.geom.D, pages, lim.max_slots, lim.max_ctx, self.device, lim.kv_bits, lim.kv_keep > 0)
+            grown = lim.kv_keep + lim.kv_slack
+            if grown > lim.max_ctx or grown > pages * PAGE:
+                raise ValueError(f"eviction: a conversation is cut when it has grown to kv_keep + kv_slack = {grown} tokens; the context of "
+                                 f"{lim.max_ctx} and a pool of {pages} pages have to hold that many")
+        # a cut copies what stays before it frees anything: pages for one copy are kept aside
+        self.kv = KvPool(n_attn, model.geom.Hkv, model.geom.D, pages, lim.max_slots, lim.max_ctx, self.device, lim.kv_bits, lim.kv_keep > 0,
+                         reserve=(lim.kv_keep + PAGE - 1) // PAGE)
         chunk = min(lim.prefill_chunk, lim.max_ctx)
         self.prefill_buf: Optional[Buffers] = None
         self._prefill_rows = chunk
@@ -127,6 +133,8 @@ class Engine:
         if done:
             del seq.tokens[: len(seq.tokens) - seq.length]      # drafters look for the newest tokens
             self.counters["kv_evictions"] = self.counters.get("kv_evictions", 0) + 1
+        else:                            # only where other sequences hold on to the pages that earlier cuts left (share_prefix)
+            self.counters["kv_evictions_failed"] = self.counters.get("kv_evictions_failed", 0) + 1
         return done
 
     def enable_prefix_cache(self, max_entries: int = 16):

@@ -31,10 +31,11 @@ class SeqSlot:
 
 
 class KvPool:
-    """Page allocator + per-slot block tables for ``n_layers`` attention layers."""
+    """Page allocator + per-slot block tables for ``n_layers`` attention layers.  ``reserve``: pages beyond ``num_pages`` that no
+    sequence is grown with: what ``evict`` copies to, so that a full pool can still be cut."""
 
     def __init__(self, n_layers: int, Hkv: int, D: int, num_pages: int, max_slots: int, max_ctx: int, device,
-                 bits: int = 8, mass: bool = False):
+                 bits: int = 8, mass: bool = False, reserve: int = 0):
         if bits not in (4, 8) or (mass and bits != 4):
             raise ValueError("KV pages hold 8 or 4 bits an element; the weight of cached tokens is kept with 4-bit pages")
         self.bits = bits
@@ -42,10 +43,13 @@ class KvPool:
         self.num_pages = num_pages
         self.max_slots = max_slots
         self.max_pages_per_seq = (max_ctx + PAGE - 1) // PAGE
-        alloc = (lambda: KvLayer.alloc(num_pages, Hkv, D, device)) if bits == 8 else (lambda: Kv4Layer.alloc(num_pages, Hkv, D, device, mass))
+        total = num_pages + reserve
+        alloc = (lambda: KvLayer.alloc(total, Hkv, D, device)) if bits == 8 else (lambda: Kv4Layer.alloc(total, Hkv, D, device, mass))
         self.layers = [alloc() for _ in range(n_layers)]
-        self.refcount = [0] * num_pages
+        self.refcount = [0] * total
         self.free = list(range(num_pages - 1, -1, -1))
+        self.reserve = reserve
+        self.spare = list(range(num_pages, total))          # pages of the reserve at hand
         # block table lives on the device (kernels index it) with a pinned host mirror
         self.table_host = torch.full((max_slots, self.max_pages_per_seq), -1, dtype=torch.int32)
         if self.device.type == "cuda":
@@ -60,7 +64,7 @@ class KvPool:
         return len(self.free)
 
     def pages_used(self) -> int:
-        return self.num_pages - len(self.free)
+        return self.num_pages + self.reserve - len(self.free) - len(self.spare)
 
     def bytes_per_token(self) -> int:
         return sum(l.bytes_per_token() for l in self.layers)
@@ -99,14 +103,18 @@ class KvPool:
         if grew:
             self._sync_row(seq.slot)
 
+    def _drop(self, pg: int) -> None:
+        """One owner less; a page without any goes back, to the reserve first."""
+        self.refcount[pg] -= 1
+        if self.refcount[pg] == 0:
+            (self.spare if len(self.spare) < self.reserve else self.free).append(pg)
+
     def _sync_row(self, slot: int) -> None:
         self.table[slot].copy_(self.table_host[slot], non_blocking=True)
 
     def release(self, seq: SeqSlot) -> None:
         for pg in seq.pages:
-            self.refcount[pg] -= 1
-            if self.refcount[pg] == 0:
-                self.free.append(pg)
+            self._drop(pg)
         self.table_host[seq.slot].fill_(-1)
         self._sync_row(seq.slot)
         seq.pages.clear()
@@ -121,9 +129,7 @@ class KvPool:
         while len(seq.pages) > keep:
             pg = seq.pages.pop()
             self.table_host[seq.slot, len(seq.pages)] = -1
-            self.refcount[pg] -= 1
-            if self.refcount[pg] == 0:
-                self.free.append(pg)
+            self._drop(pg)
         seq.length = min(seq.length, length)
         del seq.tokens[length:]
         self._sync_row(seq.slot)
@@ -137,20 +143,18 @@ class KvPool:
         need = (keep + PAGE - 1) // PAGE
         if seq.length <= keep:
             return False
-        if need > len(self.free) and self.reclaim is not None:
-            self.reclaim(need)
-        if need > len(self.free):
+        if need > len(self.spare) + len(self.free) and self.reclaim is not None:
+            self.reclaim(need - len(self.spare))
+        if need > len(self.spare) + len(self.free):
             return False
-        fresh = [self.free.pop() for _ in range(need)]
+        fresh = [(self.spare or self.free).pop() for _ in range(need)]
         i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=self.device)
         slot, length, dst = i32([seq.slot]), i32([seq.length]), i32([fresh])
         for layer in self.layers:
             kept = kv4_select(layer, slot, length, self.table, keep, recent, sink)
             kv4_compact(layer, slot, kept, self.table, dst)
         for pg in seq.pages:
-            self.refcount[pg] -= 1
-            if self.refcount[pg] == 0:
-                self.free.append(pg)
+            self._drop(pg)
         for pg in fresh:
             self.refcount[pg] = 1
         self.table_host[seq.slot].fill_(-1)

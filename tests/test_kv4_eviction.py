@@ -105,3 +105,50 @@ def test_scheduler_observes_a_sliced_prompt_once():
     slices = seen[1:]
     assert seen[0] == (8, 8, "set") and len(slices) > 1 and sum(x[0] for x in slices) == 100
     assert [x[1] for x in slices] == [0] * (len(slices) - 1) + [32]
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("slots,pages", [(1, 0), (1, 4), (2, 8)])
+def test_a_full_pool_can_still_be_cut(device, slots, pages):
+    """A pool that conversations fill to the last page: every one is cut in its turn, and never grows past keep + slack tokens."""
+    eng = _engine(device, **CUT, max_slots=slots, max_ctx=64, kv_pages=pages)
+    seqs = [eng.open() for _ in range(slots)]
+    for i, s in enumerate(seqs):
+        eng.prefill(s, _prompt(60, i))
+    for i, t in enumerate(_prompt(60, 6)):
+        eng.decode_rows([t] * slots, seqs, [s.length for s in seqs])
+        eng.commit_rows(seqs, [t] * slots, [s.length for s in seqs])
+        for s in seqs:
+            assert eng.trim(s) == ((60 + i + 1 - 64) % 16 == 0 and i >= 3)
+    assert eng.counters["kv_evictions"] == 4 * slots and "kv_evictions_failed" not in eng.counters
+    assert eng.kv.pages_free() == eng.kv.num_pages - sum(len(s.pages) for s in seqs)
+    for s in seqs:
+        eng.release(s)
+    assert eng.kv.pages_used() == 0 and eng.kv.pages_free() == eng.kv.num_pages
+
+
+def test_one_request_in_a_pool_of_its_own_size_is_bounded():
+    """The path of a single request with one slot, whose pool holds one context: cut instead of growing to the end of it."""
+    eng = _engine("cpu", **CUT, max_slots=1, max_ctx=96)
+    toks = eng.generate(_prompt(40), 56, use_graph=False)
+    assert len(toks) == 56 and eng.counters["kv_evictions"] == 2
+
+
+def test_limits_that_would_never_cut_are_refused():
+    for lim in (dict(kv_keep=48, kv_slack=16, max_ctx=63), dict(kv_keep=48, kv_slack=16, max_ctx=96, kv_pages=3)):
+        with pytest.raises(ValueError):
+            _engine("cpu", **lim)
+    _engine("cpu", kv_keep=48, kv_slack=16, max_ctx=64, kv_pages=4)
+
+
+def test_a_cut_that_finds_no_pages_is_counted():
+    """Sequences that share pages keep them from the reserve: the cut is refused, counted, and tried again later."""
+    eng = _engine("cpu", **CUT, max_slots=3, max_ctx=64, kv_pages=8)
+    a, b, c = eng.open(), eng.open(), eng.open()
+    eng.prefill(a, _prompt(64))
+    eng.kv.share_prefix(a, b, 64)
+    eng.prefill(c, _prompt(64, 2))
+    assert eng.trim(a) and eng.kv.pages_free() == 0                  # b holds what a left
+    assert not eng.trim(c) and c.length == 64 and eng.counters["kv_evictions_failed"] == 1
+    eng.release(b)
+    assert eng.trim(c) and c.length == 48
