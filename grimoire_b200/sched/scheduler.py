@@ -365,6 +365,9 @@ class Scheduler:
             eng.commit_rows([job.seq] * len(keep), keep, list(range(pos0, pos0 + len(keep))))
             if n > 1 and hasattr(eng, "rollback"):
                 eng.rollback(job.seq, pos0 + len(keep))
+            # the next token's position in the conversation: a draw is a function of seed and position, and cached positions come back
+            # after every cut
+            place = pos0 + len(keep) + getattr(job.seq, "dropped", 0)
             if hasattr(eng, "trim"):
                 eng.trim(job.seq)                                      # KV eviction, where the engine is set up for it
             if self.drafter is not None:
@@ -379,6 +382,6 @@ class Scheduler:
             if job.sampling.greedy:
                 nxt = int(chosen[o + accepted])
             else:
-                nxt = self._pick(job, logits[o + accepted], pos0 + accepted + 1)
+                nxt = self._pick(job, logits[o + accepted], place)
             job.next_token = nxt
             self._emit(job, nxt)

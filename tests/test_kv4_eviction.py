@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from grimoire_b200.engine.generation import CopyDrafter, GenerationOptions, generate_tokens
+from grimoire_b200.engine.sampling import SamplingOptions
 from grimoire_b200.sched.scheduler import Scheduler
 
 from .test_kv4_engine import DEVICES, _engine, _prompt
@@ -152,3 +153,23 @@ def test_a_cut_that_finds_no_pages_is_counted():
     assert not eng.trim(c) and c.length == 64 and eng.counters["kv_evictions_failed"] == 1
     eng.release(b)
     assert eng.trim(c) and c.length == 48
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_sampled_tokens_are_drawn_at_positions_that_never_come_back(device):
+    """A draw is a function of (seed, position): over several cuts the positions are those of the conversation."""
+    eng = _engine(device, **CUT)
+    drawn, real = [], eng.sample_rows
+
+    def sample_rows(logits, opts, positions):
+        drawn.extend(positions)
+        return real(logits, opts, positions)
+
+    eng.sample_rows = sample_rows
+    s = Scheduler(eng, width=2, hold_ms=0, hold_long_ms=0)
+    try:
+        out, _, _ = s.generate(_prompt(40), 80, sampling=SamplingOptions(temperature=0.8, top_k=20, seed=3))
+    finally:
+        s.shutdown()
+    assert eng.counters["kv_evictions"] >= 3 and len(out) == 80
+    assert drawn == list(range(40, 120))
