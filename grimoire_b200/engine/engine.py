@@ -83,7 +83,6 @@ class Engine:
         self.d_groups = torch.zeros(4, lim.max_decode_rows, dtype=torch.int32, device=self.device)
         self.h_next = torch.zeros(lim.max_decode_rows, dtype=torch.int32, pin_memory=pin)
         self.prefix_cache = None
-        self._warming = False             # a run before a capture: its rows are counted once, by the replay
         self._verify: dict = {}           # slot -> (handle, first row, rows, first position) of its last verify block
         self._reused_head_logits = None
         self.graphs: dict[tuple, "torch.cuda.CUDAGraph"] = {}      # (rows, splits, distinct sequences)
@@ -305,12 +304,13 @@ class Engine:
             return length_bucket(max_len)
         return K.decode_splits(max_len, M, self.model.geom.Hkv)
 
-    def _run_rows(self, M: int, splits: int, distinct: bool = False, runs=None, full_logits: bool = True, ngroups: int = 0) -> torch.Tensor:
+    def _run_rows(self, M: int, splits: int, distinct: bool = False, runs=None, full_logits: bool = True, ngroups: int = 0,
+                  observe: bool = True) -> torch.Tensor:
         hs = getattr(self.model, "head_split", None)
         rb = RowBatch(self.d_tokens[:M], self.d_row_seq[:M], self.d_row_pos[:M], mode="decode", splits=splits, distinct=distinct, runs=runs,
                       full_logits=full_logits or hs is None, verify=(self.d_groups, ngroups) if ngroups else None)
         if self.limits.kv_keep:
-            rb.row_rope, rb.observe = self.d_row_rope[:M], None if self._warming else "add"
+            rb.row_rope, rb.observe = self.d_row_rope[:M], "add" if observe else None
         logits = self.model.forward(rb, self.decode_buf, self.kv.layers, self.kv.table)
         pp = getattr(self.model, "pp", None)
         if logits is not None and hs is not None and not rb.full_logits:
@@ -469,9 +469,7 @@ class Engine:
         # must not keep the warm-up run's update
         saved = self._save_recurrent(M)
         full = getattr(self.model, "head_split", None) is None     # a split head is captured with its (value, index) pick
-        self._warming = True
-        self._run_rows(M, splits, distinct, full_logits=full, ngroups=ngroups)
-        self._warming = False
+        self._run_rows(M, splits, distinct, full_logits=full, ngroups=ngroups, observe=False)       # (its rows are counted once, by the replay)
         torch.cuda.current_stream().synchronize()
         self._restore_recurrent(saved)
         g = torch.cuda.CUDAGraph()
@@ -498,17 +496,15 @@ class Engine:
         splits = self._splits_for(M, max_len)
         distinct = len({s.slot for s in seqs}) == M
 
-        def body():
-            self._run_rows(M, splits, distinct, full_logits=getattr(self.model, "head_split", None) is None)
+        def body(observe=True):
+            self._run_rows(M, splits, distinct, full_logits=getattr(self.model, "head_split", None) is None, observe=observe)
             self.d_tokens[:M].copy_(self.decode_buf.next_ids[:M])
             self.d_row_pos[:M].add_(1)
             self.d_row_rope[:M].add_(1)
 
         saved = (self.d_tokens[:M].clone(), self.d_row_pos[:M].clone(), self.d_row_rope[:M].clone())
         rec = self._save_recurrent(M)
-        self._warming = True
-        body()                       # warm-up outside capture (also sizes the workspace)
-        self._warming = False
+        body(observe=False)          # warm-up outside capture (also sizes the workspace)
         torch.cuda.current_stream().synchronize()
         self.d_tokens[:M].copy_(saved[0]); self.d_row_pos[:M].copy_(saved[1]); self.d_row_rope[:M].copy_(saved[2])
         self._restore_recurrent(rec)

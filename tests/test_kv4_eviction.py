@@ -173,3 +173,35 @@ def test_sampled_tokens_are_drawn_at_positions_that_never_come_back(device):
         s.shutdown()
     assert eng.counters["kv_evictions"] >= 3 and len(out) == 80
     assert drawn == list(range(40, 120))
+
+
+def test_a_failed_capture_does_not_stop_the_weight():
+    """The run before a capture counts no rows; where it fails, the steps after it count theirs."""
+    eng = _engine("cpu", **CUT)
+    s = eng.open()
+    eng.prefill(s, _prompt(40))
+    real = eng.model.forward
+    eng.model.forward = lambda *a: (_ for _ in ()).throw(RuntimeError("out of memory"))
+    eng._stage_rows([1], [s.slot], [40], [s])
+    with pytest.raises(RuntimeError):
+        eng._capture(1, 64)
+    eng.model.forward = real
+    before = float(_mass(eng, s).sum())
+    eng.decode_rows([1], [s], [40], use_graph=False)
+    eng.commit_rows([s], [1], [40])
+    rows = len(eng.kv.layers) * eng.model.geom.Hq                    # a row gives a weight of one a layer and query head
+    assert abs(float(_mass(eng, s).sum()) - before - rows) < 2 ** -9 * rows
+
+
+@pytest.mark.gpu
+def test_replayed_steps_count_their_rows_once():
+    """The run before a capture and the capture itself add nothing; every replay adds its row."""
+    eng = _engine("cuda", kv_keep=200, kv_recent=16, kv_slack=40)
+    s = eng.open()
+    eng.prefill(s, _prompt(40))
+    rows = len(eng.kv.layers) * eng.model.geom.Hq
+    for i in range(4):
+        before = float(_mass(eng, s).sum())
+        eng.decode_rows([1], [s], [40 + i], use_graph=True)
+        eng.commit_rows([s], [1], [40 + i])
+        assert abs(float(_mass(eng, s).sum()) - before - rows) < 2 ** -9 * rows
