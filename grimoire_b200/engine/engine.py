@@ -64,6 +64,7 @@ class Engine:
             if grown > lim.max_ctx or grown > pages * PAGE:
                 raise ValueError(f"eviction: a conversation is cut when it has grown to kv_keep + kv_slack = {grown} tokens; the context of "
                                  f"{lim.max_ctx} and a pool of {pages} pages have to hold that many")
+            model.cut_cache = True           # (what is attached to the model later refuses by it)
         # a cut copies what stays before it frees anything: pages for one copy are kept aside
         self.kv = KvPool(n_attn, model.geom.Hkv, model.geom.D, pages, lim.max_slots, lim.max_ctx, self.device, lim.kv_bits, lim.kv_keep > 0,
                          reserve=(lim.kv_keep + PAGE - 1) // PAGE)

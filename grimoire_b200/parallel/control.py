@@ -67,6 +67,8 @@ class ControlledEngine:
     """Front-end side: same interface as ``Engine``; every call is announced before it runs."""
 
     def __init__(self, engine, channel: ControlChannel):
+        if getattr(engine.limits, "kv_keep", 0):
+            raise ValueError("eviction from the KV cache runs on one device: its cuts are not announced to other ranks")
         self.engine, self.ch = engine, channel
         self.limits, self.device, self.cfg, self.kv, self.model = engine.limits, engine.device, engine.cfg, engine.kv, engine.model
 

@@ -53,6 +53,8 @@ class ContextParallel:
         context-parallel path."""
         if getattr(model, "tp_world", 1) != 1 or getattr(model, "pp_world", 1) != 1:
             raise ValueError("context parallelism runs over whole model replicas (no tensor / pipeline shards)")
+        if getattr(model, "cut_cache", False):
+            raise ValueError("eviction from the KV cache runs on one device, not under context parallelism")
         model.cp = self
         geom = model.geom
         self.width = 2 * geom.Hkv * geom.D
