@@ -123,6 +123,16 @@ def _check_rows(t: torch.Tensor, M: int, W: int, dev: int, name: str, what: str)
     return t.data_ptr(), stride[0]
 
 
+def _apart(t: torch.Tensor) -> bool:
+    """Whether no two rows of ``t`` (the last dimension, contiguous) share memory: what a call writes must have places of its own."""
+    extent = t.shape[-1]
+    for stride, n in sorted((st, n) for st, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1):
+        if stride < extent:
+            return False
+        extent += stride * (n - 1)
+    return True
+
+
 def _ptr(t: Optional[torch.Tensor]) -> int:
     return 0 if t is None else t.data_ptr()
 
@@ -184,6 +194,8 @@ def kv4_gather(kv: Kv4Layer, block_table: torch.Tensor, slots: Optional[torch.Te
     for t in (out_k, out_v):
         if t.dtype is not _BF16 or t.dim() != 3 or t.shape[2] != Hkv * D or t.shape[:2] != out_k.shape[:2] or t.get_device() != dev or t.stride(2) != 1:
             raise ValueError("kv4_gather: out_k / out_v must be bf16 [sequences][tokens][kv heads * head_dim] with contiguous rows on the cache's device")
+        if not (t.is_contiguous() or _apart(t)):
+            raise ValueError("kv4_gather: rows of out_k / out_v must not share memory")
     S, T = out_k.shape[:2]
     seq, length = _check_ints(slots, S, dev, what), _check_ints(lengths, S, dev, what)
     if slots is None and S > table[1]:
@@ -239,6 +251,8 @@ def kv4_attn(q: torch.Tensor, row_seq: torch.Tensor, row_pos: torch.Tensor, bloc
         raise ValueError(f"kv4_attn: {Hq} query heads over {Hkv} kv heads: 1 to {MAX_GROUP} query heads a kv head are served")
     qp, qs = _check_rows(q, M, Hq * D, dev, "q", what)
     op, os_ = _check_rows(out, M, Hq * D, dev, "out", what)
+    if os_ < Hq * D and M > 1:
+        raise ValueError("kv4_attn: rows of out must not share memory")
     gp, gs = (0, 0) if gate is None else _check_rows(gate, M, Hq * D, dev, "gate", what)
     seq, pos = _check_ints(row_seq, M, dev, what), _check_ints(row_pos, M, dev, what)
     if block < 1 or M % block or M > 65535:

@@ -135,3 +135,33 @@ def test_rows_of_a_verify_block_equal_single_steps_at_announced_lengths(D, Hkv, 
     block = call(c, [0] * 5, q, pos, G, max_len, 1, alone=True)
     for i in range(5):
         assert torch.equal(call(c, [0], q[i: i + 1], pos[i: i + 1], G, max_len, 1), block[i: i + 1])
+
+
+# ---------------------------------------------------------------------------------------------
+# what a call writes
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_outputs_whose_rows_share_memory_are_refused(device):
+    D, Hkv = 64, 2
+    W = Hkv * D
+    kv = kv4.Kv4Layer.alloc(4, Hkv, D, device)
+    table = torch.zeros(2, 4, dtype=torch.int32, device=device)
+    two = torch.tensor([0, 1], dtype=torch.int32, device=device)
+    buf = torch.zeros(64 * W, dtype=torch.bfloat16, device=device)
+    q = buf[: 2 * W].view(2, W)
+    geom = AttnGeom(Hkv, Hkv, D, D, 0.1)
+    attn = lambda out: kv4.kv4_attn(q, two * 0, two, table, kv, geom, out, 2)
+    gather = lambda k, v: kv4.kv4_gather(kv, table, None, None, k, v)
+    at = lambda s, t: buf.as_strided((2, 3, W), (s, t, 1), 8 * W)
+    for out in (buf[:W].expand(2, W), buf.as_strided((2, W), (W - 8, 1))):
+        with pytest.raises(ValueError):
+            attn(out)
+    ok = at(3 * W, W)
+    for bad in (at(0, W), at(3 * W, 0), at(2 * W, W), at(W, W), at(W, 2 * W - 8)):
+        for k, v in ((bad, ok), (ok, bad)):
+            with pytest.raises(ValueError):
+                gather(k, v)
+    attn(buf.as_strided((2, W), (W + 2, 1), 4 * W))
+    attn(buf[4 * W:].as_strided((2, W), (W, 1)))
+    gather(ok, at(W, 2 * W))                                           # sequences inside, tokens outside
+    kv4.kv4_attn(q[:1], two[:1], two[:1], table, kv, geom, buf[4 * W: 5 * W].expand(1, W), 2)
