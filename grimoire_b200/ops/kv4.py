@@ -231,15 +231,23 @@ def kv4_attn(q: torch.Tensor, row_seq: torch.Tensor, row_pos: torch.Tensor, bloc
     """Attention of M rows over the 4-bit pages: row m (bf16 [Hq * D], after norm and RoPE) of sequence slot ``row_seq[m]`` sees
     the cached positions 0 .. ``row_pos[m]``, the last ``geom.window`` of them with a window, and leaves its output (bf16,
     times sigmoid(``gate[m]``) with a gate) in ``out[m]`` (which must not overlap ``q``).  A row that sees no key (a negative position, no mapped page)
-    gives zeros.  Within a block, values below 2^-24 of the largest one that any of its rows sees are rounded to fewer bits (2^-36 of
-    that one at worst).  ``max_len`` is the longest row's ``row_pos + 1`` as the host knows it: it sets how the keys are split, and
+    gives zeros.
+
+    Softmax weights, and codes times their maxima, are fp16 operands (11 bits) of products that are summed in fp32.  Hence: within
+    a block, values below 2^-24 of the largest one that any of its rows sees are rounded to fewer bits (2^-36 of that one at
+    worst); so are, for blocks of many rows and for the observed weight, keys below 2^-24 of the largest one of their page, whether
+    a row sees that one or not.  Keys are served up to a magnitude of 2^64 (scores are held without the query's power of two and
+    would overflow from 2^100 on).
+
+    ``max_len`` is the longest row's ``row_pos + 1`` as the host knows it: it sets how the keys are split, and
     bounds the tokens that ``observe`` covers.
 
     ``block`` > 1: every ``block`` consecutive rows belong to one sequence (the last rows of a prompt, a verify block).
     ``alone``: cut every block's keys as a call of that block alone would (of the same ``max_len``), so that a row's output does
     not depend on the other rows of the call, to the bit.
     ``observe``: "set" or "add" the softmax weight that every token drew from the rows of its sequence in this call, summed
-    over the rows and the query heads of a kv head, to ``kv.mass``; "set" covers all tokens up to the block's last position.
+    over the rows and the query heads of a kv head, to ``kv.mass``; "set" covers all tokens up to the block's last position.  No page
+    may belong to two of the call's sequences then: their sums would race.
     """
     data = kv.data
     P, heads, rec = data.shape

@@ -8,7 +8,7 @@ import torch
 from grimoire_b200.ops import kv4, ref
 from grimoire_b200.ops.core import AttnGeom
 
-from .test_kv4_ops import close, scores_in_range
+from .test_kv4_ops import Cache, close, scores_in_range
 
 PAGE = 16
 
@@ -165,3 +165,27 @@ def test_outputs_whose_rows_share_memory_are_refused(device):
     attn(buf[4 * W:].as_strided((2, W), (W, 1)))
     gather(ok, at(W, 2 * W))                                           # sequences inside, tokens outside
     kv4.kv4_attn(q[:1], two[:1], two[:1], table, kv, geom, buf[4 * W: 5 * W].expand(1, W), 2)
+
+
+# ---------------------------------------------------------------------------------------------
+# the documented range of keys
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("amp", [2.0 ** -64, 2.0 ** 62])
+@pytest.mark.parametrize("block,max_len", [(1, 333), (12, 333), (12, 1 << 20)])
+def test_keys_at_the_ends_of_their_range(device, amp, block, max_len):
+    """Single rows, short blocks and tiles; queries carry the inverse factor, so that scores are of order one."""
+    D, Hkv, G, n = 128, 2, 4, 333
+    c = Cache([n], Hkv, D, device, seed=31, amp=amp)                                  # (normal values: up to four times amp)
+    q = (torch.randn(block, Hkv * G * D, generator=torch.Generator().manual_seed(3)) / amp).bfloat16()
+    pos = list(range(n - block, n))
+    want, size, w, top = c.expect([0] * block, pos, q, G, 0.1)
+    scores_in_range(D, top)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=device)
+    out = torch.zeros(block, Hkv * G * D, dtype=torch.bfloat16, device=device)
+    kv4.kv4_attn(q.to(device), i32([int(c.slots[0])] * block), i32(pos), c.table, c.kv, AttnGeom(Hkv * G, Hkv, D, D, 0.1), out, max_len, block=block,
+                 observe="set")
+    close(out.cpu(), want, size)
+    total = sum(torch.nn.functional.pad(x, (0, n - x.shape[1])) for x in w)
+    eps = 2 * (D + 16) * 2 ** -24 * top + 2 ** -19 + 64 * 2 ** -24                    # as in tiles above; few blocks and parts
+    assert bool(((c.mass_of(0).double() - total).abs() <= eps * total + 1e-35).all())
