@@ -31,8 +31,9 @@ struct AppendParams {
 // kHeads heads of a row a warp: one where there are few rows, four (their loads in flight together, one look into the table) where
 // there are many.
 //
-// Bound by bytes: 4096 rows x 8 heads x 128 (21.5 MB in and out, part of it from L2) take 9.0 us, 2.4 TB/s; one row 1.7 us, which is
-// a launch in a graph.
+// 4096 rows x 8 heads x 128 (21.5 MB in and out, part of it from L2) take 8.9 us, 2.4 TB/s, where the bytes alone take 3.3: a warp
+// loads once, computes and leaves, so the wait for its loads is the largest stall (5.3 an issue; issue slots 60 % busy, integer pipe
+// 49 %).  One row takes 1.8 us, which is a launch in a graph.
 template <int D, int kHeads>
 __global__ void __launch_bounds__(128) append_kernel(const AppendParams p) {
   using G = Geo<D>;
@@ -221,8 +222,10 @@ __device__ __forceinline__ int block_scan(int v, int* warp_sums) {
 // stretch too long for that is read again in every pass).  Radix selection: three passes of 11, 11 and 10 bits over the tokens
 // that are neither among the first `sink` nor the last `recent` find the key of the last token that stays and how many tokens
 // of exactly that key do, the earliest ones; the histograms of the cluster are added through distributed shared memory.  Then
-// every warp writes the kept positions of its own stretch behind those of the stretches before it.  Bound by the barriers between the
-// passes, not by the 4 bytes a token: 2000 tokens x 8 heads take 10 us, eight sequences of up to 32768 27 us, one of 100000 37 us.
+// every warp writes the kept positions of its own stretch behind those of the stretches before it.  2000 tokens x 8 heads take 10 us,
+// the barriers and launch of a few short passes; eight sequences of up to 32768 27 us, one of 100000 37 us, where the 4 bytes a token
+// take 1.3: five walks over the keys in shared memory (issue slots 57 % busy; per issue 2.7 cycles of fixed-latency waits, 2.1 for
+// loads, 1.5 at barriers).
 __global__ void __launch_bounds__(kSelThreads) select_kernel(const SelectParams p, int nctas) {
   extern __shared__ __align__(16) uint32_t keys[];       // [kSelKeys]
   __shared__ int hist[kSelBins];

@@ -311,8 +311,9 @@ __device__ __forceinline__ int stream_schedule(const AttnParams& p, int (&before
 // Softmax statistics, scores and outputs are fp32.
 //
 // Measured (5 heads a kv head of 128, 8 kv heads; merge included): 32 rows of 16384 to 32768 tokens 222 us, 4.1 TB/s, 0.63 of a copy;
-// one row of 131072 tokens 47 us, 3.2 TB/s; 8 rows of 2500 to 4999 21 us.  What is left is the unpacking: of some 350 instructions a warp
-// and page 160 make fp16 operands of 512 codes, and the copies alone take 147 of the 222 us.
+// one row of 131072 tokens 47 us, 3.2 TB/s; 8 rows of 2500 to 4999 21 us.  The copies alone take 147 of the 222 us.  What is left is
+// latency: twelve warps an SM, each with one chain of unpacking (160 of 350 instructions a page), MMA, softmax and MMA.  No pipe is full
+// (issue slots 57 % busy, integer 47 %, tensor 20 %) and the largest stall is the fixed-latency wait.
 template <int D, int HH>
 __global__ void __launch_bounds__(kThreads, Ring<D>::kCtas) attn_kernel(const AttnParams p) {
   using Gm = Geo<D>;
@@ -701,7 +702,8 @@ __global__ void __launch_bounds__(kThreads, Ring<D>::kCtas) attn_kernel(const At
 // token remember the group.  Scores, statistics and outputs are fp32.
 //
 // Four blocks of 32 rows x 40 heads over 8192 to 16384 tokens of 8 kv heads of 128: 138 us with the merge (the kernel above: 250), 0.2
-// PFLOP/s.  Bound by issue slots of unpacking and softmax (3500 a 64 tokens, two CTAs an SM at 2 a cycle) and by the CTAs' start.
+// PFLOP/s.  Bound by the chain of 64 tokens (unpack, S, softmax, P V; 3500 instructions) with two CTAs an SM to overlap, and by the
+// CTAs' start: issue slots are 42 % busy, the tensor pipe 21 %; the stalls are loads, barriers and fixed latencies.
 template <int D>
 struct Tile {
   static constexpr int kTok = 64, kRows = 128, kThreads = 288;
@@ -1217,9 +1219,10 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const AttnParams p
 // Scores are computed once more rather than stored: K is half of the cache, a stored score would be 4 bytes per query head.  A
 // warp takes whole pages; the page's K becomes the MMA's row operand once, (code - 8) / 2 times its group's maximum, which fp16
 // holds exactly (3 + 8 bits), and every tile of 8 (row, head) pairs is one column operand from shared memory: D / 16 MMAs and
-// four exponentials a lane.  Bound by the MMAs (16 cycles of an SM a tile and page at D = 128) and the operands' way out of shared memory
-// where a block has many pairs, by the K bytes where it has few: 160 pairs over four sequences of 8192 to 16384 tokens x 8 kv heads of 128
-// take 81 us, one row's 5 pairs 20 us.  All rows of one sequence are summed by the CTAs of its first block, in the order of the rows:
+// four exponentials a lane.  160 pairs over four sequences of 8192 to 16384 tokens x 8 kv heads of 128 take 82 us: MMAs (16 cycles of an
+// SM a tile and page at D = 128; the tensor pipe is 44 % busy) in a chain behind operands from shared memory.  One row's 5 pairs take
+// 20 us, 1.4 TB/s of K: latency, of the loads of one page at a time a warp and of the CTAs' start (queries, the search for blocks of
+// the same sequence).  All rows of one sequence are summed by the CTAs of its first block, in the order of the rows:
 // two blocks of one sequence neither race nor depend on timing.
 template <int D>
 struct MassTile {
@@ -1418,8 +1421,8 @@ int plan(Plan& pl, long M, long Hq, long Hkv, long D, long block, long max_len, 
   // (row, head) pairs of a CTA: one MMA column tile holds 8.  Two tiles where more pairs than that share the keys, except at
   // head_dim 256, whose accumulators fill the registers with one.
   // Tiles of 128 pairs pay where a block has many and the keys are long enough to carry the wider kernel's start (10 us).  Measured,
-  // us without / with tiles, observed weight included: 160 pairs, 4 x 16384 tokens x 8 kv heads 375 / 269; 512 pairs at head_dim 64,
-  // 2 x 8192 x 4 138 / 109; 96 pairs at head_dim 256, 2 x 8192 x 4 152 / 123; 40 pairs, 4 x 8192 x 8 109 / 106; but 20 pairs of
+  // us without / with tiles, observed weight included: 160 pairs, 4 x 16384 tokens x 8 kv heads 375 / 268; 512 pairs at head_dim 64,
+  // 2 x 8192 x 4 138 / 104; 96 pairs at head_dim 256, 2 x 8192 x 4 152 / 121; 40 pairs, 4 x 8192 x 8 109 / 104; but 20 pairs of
   // those 94 / 102, 40 pairs, 8192 x 8 56 / 61, 80 pairs, 2001 x 8 44 / 50.
   const long key_pages = (max_len + kPage - 1) / kPage;
   // alone: as in a call of one block, in this as in the cut of the keys below
