@@ -354,8 +354,8 @@ def kv4_select(kv: Kv4Layer, slots: Optional[torch.Tensor], lengths: torch.Tenso
 def kv4_compact(kv: Kv4Layer, slots: Optional[torch.Tensor], idx: torch.Tensor, block_table: torch.Tensor, dst_table: torch.Tensor) -> None:
     """Copy token ``idx[i][h][j]`` of sequence ``slots[i]`` (kv head h, codes, maxima and mass as they are) to place j of the
     pages ``dst_table[i]`` (int32 [S][>= ceil(keep / 16)]).  The destination pages must not be among the sources, nor come twice:
-    pages that other sequences share stay intact, and the caller swaps the tables afterwards.  Places whose ``idx`` is -1 stay as they
-    are."""
+    pages that other sequences share stay intact, and the caller swaps the tables afterwards.  Places whose ``idx`` is -1, or whose token
+    has no page (``kv4_select`` takes such a token only where too few others are left), stay as they are."""
     data = kv.data
     P, Hkv, rec = data.shape
     dev, what = data.get_device(), "kv4_compact"

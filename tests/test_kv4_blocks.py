@@ -189,3 +189,24 @@ def test_keys_at_the_ends_of_their_range(device, amp, block, max_len):
     total = sum(torch.nn.functional.pad(x, (0, n - x.shape[1])) for x in w)
     eps = 2 * (D + 16) * 2 ** -24 * top + 2 ** -19 + 64 * 2 ** -24                    # as in tiles above; few blocks and parts
     assert bool(((c.mass_of(0).double() - total).abs() <= eps * total + 1e-35).all())
+
+
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+def test_places_of_kept_tokens_without_a_page_stay(device):
+    """Selection puts tokens of an unmapped page last; where they are kept all the same, their places are not written."""
+    c = Cache([64], 2, 64, device, seed=8, spare=6)
+    slot = int(c.slots[0])
+    c.kv.mass.copy_(torch.rand(c.kv.mass.shape, generator=torch.Generator().manual_seed(3)) + 1)
+    c.table[slot, 1] = -1                                              # tokens 16 .. 31
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=device)
+    idx = kv4.kv4_select(c.kv, i32(slot), i32(64), c.table, 50, 0, 0)
+    want = list(range(18)) + list(range(32, 64))                       # the 48 that exist, and the two earliest of the others
+    assert idx[0].tolist() == [want, want]
+    fresh = c.fresh[:4][None].contiguous()
+    c.kv.data[fresh[0].long()] = 0x5a
+    c.kv.mass[fresh[0].long()] = 7
+    kv4.kv4_compact(c.kv, i32(slot), idx, c.table, fresh)
+    mass = c.kv.mass[fresh[0].long()].transpose(1, 2).reshape(64, 2).cpu()
+    assert bool((mass[[16, 17] + list(range(50, 64))] == 7).all()) and bool((mass[:16] < 2).all()) and bool((mass[18:50] < 2).all())
+    codes, _ = ref.kv4_views(c.kv.data[fresh[0].long()].cpu())
+    assert bool((codes[1, :, :, :2] == 0x5a).all()) and bool((codes[3, :, :, 2:] == 0x5a).all())
