@@ -296,8 +296,8 @@ __device__ __forceinline__ int stream_schedule(const AttnParams& p, int (&before
 
 // Attention of up to 8 * HH (row, head) pairs of one kv head over one split of the sequence's pages.
 //
-// Bound by the cache's bytes (18 D per 16 tokens and kv head) and, close behind, by issue slots (a record has to cost a warp less
-// than four times the ~100 cycles in which an SM receives it), of them most by the integer pipe that unpacks the codes.  Hence
+// It has to keep up with the cache's bytes (18 D per 16 tokens and kv head): a record may cost a
+// warp no more issue slots than four times the ~100 cycles in which an SM receives it, and unpacking takes most of them.  Hence
 //   * a warp owns steps of two pages (32 tokens); a page is ONE bulk copy (the record is contiguous) into a per-warp ring;
 //   * S^T[token][pair] = K Q^T with the codes, as the fp16 integers that they are, as the MMA's row operand: 16 tokens fill its
 //     rows and 8 pairs its columns.  q is scaled by a power of two to fill fp16's range (bf16 has fewer bits: exact); a
