@@ -210,3 +210,31 @@ def test_places_of_kept_tokens_without_a_page_stay(device):
     assert bool((mass[[16, 17] + list(range(50, 64))] == 7).all()) and bool((mass[:16] < 2).all()) and bool((mass[18:50] < 2).all())
     codes, _ = ref.kv4_views(c.kv.data[fresh[0].long()].cpu())
     assert bool((codes[1, :, :, :2] == 0x5a).all()) and bool((codes[3, :, :, 2:] == 0x5a).all())
+
+
+@pytest.mark.gpu
+def test_deep_tiles_on_two_streams_at_once_captured_and_not():
+    """Tiles of two head dimensions share the multiprocessors (and their TMEM): replayed on one stream, called on another, the bits stay."""
+    jobs = []
+    for D, seqs in ((128, 38), (256, 19)):
+        c, q, pos = deep_case(D, 8, 8, seqs, seed=D)
+        seq = torch.arange(seqs, dtype=torch.int32, device="cuda").repeat_interleave(8)
+        out = torch.empty_like(q)
+
+        def run(c=c, q=q, pos=pos, seq=seq, out=out, D=D):
+            kv4.kv4_attn(q, seq, pos, c.table, c.kv, AttnGeom(c.Hkv * 8, c.Hkv, D, D, 1 / math.sqrt(D)), out, max(c.lens), block=8, observe="set")
+
+        run()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            run()
+        jobs.append((run, g, out, c, out.clone(), c.kv.mass.clone()))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for i in range(40):
+        for j, (run, g, out, c, _, _) in enumerate(jobs):
+            with torch.cuda.stream(streams[j]):
+                g.replay() if (i + j) % 2 else run()
+    torch.cuda.synchronize()
+    for _, _, out, c, want, mass in jobs:
+        assert torch.equal(out, want) and torch.equal(c.kv.mass, mass)
