@@ -205,3 +205,23 @@ def test_replayed_steps_count_their_rows_once():
         eng.decode_rows([1], [s], [40 + i], use_graph=True)
         eng.commit_rows([s], [1], [40 + i])
         assert abs(float(_mass(eng, s).sum()) - before - rows) < 2 ** -9 * rows
+
+
+def test_a_loaded_model_whose_cache_is_cut_drafts_nothing():
+    """The loader's defaults (copy drafts on) with a cut cache: single requests and the scheduler work and draft nothing; limits that
+    cannot hold the cut are refused at load."""
+    from grimoire_b200.api import Grimoire
+    from grimoire_b200.config import EngineConfig
+    from grimoire_b200.engine.generation import SpecStats
+
+    ec = dict(model="synthetic:tiny_dense", seq_slots=2, prefill_chunk=64, kv_bits=4, kv_keep=32)
+    g = Grimoire.load(EngineConfig(ctx=320, **ec), device="cpu")
+    assert "speculation: off" in g.banner()
+    st, p = SpecStats(), _prompt(10, 5) * 3
+    toks, _ = g.generate(p, 20, draft_depth=3, stats=st)
+    out = g.generate_batch([p, p[:17]], 20)
+    assert len(toks) == 20 and st.rounds == 0 and out[0][0] == toks and len(out[1][0]) == 20
+    assert g.scheduler().metrics["spec_rounds"] == 0
+    g.close()
+    with pytest.raises(ValueError):
+        Grimoire.load(EngineConfig(ctx=256, **ec), device="cpu")
